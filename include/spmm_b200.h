@@ -358,6 +358,116 @@ int spmm_hem_hierarchy(int64_t rows, int64_t cols, const int64_t *indptr, const 
                        int32_t feasible_first, int64_t *labels, int64_t *levels, int64_t level_slots,
                        int64_t *n_levels, spmm_stream_t stream);
 
+/* ---- dense, grouped and routed products ---------------------------------
+ * No counterpart in the reference.  Products of 16-bit operands (bfloat16 or
+ * float16, sums in float32, each output rounded once):
+ *
+ *     y[r] = act(x[r] * w[g] + bias[g]) + residual[r]     for the rows r of group g
+ *
+ * Rows offsets[g] .. offsets[g+1] belong to group g (offsets: groups + 1
+ * device int32, offsets[0] = 0, non-decreasing, at most `rows`); without
+ * offsets all rows are one group (groups = 1).  Rows behind the last group are
+ * written as zeros.  With `gather`, row r of the product reads x[gather[r]]
+ * (a value outside [0, x_rows) reads a row of zeros).  Sizes may be anything,
+ * zero included; groups <= SPMM_MAX_GROUPS.  Strides are in elements; x, y,
+ * residual, dy, dx have unit stride along their columns, w and dw along k or
+ * along n.  16-byte aligned operands whose strides are multiples of 8 are read
+ * in place; others are copied into the workspace first. */
+enum spmm_dense_type { SPMM_DENSE_F32 = 0, SPMM_DENSE_BF16 = 2, SPMM_DENSE_F16 = 3 };
+enum spmm_activation { SPMM_ACT_NONE = 0, SPMM_ACT_RELU = 1, SPMM_ACT_GELU = 2 /* erf */,
+                       SPMM_ACT_GELU_TANH = 3, SPMM_ACT_SILU = 4 };
+enum { SPMM_MAX_GROUPS = 1024, SPMM_MAX_TOP = 32 };
+
+typedef struct {
+    int32_t version;            /* 1 */
+    int32_t dtype;              /* enum spmm_dense_type: BF16 or F16 */
+    int32_t activation;         /* enum spmm_activation (forward) */
+    int32_t wait_us;            /* bounded device waits: 0 = about 2 s, else at least 1000 */
+    int64_t rows, k, n, groups; /* rows of y */
+    int64_t x_rows;             /* rows of x (== rows without gather) */
+    const int32_t *offsets;     /* groups + 1, or NULL: one group */
+    const int32_t *gather;      /* rows, or NULL */
+    const int32_t *slots;       /* backward with gather: [x_rows][top], the rows of the product that */
+    int64_t top;                /*   read each row of x (-1: none) */
+    const void *x;              /* [x_rows][k] */
+    const void *w;              /* [groups][k][n] */
+    const void *bias;           /* [groups][n] or NULL */
+    const void *residual;       /* [rows][n] or NULL */
+    void *y;                    /* [rows][n] (forward output) */
+    int16_t *slope;             /* [rows][n] contiguous, or NULL: act'(z) in units of 2^-14, written by
+                                 * the forward, read by the backward (NULL there: act' = 1) */
+    const void *dy;             /* backward: [rows][n] */
+    void *dx;                   /* backward outputs, each or NULL: [x_rows][k], */
+    void *dw;                   /*   [groups][k][n], */
+    void *dbias;                /*   [groups][n] */
+    int64_t x_ld, w_k, w_n, w_g, bias_g, residual_ld, y_ld, dy_ld, dx_ld, dw_k, dw_n, dw_g, dbias_g;
+    void *workspace;            /* device scratch, 256-byte aligned, *_workspace_size() bytes */
+    uint64_t workspace_bytes;
+    int32_t *status;            /* device int32: 0, or SPMM_ETIMEOUT when a bounded wait expired */
+} spmm_linear;
+
+/* Forward product; backward: dz = dy * act'(z), dx[r] = dz[r] * w[g]^T (summed over the rows that read
+ * the same row of x), dw[g] = sum x[r]^T dz[r], dbias[g] = sum dz[r] (zero for empty groups).  dz is
+ * rounded to the operands' type for the two products unless act' = 1.  Deterministic. */
+size_t spmm_linear_forward_workspace_size(const spmm_linear *p);
+int spmm_linear_forward(const spmm_linear *p, spmm_stream_t stream);
+size_t spmm_linear_backward_workspace_size(const spmm_linear *p);
+int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream);
+
+/* Expert choice.  Of each token's `experts` logits the `top` largest by float32(logit) + bias are chosen,
+ * best first, ties to the lowest index; a -inf or NaN sum is never chosen (+inf counts as the largest
+ * float).  Weights: softmax over all logits (-inf and NaN count as zero) or sigmoid, times `scale`, of the
+ * chosen ones, divided by their sum with `renormalize`; 0 where nothing was left to choose (expert -1).
+ * The choices are then grouped by expert, tokens ascending: offsets[e] is the first position of expert e,
+ * rows[p] the token at position p (-1 behind the last group), slots[t][j] the position of a choice (-1:
+ * none).  experts <= 1024, top <= min(experts, SPMM_MAX_TOP), tokens * top < 2^31. */
+enum spmm_scoring { SPMM_SCORE_SOFTMAX = 0, SPMM_SCORE_SIGMOID = 1 };
+typedef struct {
+    int32_t version;            /* 1 */
+    int32_t dtype;              /* enum spmm_dense_type of logits and dlogits */
+    int32_t scoring, renormalize;
+    int64_t tokens, experts, top;
+    const void *logits;         /* [tokens][experts] */
+    int64_t logits_ld;
+    const float *bias;          /* [experts] or NULL */
+    float scale;
+    int32_t reserved;
+    float *weights;             /* [tokens][top] */
+    int32_t *experts_out;       /* [tokens][top] */
+    int32_t *slots;             /* [tokens][top] */
+    int32_t *rows;              /* [tokens * top] */
+    int32_t *offsets;           /* [experts + 1] */
+    const float *dweights;      /* backward: [tokens][top]; reads logits and experts_out */
+    void *dlogits;              /* backward: [tokens][experts] contiguous */
+    void *workspace;
+    uint64_t workspace_bytes;
+} spmm_route_args;
+size_t spmm_route_workspace_size(const spmm_route_args *p);
+int spmm_route(const spmm_route_args *p, spmm_stream_t stream);
+int spmm_route_backward(const spmm_route_args *p, spmm_stream_t stream);
+
+/* Weighted sums back in token order: out[t] = sum_j weights[t][j] * y[slots[t][j]] + residual[t] (slots
+ * outside [0, rows) are left out; sums in float32, one rounding).  backward: dy[slots[t][j]] =
+ * weights[t][j] * dout[t] (rows behind offsets[experts] zero) and dweights[t][j] = <dout[t],
+ * y[slots[t][j]]> (0 where there is no slot). */
+typedef struct {
+    int32_t version;            /* 1 */
+    int32_t dtype;              /* enum spmm_dense_type: BF16, F16 or F32 */
+    int64_t tokens, top, rows, n, experts;
+    const int32_t *slots;       /* [tokens][top] */
+    const int32_t *offsets;     /* [experts + 1] (backward) */
+    const float *weights;       /* [tokens][top] */
+    const void *y;              /* [rows][n] */
+    const void *residual;       /* [tokens][n] or NULL */
+    void *out;                  /* [tokens][n] */
+    const void *dout;           /* [tokens][n] */
+    void *dy;                   /* [rows][n] or NULL */
+    float *dweights;            /* [tokens][top] or NULL */
+    int64_t y_ld, residual_ld, out_ld, dout_ld, dy_ld;
+} spmm_combine_args;
+int spmm_combine(const spmm_combine_args *p, spmm_stream_t stream);
+int spmm_combine_backward(const spmm_combine_args *p, spmm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,9 +20,15 @@ from .pbr import (BlockFillStats, BlockStripeStats, DataOrder, PBRInfo, PBRMatri
                   pbr_batched_matmul_cuda, pbr_batched_matmul_nnzflat_cuda,
                   pbr_batched_matmul_variant_cuda, pbr_info, pbr_matmul, pbr_to_csr)
 from ._lib import SpmmError
+from .linear import (ACTIVATIONS, dense_matmul, dense_matmul_backward, grouped_matmul,
+                     grouped_matmul_backward)
+from .route import (SCORINGS, Routing, route_combine, route_combine_backward, route_topk,
+                    route_topk_backward)
 from .timed import BOOTimedSpMM, DirectSpMM, PBRTimedSpMM
 
 __all__ = [
+    'dense_matmul', 'dense_matmul_backward', 'grouped_matmul', 'grouped_matmul_backward', 'ACTIVATIONS',
+    'Routing', 'route_topk', 'route_topk_backward', 'route_combine', 'route_combine_backward', 'SCORINGS',
     'csr_to_boo', 'boo_to_csr', 'boo_info', 'boo_matmul', 'boo_arena_bytes', 'BOOInfo',
     'product_status', 'check_product', 'SpmmError',
     'SMALL_BLOCK_POLICIES', 'NZ_ORDERS', 'cluster_axes', 'cluster_axis', 'CLUSTER_METHODS',

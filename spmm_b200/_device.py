@@ -3,6 +3,7 @@ raw pointers of torch tensors, the caller's CUDA stream."""
 
 from __future__ import annotations
 
+import contextlib
 import threading
 
 import numpy as np
@@ -78,6 +79,13 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current one; nothing when it is already."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 NP_TO_TORCH = {np.dtype(np.float32): torch.float32, np.dtype(np.float64): torch.float64,

@@ -39,7 +39,9 @@ EXPORTS = ('spmm_status_string', 'spmm_abi_version', 'spmm_boo_build_workspace_s
            'spmm_boo_to_csr_workspace_size', 'spmm_boo_to_csr', 'spmm_pbr_to_csr_workspace_size',
            'spmm_pbr_to_csr', 'spmm_hem_labels', 'spmm_hem_level_slots', 'spmm_hem_hierarchy',
            'spmm_boo_matmul_groups', 'spmm_boo_plan_size', 'spmm_boo_plan_workspace_size',
-           'spmm_boo_plan_build')
+           'spmm_boo_plan_build', 'spmm_linear_forward_workspace_size', 'spmm_linear_forward',
+           'spmm_linear_backward_workspace_size', 'spmm_linear_backward', 'spmm_route_workspace_size',
+           'spmm_route', 'spmm_route_backward', 'spmm_combine', 'spmm_combine_backward')
 
 
 class CsrDev(C.Structure):
@@ -92,6 +94,38 @@ def launch_cfg(engine: str = 'auto', workspace: int = 0, workspace_bytes: int = 
         raise ValueError(f"engine must be one of {sorted(ENGINES)}, got {engine!r}")
     return LaunchCfg(2, int(slab_features), ENGINES[engine], int(wait_us), workspace or None, workspace_bytes,
                      status or None, int(flags), 0, plan or None)
+
+
+DENSE_F32, DENSE_BF16, DENSE_F16 = 0, 2, 3
+MAX_GROUPS, MAX_TOP = 1024, 32
+
+
+class Linear(C.Structure):
+    _fields_ = ([('version', C.c_int32), ('dtype', C.c_int32), ('activation', C.c_int32), ('wait_us', C.c_int32)]
+                + [(n, C.c_int64) for n in ('rows', 'k', 'n', 'groups', 'x_rows')]
+                + [(n, C.c_void_p) for n in ('offsets', 'gather', 'slots')] + [('top', C.c_int64)]
+                + [(n, C.c_void_p) for n in ('x', 'w', 'bias', 'residual', 'y', 'slope', 'dy', 'dx', 'dw', 'dbias')]
+                + [(n, C.c_int64) for n in ('x_ld', 'w_k', 'w_n', 'w_g', 'bias_g', 'residual_ld', 'y_ld', 'dy_ld',
+                                            'dx_ld', 'dw_k', 'dw_n', 'dw_g', 'dbias_g')]
+                + [('workspace', C.c_void_p), ('workspace_bytes', C.c_uint64), ('status', C.c_void_p)])
+
+
+class RouteArgs(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ('version', 'dtype', 'scoring', 'renormalize')]
+                + [(n, C.c_int64) for n in ('tokens', 'experts', 'top')]
+                + [('logits', C.c_void_p), ('logits_ld', C.c_int64), ('bias', C.c_void_p), ('scale', C.c_float),
+                   ('reserved', C.c_int32)]
+                + [(n, C.c_void_p) for n in ('weights', 'experts_out', 'slots', 'rows', 'offsets', 'dweights',
+                                             'dlogits', 'workspace')]
+                + [('workspace_bytes', C.c_uint64)])
+
+
+class CombineArgs(C.Structure):
+    _fields_ = ([('version', C.c_int32), ('dtype', C.c_int32)]
+                + [(n, C.c_int64) for n in ('tokens', 'top', 'rows', 'n', 'experts')]
+                + [(n, C.c_void_p) for n in ('slots', 'offsets', 'weights', 'y', 'residual', 'out', 'dout', 'dy',
+                                             'dweights')]
+                + [(n, C.c_int64) for n in ('y_ld', 'residual_ld', 'out_ld', 'dout_ld', 'dy_ld')])
 
 
 class SpmmError(RuntimeError):
@@ -167,6 +201,17 @@ def lib() -> C.CDLL:
                                          C.c_void_p, C.c_int64, C.POINTER(C.c_int64), C.c_void_p]
         L.spmm_hem_hierarchy.restype = C.c_int
         L.spmm_pbr_to_csr.restype = C.c_int
+        for n in ('spmm_linear_forward', 'spmm_linear_backward'):
+            getattr(L, n).argtypes = [C.POINTER(Linear), C.c_void_p]
+            getattr(L, n).restype = C.c_int
+            getattr(L, n + '_workspace_size').argtypes = [C.POINTER(Linear)]
+            getattr(L, n + '_workspace_size').restype = C.c_size_t
+        L.spmm_route_workspace_size.argtypes = [C.POINTER(RouteArgs)]
+        L.spmm_route_workspace_size.restype = C.c_size_t
+        for n, t in (('spmm_route', RouteArgs), ('spmm_route_backward', RouteArgs), ('spmm_combine', CombineArgs),
+                     ('spmm_combine_backward', CombineArgs)):
+            getattr(L, n).argtypes = [C.POINTER(t), C.c_void_p]
+            getattr(L, n).restype = C.c_int
         for n in ('spmm_boo_build_analyze', 'spmm_boo_build_emit', 'spmm_pbr_build_analyze',
                   'spmm_pbr_build_emit', 'spmm_boo_matmul', 'spmm_pbr_matmul'):
             getattr(L, n).restype = C.c_int

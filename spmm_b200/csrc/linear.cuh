@@ -1,0 +1,169 @@
+// linear.cuh -- shared parts of the dense, grouped and routed products.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace spmm {
+
+constexpr float kSlopeUnit = 1.f / 16384.f;   // of the 16-bit fixed-point act'(z)
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+
+// 8 16-bit values (16 bytes) as floats and back.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 &v, float (&f)[8]) {
+    T t[8];
+    memcpy(t, &v, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(t[i]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(f[i]);
+    uint4 v;
+    memcpy(&v, t, 16);
+    return v;
+}
+
+// First row of group g (offsets clamped into [0, total], so a wrong table reads and writes nothing outside).
+__device__ __forceinline__ int64_t group_first(const int32_t *offsets, int64_t g, int64_t total) {
+    const int64_t o = __ldg(offsets + g);
+    return o < 0 ? 0 : o > total ? total : o;
+}
+
+// A tile of up to `size` consecutive rows of one group; group == groups is the
+// tail of rows behind the last group, group > groups no tile.
+struct RowTile {
+    int64_t group, first;
+    int rows;
+};
+
+// The t-th tile when every group's rows (and then the tail's) are cut into
+// tiles of `size` rows.  Called by a whole warp; a prefix sum over 32 groups
+// at a time.
+__device__ __forceinline__ RowTile find_row_tile(const int32_t *offsets, int64_t groups, int64_t total, int size,
+                                                 int64_t t) {
+    RowTile r{groups + 1, 0, 0};
+    if (offsets == nullptr) {
+        if (t * size < total) {
+            const int64_t left = total - t * size;
+            r = RowTile{0, t * size, (int)(left < size ? left : size)};
+        }
+        return r;
+    }
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int64_t g0 = 0; g0 <= groups; g0 += 32) {
+        const int64_t g = g0 + lane;
+        int64_t a = 0, b = 0;
+        if (g <= groups) {
+            a = group_first(offsets, g, total);
+            b = g < groups ? group_first(offsets, g + 1, total) : total;
+            if (b < a) b = a;
+        }
+        const int64_t tiles = (b - a + size - 1) / size;
+        int64_t incl = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(kFullMask, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const unsigned past = __ballot_sync(kFullMask, before + incl > t);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const int64_t first = a + (t - before - (incl - tiles)) * size;
+            const int64_t left = b - first;
+            r.group = g0 + l;
+            r.first = __shfl_sync(kFullMask, first, l);
+            r.rows = (int)__shfl_sync(kFullMask, left < size ? left : (int64_t)size, l);
+            return r;
+        }
+        before += __shfl_sync(kFullMask, incl, 31);
+    }
+    return r;
+}
+
+// The activation and its derivative at z.  Both are bounded functions of z in
+// float32: exp and erf go through the CUDA library, 1/(1 + exp) cannot
+// overflow to NaN (exp(-z) = inf gives 0).
+struct ActValue {
+    float y, slope;
+};
+template <int ACT>
+__device__ __forceinline__ ActValue activate(float z) {
+    if constexpr (ACT == SPMM_ACT_RELU) {
+        return {z > 0.f ? z : (z != z ? z : 0.f), z > 0.f ? 1.f : 0.f};
+    } else if constexpr (ACT == SPMM_ACT_SILU) {
+        if (z == -INFINITY) return {0.f, 0.f};   // the limits; z * 0 would be NaN
+        const float s = 1.f / (1.f + expf(-z));
+        const float rest = z == INFINITY ? 0.f : z * (1.f - s);
+        return {z * s, s * (1.f + rest)};
+    } else if constexpr (ACT == SPMM_ACT_GELU) {
+        if (z == -INFINITY) return {0.f, 0.f};
+        const float cdf = 0.5f * erfcf(z * -0.70710678118654752f);
+        const float pdf = 0.3989422804014327f * expf(-0.5f * z * z);
+        return {z * cdf, cdf + (pdf > 0.f ? z * pdf : 0.f)};
+    } else if constexpr (ACT == SPMM_ACT_GELU_TANH) {
+        // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u))
+        if (z == -INFINITY) return {0.f, 0.f};
+        const float z2 = z * z;
+        const float u2 = 1.5957691216057308f * z * (1.f + 0.044715f * z2);
+        const float s = 1.f / (1.f + expf(-u2));
+        const float r = s * (1.f - s) * 1.5957691216057308f;
+        return {z * s, s + (r > 0.f ? z * r * (1.f + 0.134145f * z2) : 0.f)};
+    } else {
+        return {z, 1.f};
+    }
+}
+
+// act'(z) in 16 bits.  It lies within (-2, 2), so fixed point in units of 2^-14
+// (off by at most 2^-15) keeps 4 to 30 times more of it than a 16-bit float
+// would; -32768 stands for NaN.
+__device__ __forceinline__ int16_t slope_code(float s) {
+    return s != s ? (int16_t)-32768 : (int16_t)__float2int_rn(s * 16384.f);
+}
+__device__ __forceinline__ float slope_value(int16_t c) {
+    return c == -32768 ? __int_as_float(0x7fc00000) : (float)c * kSlopeUnit;
+}
+
+// One product D[p][q] = sum_r A[p][r] * B[q][r], stored as C[q * c_q + p].
+//   ragged rows (red == 0): q runs over the rows of all groups, group g's rows
+//     use A + g * a_g; epilogue bias, activation, slope, residual.
+//   ragged sums (red == 1): r runs over the rows of group g, for every group.
+struct Product {
+    int64_t P, Q, R;             // Q (red == 0) or R (red == 1) counts the rows of all groups
+    int64_t groups;
+    const int32_t *offsets;      // null: one group
+    int32_t red, act, f16, out_f32;
+    const void *A, *B;
+    int64_t a_p, a_r, a_g, b_q, b_r;   // one of (a_p, a_r) and of (b_q, b_r) is 1
+    void *C;
+    int64_t c_q, c_g;
+    const void *bias;
+    int64_t bias_g;
+    const void *residual;
+    int64_t residual_ld;
+    int16_t *slope;              // [Q][P]
+    int32_t *status;
+    int64_t wait_cycles;
+};
+
+int launch_product(const Product &p, cudaStream_t s);
+
+// out[t] = sum_j weight * src[slots[t][j]] over float32 rows (the gradient of gathered rows).
+int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,
+                      void *out, int64_t out_ld, int f16, cudaStream_t s);
+
+}  // namespace spmm

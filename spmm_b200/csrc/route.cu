@@ -1,0 +1,630 @@
+// route.cu -- expert choice, the grouping of the chosen rows, and the weighted
+// sums back in token order.
+//
+// Choice.  A warp per token holds the token's logits in registers (expert e in
+// lane e % 32); top rounds of a warp-wide maximum over order-preserving 32-bit
+// keys, ties resolved to the lowest expert by a second reduction.  The choice
+// depends on float32(logit) + bias alone, so it is exact; weights come from
+// float32 exponentials relative to the row's maximum.
+//
+// Grouping.  A stable counting sort by expert: tokens are cut into chunks, a
+// CTA counts its chunk's choices per expert, one pass turns the counts into
+// first positions, and a CTA per chunk places its choices in order (ranks
+// within a warp by match, warps by a prefix over their counts).  Integer sums
+// only: the result does not depend on the order of the atomics.
+#include "linear.cuh"
+
+namespace spmm {
+namespace {
+
+constexpr int kWarps = 8;                  // warps of a routing CTA
+constexpr int kMaxExperts = SPMM_MAX_GROUPS;
+constexpr uint32_t kNone = 0x007FFFFFu;    // key of -inf: not selectable, like every smaller key
+
+// Order-preserving key: a < b as floats <=> key(a) < key(b); -0 counts as +0, NaN as -inf.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    if (v != v) return kNone;
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// A logit as the weights use it: +inf as the largest float, NaN as -inf.
+__device__ __forceinline__ float clean_logit(float v) {
+    return v != v ? -INFINITY : fminf(v, 3.402823466e38f);
+}
+
+struct Row {
+    float peak;    // softmax: largest logit (0 when there is none)
+    float total;   // softmax: sum of exp(logit - peak)
+};
+
+template <int V>
+__device__ __forceinline__ Row softmax_row(const float (&l)[V]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m = fmaxf(m, l[v]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+    if (m == -INFINITY) m = 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) s += expf(l[v] - m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+    return {m, s};
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T *row, int experts, int lane, float (&l)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int e = v * 32 + lane;
+        l[v] = e < experts ? to_f32(row[e]) : -INFINITY;
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+
+// One token: lane j < top ends with choice j in (expert, weight).
+template <typename T, int V>
+__device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int lane, int &expert, float &weight) {
+    const int experts = (int)p.experts, top = (int)p.top;
+    float l[V];
+    load_row<T, V>((const T *)p.logits + t * p.logits_ld, experts, lane, l);
+    uint32_t key[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int e = v * 32 + lane;
+        key[v] = e >= experts ? 0u : order_key(p.bias ? l[v] + __ldg(p.bias + e) : l[v]);
+        l[v] = clean_logit(l[v]);
+    }
+    expert = -1;
+    float mine = -INFINITY;   // the logit of this lane's choice
+    for (int j = 0; j < top; ++j) {
+        uint32_t best = 0u;
+        int at = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (key[v] > best) {
+                best = key[v];
+                at = v;
+            }
+        const uint32_t m = __reduce_max_sync(kFullMask, best);
+        if (m <= kNone) break;
+        const int e = (int)__reduce_min_sync(kFullMask, best == m ? (unsigned)(at * 32 + lane) : ~0u);
+        float val = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (v * 32 + lane == e) {
+                key[v] = 0u;
+                val = l[v];
+            }
+        val = __shfl_sync(kFullMask, val, e & 31);
+        if (lane == j) {
+            expert = e;
+            mine = val;
+        }
+    }
+    // weights
+    if (p.scoring == SPMM_SCORE_SOFTMAX) {
+        Row r;
+        if (p.renormalize) {   // relative to the chosen ones alone
+            float c[1] = {expert >= 0 ? mine : -INFINITY};
+            r = softmax_row<1>(c);
+        } else {
+            r = softmax_row<V>(l);
+        }
+        weight = expert >= 0 && r.total > 0.f ? expf(mine - r.peak) / r.total : 0.f;
+    } else {
+        weight = expert >= 0 ? sigmoid(mine) : 0.f;
+        if (p.renormalize) {
+            float s = weight;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+            weight = s > 0.f ? weight / s : 0.f;
+        }
+    }
+    weight *= p.scale;
+}
+
+// Choices of the tokens [t0, t1) of this CTA, and their counts per expert in `count`.
+template <typename T, int V>
+__device__ __forceinline__ void choose_chunk(const spmm_route_args &p, int64_t t0, int64_t t1, int *count) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (int64_t t = t0 + warp; t < t1; t += warps) {
+        int e;
+        float w;
+        choose<T, V>(p, t, lane, e, w);
+        if (lane < p.top) {
+            p.weights[t * p.top + lane] = w;
+            p.experts_out[t * p.top + lane] = e;
+            if (e >= 0) atomicAdd(count + e, 1);
+        }
+    }
+}
+
+// Exclusive prefix sums of v[0, n) in place, the total returned; the whole CTA.
+__device__ __forceinline__ int cta_exclusive(int *v, int n, int *tmp /* 33 */) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int carry = 0;
+    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x;
+        const int x = i < n ? v[i] : 0;
+        int s = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(kFullMask, s, o);
+            if (lane >= o) s += y;
+        }
+        if (lane == 31) tmp[warp] = s;
+        __syncthreads();
+        if (warp == 0) {
+            const int own = lane < warps ? tmp[lane] : 0;
+            int b = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(kFullMask, b, o);
+                if (lane >= o) b += y;
+            }
+            tmp[lane] = b - own;
+            if (lane == 31) tmp[32] = b;
+        }
+        __syncthreads();
+        if (i < n) v[i] = carry + tmp[warp] + s - x;
+        carry += tmp[32];
+        __syncthreads();
+    }
+    return carry;
+}
+
+// Places the choices [i0, i1) (flat, in order) of this CTA: base[e] is the position of the chunk's first choice
+// of expert e.  `wcount`: [warps][experts].  Each warp owns a contiguous part.
+__device__ __forceinline__ void place(const spmm_route_args &p, int64_t i0, int64_t i1, const int *base,
+                                      int *wcount) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int experts = (int)p.experts;
+    const int64_t part = ((i1 - i0 + warps - 1) / warps + 31) / 32 * 32;
+    const int64_t a = i0 + warp * part, b = a + part < i1 ? a + part : i1;
+    int *mine = wcount + warp * experts;
+    for (int e = lane; e < experts; e += 32) mine[e] = 0;
+    __syncwarp();
+    for (int64_t i = a + lane; i < b; i += 32) {
+        const int e = p.experts_out[i];
+        if (e >= 0) atomicAdd(mine + e, 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        int run = base[e];
+        for (int w = 0; w < warps; ++w) {
+            const int c = wcount[w * experts + e];
+            wcount[w * experts + e] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+    for (int64_t i = a; i < b; i += 32) {   // a and the loop bound are the same for the whole warp
+        const bool in = i + lane < b;
+        const int e = in ? p.experts_out[i + lane] : -1;
+        const unsigned same = __match_any_sync(kFullMask, e);
+        const int rank = __popc(same & lanemask_lt());
+        int pos = -1;
+        if (e >= 0) pos = mine[e] + rank;
+        __syncwarp();
+        if (e >= 0 && rank == 0) mine[e] += __popc(same);
+        __syncwarp();
+        if (in) {
+            p.slots[i + lane] = pos;
+            if (pos >= 0) p.rows[pos] = (int32_t)((i + lane) / p.top);
+        }
+    }
+}
+
+// Everything in one CTA: for few tokens, where launches are what it costs.
+template <typename T, int V>
+__global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_route_args p) {
+    extern __shared__ int sm[];
+    __shared__ int tmp[33];
+    const int experts = (int)p.experts;
+    int *count = sm, *wcount = sm + experts;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) count[e] = 0;
+    __syncthreads();
+    choose_chunk<T, V>(p, 0, p.tokens, count);
+    __syncthreads();
+    const int total = cta_exclusive(count, experts, tmp);
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) p.offsets[e] = count[e];
+    if (threadIdx.x == 0) p.offsets[experts] = total;
+    const int64_t all = p.tokens * p.top;
+    for (int64_t i = total + threadIdx.x; i < all; i += blockDim.x) p.rows[i] = -1;
+    place(p, 0, all, count, wcount);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kWarps * 32) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
+    extern __shared__ int sm[];
+    const int experts = (int)p.experts;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) sm[e] = 0;
+    __syncthreads();
+    const int64_t t0 = blockIdx.x * chunk, t1 = t0 + chunk < p.tokens ? t0 + chunk : p.tokens;
+    choose_chunk<T, V>(p, t0, t1, sm);
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[(int64_t)blockIdx.x * experts + e] = sm[e];
+}
+
+// counts[chunk][e] -> the chunk's choices of e before it; totals[e].  A CTA per 32 experts, a warp per run of chunks.
+__global__ void __launch_bounds__(1024) route_scan_kernel(int *counts, int chunks, int experts, int *totals) {
+    __shared__ int part[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int e = blockIdx.x * 32 + lane;
+    const int per = (chunks + 31) / 32, a = warp * per, b = a + per < chunks ? a + per : chunks;
+    int s = 0;
+    if (e < experts)
+        for (int c = a; c < b; ++c) s += counts[(int64_t)c * experts + e];
+    part[warp][lane] = s;
+    __syncthreads();
+    int run = 0;
+    for (int w = 0; w < warp; ++w) run += part[w][lane];
+    if (e < experts) {
+        for (int c = a; c < b; ++c) {
+            const int v = counts[(int64_t)c * experts + e];
+            counts[(int64_t)c * experts + e] = run;
+            run += v;
+        }
+        if (warp == 31) totals[e] = run;
+    }
+}
+
+__global__ void __launch_bounds__(kWarps * 32) route_place_kernel(spmm_route_args p, int64_t chunk, const int *counts,
+                                                                  const int *totals) {
+    extern __shared__ int sm[];
+    __shared__ int tmp[33];
+    const int experts = (int)p.experts;
+    int *base = sm, *wcount = sm + experts;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) base[e] = totals[e];
+    __syncthreads();
+    const int total = cta_exclusive(base, experts, tmp);
+    if (blockIdx.x == 0) {
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) p.offsets[e] = base[e];
+        if (threadIdx.x == 0) p.offsets[experts] = total;
+        __syncthreads();
+    }
+    const int64_t all = p.tokens * p.top;
+    const int64_t i0 = blockIdx.x * chunk * p.top, i1 = i0 + chunk * p.top < all ? i0 + chunk * p.top : all;
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x)
+        if (i >= total) p.rows[i] = -1;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x)
+        base[e] += counts[(int64_t)blockIdx.x * experts + e];
+    __syncthreads();
+    place(p, i0, i1, base, wcount);
+}
+
+// dlogits, a warp per token.  With g = scale * dweights at the chosen experts and 0 elsewhere:
+//   renormalised, w = s / sum s:  ds = (g - <g, w>) / sum s at the chosen ones
+//   softmax over all:             dl = p (ds - <ds, p>);  renormalised, s = exp(l) of the chosen ones: w (g - <g, w>)
+//   sigmoid:                      dl = ds s (1 - s)
+template <typename T, int V>
+__global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(spmm_route_args p) {
+    const int lane = threadIdx.x & 31;
+    const int experts = (int)p.experts, top = (int)p.top;
+    const int64_t step = (int64_t)gridDim.x * kWarps;
+    for (int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); t < p.tokens; t += step) {
+        const T *row = (const T *)p.logits + t * p.logits_ld;
+        T *out = (T *)p.dlogits + t * experts;
+        int e = -1;
+        float g = 0.f, l = -INFINITY;
+        if (lane < top) {
+            e = p.experts_out[t * top + lane];
+            if (e >= experts) e = -1;
+            if (e >= 0) {
+                g = p.scale * p.dweights[t * top + lane];
+                l = clean_logit(to_f32(row[e]));
+            }
+        }
+        float d;               // gradient at this lane's choice
+        float all = 0.f;       // softmax over all: <g, p>
+        Row r{0.f, 1.f};
+        float s = 0.f;
+        if (p.scoring == SPMM_SCORE_SOFTMAX) {
+            if (p.renormalize) {
+                float c[1] = {l};
+                r = softmax_row<1>(c);
+            } else {
+                float x[V];
+                load_row<T, V>(row, experts, lane, x);
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[v] = clean_logit(x[v]);
+                r = softmax_row<V>(x);
+            }
+            s = e >= 0 && r.total > 0.f ? expf(l - r.peak) / r.total : 0.f;
+        } else {
+            s = e >= 0 ? sigmoid(l) : 0.f;
+        }
+        float w = s;
+        if (p.renormalize && p.scoring == SPMM_SCORE_SIGMOID) {
+            float sum = s;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+            w = sum > 0.f ? s / sum : 0.f;
+        }
+        float dot = g * w;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
+        if (p.scoring == SPMM_SCORE_SOFTMAX) {
+            d = s * (g - dot);
+            all = p.renormalize ? 0.f : dot;
+        } else {
+            d = p.renormalize ? w * (g - dot) * (1.f - s) : g * s * (1.f - s);
+        }
+        if (all != 0.f) {      // softmax over all: experts that were not chosen have -p <g, p>
+            float x[V];
+            load_row<T, V>(row, experts, lane, x);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v * 32 + lane < experts)
+                    out[v * 32 + lane] = from_f32<T>(-all * (expf(clean_logit(x[v]) - r.peak) / r.total));
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v * 32 + lane < experts) out[v * 32 + lane] = from_f32<T>(0.f);
+        }
+        __syncwarp();
+        if (e >= 0) out[e] = from_f32<T>(d);
+    }
+}
+
+// ---- combine --------------------------------------------------------------------
+
+template <typename T, int VEC> struct Pack { T v[VEC]; };
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T *p, float (&f)[VEC]) {
+    if constexpr (VEC * sizeof(T) == 16) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+        T t[VEC];
+        memcpy(t, &u, 16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = to_f32(t[i]);
+    } else {
+        static_assert(VEC == 1, "one value or 16 bytes");
+        f[0] = to_f32(p[0]);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC]) {
+    T t[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = from_f32<T>(f[i]);
+    if constexpr (VEC * sizeof(T) == 16) {
+        uint4 u;
+        memcpy(&u, t, 16);
+        *reinterpret_cast<uint4 *>(p) = u;
+    } else {
+        p[0] = t[0];
+    }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) combine_kernel(spmm_combine_args p, int64_t per) {
+    const int64_t items = p.tokens * per, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += step) {
+        const int64_t t = i / per, c = (i - t * per) * VEC;
+        float acc[VEC] = {};
+        for (int64_t j0 = 0; j0 < p.top; j0 += 4) {
+            float f[4][VEC], w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                w[u] = 0.f;
+#pragma unroll
+                for (int x = 0; x < VEC; ++x) f[u][x] = 0.f;
+                if (j0 + u < p.top) {
+                    const int64_t s = __ldg(p.slots + t * p.top + j0 + u);
+                    if (s >= 0 && s < p.rows) {
+                        w[u] = __ldg(p.weights + t * p.top + j0 + u);
+                        load_vec<T, VEC>((const T *)p.y + s * p.y_ld + c, f[u]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int x = 0; x < VEC; ++x) acc[x] = fmaf(w[u], f[u][x], acc[x]);
+        }
+        if (p.residual) {
+            float f[VEC];
+            load_vec<T, VEC>((const T *)p.residual + t * p.residual_ld + c, f);
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) acc[x] += f[x];
+        }
+        store_vec<T, VEC>((T *)p.out + t * p.out_ld + c, acc);
+    }
+}
+
+// A warp per token: dout's row against each chosen row of y.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) combine_backward_kernel(spmm_combine_args p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t per = p.n / VEC, step = (int64_t)gridDim.x * 8;
+    const int64_t w0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    for (int64_t t = w0; t < p.tokens; t += step) {
+        for (int64_t j = 0; j < p.top; ++j) {
+            const int64_t s = __ldg(p.slots + t * p.top + j);
+            const bool in = s >= 0 && s < p.rows;
+            float dot = 0.f;
+            if (in) {
+                const float w = p.dy ? __ldg(p.weights + t * p.top + j) : 0.f;
+                for (int64_t c = lane; c < per; c += 32) {
+                    float d[VEC];
+                    load_vec<T, VEC>((const T *)p.dout + t * p.dout_ld + c * VEC, d);
+                    if (p.dweights) {
+                        float y[VEC];
+                        load_vec<T, VEC>((const T *)p.y + s * p.y_ld + c * VEC, y);
+#pragma unroll
+                        for (int x = 0; x < VEC; ++x) dot = fmaf(d[x], y[x], dot);
+                    }
+                    if (p.dy) {
+#pragma unroll
+                        for (int x = 0; x < VEC; ++x) d[x] *= w;
+                        store_vec<T, VEC>((T *)p.dy + s * p.dy_ld + c * VEC, d);
+                    }
+                }
+            }
+            if (p.dweights) {
+#pragma unroll
+                for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
+                if (lane == 0) p.dweights[t * p.top + j] = dot;
+            }
+        }
+    }
+    if (p.dy) {   // rows behind the last group
+        for (int64_t r = group_first(p.offsets, p.experts, p.rows) + w0; r < p.rows; r += step)
+            for (int64_t c = lane; c < p.n; c += 32) ((T *)p.dy)[r * p.dy_ld + c] = from_f32<T>(0.f);
+    }
+}
+
+// ---- host side --------------------------------------------------------------------
+
+constexpr int64_t kChunks = 512;   // chunks of the grouping, at most
+
+int check_route(const spmm_route_args *p) {
+    if (!p || p->version != 1) return SPMM_EINVAL;
+    if (p->dtype != SPMM_DENSE_F32 && p->dtype != SPMM_DENSE_BF16 && p->dtype != SPMM_DENSE_F16)
+        return SPMM_EUNSUPPORTED;
+    if (p->tokens < 0 || p->experts < 1 || p->top < 1 || p->top > p->experts) return SPMM_EINVAL;
+    if (p->experts > kMaxExperts || p->top > SPMM_MAX_TOP || p->tokens > INT32_MAX / p->top)
+        return SPMM_EUNSUPPORTED;
+    if (p->scoring != SPMM_SCORE_SOFTMAX && p->scoring != SPMM_SCORE_SIGMOID) return SPMM_EINVAL;
+    return SPMM_OK;
+}
+
+bool small_route(const spmm_route_args *p) { return p->tokens <= 128; }
+
+int64_t chunk_tokens(const spmm_route_args *p) {
+    const int64_t c = ceil_div(p->tokens, kChunks);
+    return c < 32 ? 32 : c;
+}
+
+template <typename T, int V>
+int run_route(const spmm_route_args &p, cudaStream_t s) {
+    const int e4 = (int)p.experts * 4;
+    if (small_route(&p)) {
+        const int most = V <= 8 ? 32 : 16;   // registers: V logits and keys a thread
+        int warps = (int)(p.tokens < 1 ? 1 : p.tokens < most ? p.tokens : most);
+        while (warps > 1 && (warps + 1) * e4 > 40 * 1024) --warps;   // below 48 KB with the static part
+        route_small_kernel<T, V><<<1, warps * 32, (warps + 1) * e4, s>>>(p);
+        SPMM_PRODUCT_LAUNCHED();
+        return SPMM_OK;
+    }
+    const int64_t chunk = chunk_tokens(&p), chunks = ceil_div(p.tokens, chunk);
+    int *counts = (int *)p.workspace, *totals = counts + chunks * p.experts;
+    route_choose_kernel<T, V><<<(unsigned)chunks, kWarps * 32, e4, s>>>(p, chunk, counts);
+    SPMM_PRODUCT_LAUNCHED();
+    route_scan_kernel<<<(unsigned)ceil_div(p.experts, 32), 1024, 0, s>>>(counts, (int)chunks, (int)p.experts, totals);
+    SPMM_PRODUCT_LAUNCHED();
+    route_place_kernel<<<(unsigned)chunks, kWarps * 32, (kWarps + 1) * e4, s>>>(p, chunk, counts, totals);
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
+}
+
+template <typename T, int V>
+int run_route_backward(const spmm_route_args &p, cudaStream_t s) {
+    int64_t grid = ceil_div(p.tokens, kWarps);
+    if (grid > 148 * 8) grid = 148 * 8;
+    route_backward_kernel<T, V><<<(unsigned)grid, kWarps * 32, 0, s>>>(p);
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
+}
+
+template <typename T>
+int by_width(const spmm_route_args &p, bool backward, cudaStream_t s) {
+#define SPMM_ROUTE_V(V) return backward ? run_route_backward<T, V>(p, s) : run_route<T, V>(p, s)
+    if (p.experts <= 32) SPMM_ROUTE_V(1);
+    if (p.experts <= 64) SPMM_ROUTE_V(2);
+    if (p.experts <= 128) SPMM_ROUTE_V(4);
+    if (p.experts <= 256) SPMM_ROUTE_V(8);
+    if (p.experts <= 512) SPMM_ROUTE_V(16);
+    SPMM_ROUTE_V(32);
+#undef SPMM_ROUTE_V
+}
+
+int by_type(const spmm_route_args &p, bool backward, cudaStream_t s) {
+    if (p.dtype == SPMM_DENSE_F32) return by_width<float>(p, backward, s);
+    if (p.dtype == SPMM_DENSE_F16) return by_width<__half>(p, backward, s);
+    return by_width<__nv_bfloat16>(p, backward, s);
+}
+
+int check_combine(const spmm_combine_args *p) {
+    if (!p || p->version != 1) return SPMM_EINVAL;
+    if (p->dtype != SPMM_DENSE_F32 && p->dtype != SPMM_DENSE_BF16 && p->dtype != SPMM_DENSE_F16)
+        return SPMM_EUNSUPPORTED;
+    if (p->tokens < 0 || p->top < 1 || p->rows < 0 || p->n < 0) return SPMM_EINVAL;
+    return SPMM_OK;
+}
+
+bool aligned16(const void *p, int64_t ld, int64_t per) { return (uintptr_t)p % 16 == 0 && ld % per == 0; }
+
+template <typename T>
+int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
+    constexpr int W = 16 / sizeof(T);
+    bool vec = p.n % W == 0 && aligned16(p.y, p.y_ld, W);
+    if (backward)
+        vec = vec && aligned16(p.dout, p.dout_ld, W) && aligned16(p.dy, p.dy_ld, W);
+    else
+        vec = vec && aligned16(p.out, p.out_ld, W) && aligned16(p.residual, p.residual_ld, W);
+    if (backward) {
+        int64_t grid = ceil_div(p.tokens > 0 ? p.tokens : 1, 8);
+        if (grid > 148 * 8) grid = 148 * 8;
+        if (vec) combine_backward_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p);
+        else combine_backward_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
+    } else {
+        const int64_t per = vec ? p.n / W : p.n;
+        int64_t grid = ceil_div(p.tokens * per, 256);
+        if (grid > 148 * 32) grid = 148 * 32;
+        if (vec) combine_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p, per);
+        else combine_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p, per);
+    }
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
+}
+
+}  // namespace
+}  // namespace spmm
+
+using namespace spmm;
+
+extern "C" size_t spmm_route_workspace_size(const spmm_route_args *p) {
+    if (check_route(p) != SPMM_OK || small_route(p)) return 0;
+    return (size_t)(ceil_div(p->tokens, chunk_tokens(p)) + 1) * p->experts * 4;
+}
+
+extern "C" int spmm_route(const spmm_route_args *p, spmm_stream_t stream) {
+    SPMM_TRY(check_route(p));
+    if (!p->offsets || (p->tokens && (!p->logits || !p->weights || !p->experts_out || !p->slots || !p->rows)))
+        return SPMM_EINVAL;
+    const size_t need = spmm_route_workspace_size(p);
+    if (need && (!p->workspace || p->workspace_bytes < need)) return SPMM_EWORKSPACE;
+    return by_type(*p, false, (cudaStream_t)stream);
+}
+
+extern "C" int spmm_route_backward(const spmm_route_args *p, spmm_stream_t stream) {
+    SPMM_TRY(check_route(p));
+    if (p->tokens == 0) return SPMM_OK;
+    if (!p->logits || !p->experts_out || !p->dweights || !p->dlogits) return SPMM_EINVAL;
+    return by_type(*p, true, (cudaStream_t)stream);
+}
+
+extern "C" int spmm_combine(const spmm_combine_args *p, spmm_stream_t stream) {
+    SPMM_TRY(check_combine(p));
+    if (p->tokens == 0 || p->n == 0) return SPMM_OK;
+    if (!p->slots || !p->weights || !p->out || (p->rows && !p->y)) return SPMM_EINVAL;
+    if (p->dtype == SPMM_DENSE_F32) return run_combine<float>(*p, false, (cudaStream_t)stream);
+    if (p->dtype == SPMM_DENSE_F16) return run_combine<__half>(*p, false, (cudaStream_t)stream);
+    return run_combine<__nv_bfloat16>(*p, false, (cudaStream_t)stream);
+}
+
+extern "C" int spmm_combine_backward(const spmm_combine_args *p, spmm_stream_t stream) {
+    SPMM_TRY(check_combine(p));
+    if (!p->dy && !p->dweights) return SPMM_OK;
+    if (p->tokens && (!p->slots || !p->weights || (p->n && (!p->dout || (p->rows && !p->y))))) return SPMM_EINVAL;
+    if (p->dy && (!p->offsets || p->experts < 0)) return SPMM_EINVAL;
+    if (p->dtype == SPMM_DENSE_F32) return run_combine<float>(*p, true, (cudaStream_t)stream);
+    if (p->dtype == SPMM_DENSE_F16) return run_combine<__half>(*p, true, (cudaStream_t)stream);
+    return run_combine<__nv_bfloat16>(*p, true, (cudaStream_t)stream);
+}
