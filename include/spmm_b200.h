@@ -383,6 +383,8 @@ typedef struct {
     int32_t dtype;              /* enum spmm_dense_type: BF16 or F16 */
     int32_t activation;         /* enum spmm_activation (forward) */
     int32_t wait_us;            /* bounded device waits: 0 = about 2 s, else at least 1000 */
+    int32_t flags;              /* 0, or SPMM_CFG_EXPIRE_FIRST_WAIT (tests of the timeout path) */
+    int32_t reserved;           /* 0 */
     int64_t rows, k, n, groups; /* rows of y */
     int64_t x_rows;             /* rows of x (== rows without gather) */
     const int32_t *offsets;     /* groups + 1, or NULL: one group */

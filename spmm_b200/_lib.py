@@ -101,7 +101,8 @@ MAX_GROUPS, MAX_TOP = 1024, 32
 
 
 class Linear(C.Structure):
-    _fields_ = ([('version', C.c_int32), ('dtype', C.c_int32), ('activation', C.c_int32), ('wait_us', C.c_int32)]
+    _fields_ = ([('version', C.c_int32), ('dtype', C.c_int32), ('activation', C.c_int32), ('wait_us', C.c_int32),
+                 ('flags', C.c_int32), ('reserved', C.c_int32)]
                 + [(n, C.c_int64) for n in ('rows', 'k', 'n', 'groups', 'x_rows')]
                 + [(n, C.c_void_p) for n in ('offsets', 'gather', 'slots')] + [('top', C.c_int64)]
                 + [(n, C.c_void_p) for n in ('x', 'w', 'bias', 'residual', 'y', 'slope', 'dy', 'dx', 'dw', 'dbias')]

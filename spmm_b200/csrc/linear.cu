@@ -1,5 +1,5 @@
 // linear.cu -- dense and grouped products of 16-bit operands: the C entries,
-// operand copies, the gradient of the activation, and a plain product kernel.
+// operand copies and the gradient of the activation.
 //
 //   forward   y[r] = act(x[r] w[g] + bias[g]) + residual[r]
 //   backward  dz = dy * act'(z), dx = dz w^T, dw = x^T dz, dbias = sum dz
@@ -10,91 +10,6 @@
 
 namespace spmm {
 namespace {
-
-// ---- plain product ----------------------------------------------------------
-
-// Any strides, any sizes: a 64 x 64 tile per CTA of 256 threads, 4 x 4 sums
-// each, operands through shared memory 16 at a time.
-template <typename T, typename O, int ACT>
-__global__ void __launch_bounds__(256) product_kernel(Product p) {
-    __shared__ float As[16][65], Bs[16][65];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int64_t p0 = (int64_t)blockIdx.x * 64;
-    RowTile t;
-    int64_t r0 = 0, r1 = p.R, q0, g;
-    int nq;
-    if (p.red) {
-        const int64_t qt = (p.Q + 63) / 64;
-        g = blockIdx.y / qt;
-        q0 = (blockIdx.y % qt) * 64;
-        nq = (int)(p.Q - q0 < 64 ? p.Q - q0 : 64);
-        if (p.offsets) {
-            r0 = group_first(p.offsets, g, p.R);
-            r1 = group_first(p.offsets, g + 1, p.R);
-        }
-    } else {
-        t = find_row_tile(p.offsets, p.groups, p.Q, 64, blockIdx.y);
-        if (t.group > p.groups) return;
-        g = t.group;
-        q0 = t.first;
-        nq = t.rows;
-    }
-    const bool tail = !p.red && p.offsets && g == p.groups;
-    if (tail) r1 = 0;
-    const int64_t gi = tail ? 0 : g;
-    const T *A = (const T *)p.A + (p.red ? 0 : gi * p.a_g), *B = (const T *)p.B;
-    float acc[4][4] = {};
-    for (int64_t r = r0; r < r1; r += 16) {
-        for (int i = tid; i < 64 * 16; i += 256) {
-            const int pr = p.a_r == 1 ? i & 15 : i >> 6, pp = p.a_r == 1 ? i >> 4 : i & 63;
-            As[pr][pp] = r + pr < r1 && p0 + pp < p.P ? to_f32(A[(p0 + pp) * p.a_p + (r + pr) * p.a_r]) : 0.f;
-            const int qr = p.b_r == 1 ? i & 15 : i >> 6, qq = p.b_r == 1 ? i >> 4 : i & 63;
-            Bs[qr][qq] = r + qr < r1 && qq < nq ? to_f32(B[(q0 + qq) * p.b_q + (r + qr) * p.b_r]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[k][tx + 16 * i], Bs[k][ty + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-    O *C = (O *)p.C + (p.red ? g * p.c_g : 0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int qq = ty + 16 * j;
-        if (qq >= nq) continue;
-        const int64_t q = q0 + qq;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t pp = p0 + tx + 16 * i;
-            if (pp >= p.P) continue;
-            float z = acc[i][j];
-            ActValue a{0.f, 0.f};
-            if (!tail) {
-                if (p.bias) z += to_f32(((const T *)p.bias)[gi * p.bias_g + pp]);
-                a = activate<ACT>(z);
-                if (p.residual) a.y += to_f32(((const T *)p.residual)[q * p.residual_ld + pp]);
-            }
-            C[q * p.c_q + pp] = from_f32<O>(a.y);
-            if (p.slope) p.slope[q * p.P + pp] = slope_code(a.slope);
-        }
-    }
-}
-
-template <typename T, typename O>
-int launch_act(const Product &p, dim3 grid, cudaStream_t s) {
-    switch (p.act) {
-        case SPMM_ACT_NONE: product_kernel<T, O, SPMM_ACT_NONE><<<grid, 256, 0, s>>>(p); break;
-        case SPMM_ACT_RELU: product_kernel<T, O, SPMM_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
-        case SPMM_ACT_GELU: product_kernel<T, O, SPMM_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
-        case SPMM_ACT_GELU_TANH: product_kernel<T, O, SPMM_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p); break;
-        default: product_kernel<T, O, SPMM_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
-    }
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
-}
 
 // ---- operand copies -----------------------------------------------------------
 
@@ -204,8 +119,6 @@ __global__ void gather_sum_kernel(const float *src, int64_t rows, const int32_t 
         }
 }
 
-__global__ void clear_status_kernel(int32_t *status) { *status = 0; }
-
 // ---- host side ------------------------------------------------------------------
 
 int check_sizes(const spmm_linear *p) {
@@ -217,31 +130,64 @@ int check_sizes(const spmm_linear *p) {
         return SPMM_EUNSUPPORTED;
     if (!p->offsets && p->groups != 1) return SPMM_EINVAL;
     if (!p->gather && p->x_rows != p->rows) return SPMM_EINVAL;
-    if (p->wait_us != 0 && p->wait_us < 1000) return SPMM_EINVAL;
+    if ((p->wait_us != 0 && p->wait_us < 1000) || (p->flags & ~SPMM_CFG_EXPIRE_FIRST_WAIT)) return SPMM_EINVAL;
     if (p->w_k != 1 && p->w_n != 1) return SPMM_EUNSUPPORTED;
     return SPMM_OK;
 }
 
-// x as the product reads it: in place, or a copy (gathered).
+// An operand as the product reads it: in place, or a copy with aligned rows.
 struct Operand {
     const void *ptr;
-    int64_t ld;
+    int64_t ld, gs;   // row stride, group stride
 };
 
-int carve_x(const spmm_linear *p, Arena &a, bool sizing, Operand &x, cudaStream_t s) {
-    x = Operand{p->x, p->x_ld};
-    if (!p->gather || p->rows == 0 || p->k == 0) return SPMM_OK;
-    const int64_t ld = ceil_div(p->k, 8) * 8;
-    uint16_t *buf = a.take<uint16_t>(p->rows * ld);
+// Tensor copies need 16-byte aligned rows.
+bool in_place(const void *p, int64_t ld, int64_t gs, int64_t cols) {
+    return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && gs % 8 == 0 && ld >= cols;
+}
+
+// `rows` x `cols` values (per group), gathered by `map` or copied where they are not aligned.
+int carve(const Operand src, int64_t src_rows, const int32_t *map, int64_t groups, int64_t rows, int64_t cols,
+          Arena &a, bool sizing, Operand &out, cudaStream_t s) {
+    out = src;
+    if (rows == 0 || cols == 0) return SPMM_OK;
+    const int64_t ld = ceil_div(cols, 8) * 8;
+    if (rows == 1) out.ld = ld;         // one row: its stride is never used
+    if (groups == 1) out.gs = 0;
+    if (!map && in_place(src.ptr, out.ld, out.gs, cols)) return SPMM_OK;
+    const int64_t copies = groups > 1 && src.gs == 0 ? 1 : groups;   // a block shared by all groups
+    out.ld = ld;
+    out.gs = copies > 1 ? rows * ld : 0;
+    uint16_t *buf = a.take<uint16_t>(copies * rows * ld);
     if (sizing) return SPMM_OK;
     if (!buf) return SPMM_EWORKSPACE;
-    const int vec = p->k % 8 == 0 && p->x_ld % 8 == 0 && (uintptr_t)p->x % 16 == 0;
-    const int64_t per = vec ? p->k / 8 : p->k;
+    out.ptr = buf;
+    const int vec = cols % 8 == 0 && in_place(src.ptr, src.ld, src.gs, cols);
+    const int64_t per = vec ? cols / 8 : cols;
     const int threads = per >= 256 ? 256 : (int)ceil_div(per, 32) * 32;
-    copy_rows_kernel<<<(unsigned)(p->rows < 65536 ? p->rows : 65536), threads, 0, s>>>(
-        (const uint16_t *)p->x, p->x_ld, 0, p->x_rows, p->gather, buf, ld, 0, p->rows, p->k, vec);
+    const dim3 grid((unsigned)(rows < 65536 ? rows : 65536), 1, (unsigned)copies);
+    copy_rows_kernel<<<grid, threads, 0, s>>>((const uint16_t *)src.ptr, src.ld, src.gs, src_rows, map, buf, ld,
+                                              out.gs, rows, cols, vec);
     SPMM_PRODUCT_LAUNCHED();
-    x = Operand{buf, ld};
+    return SPMM_OK;
+}
+
+int carve_x(const spmm_linear *p, Arena &a, bool sizing, Operand &x, cudaStream_t s) {
+    return carve({p->x, p->x_ld, 0}, p->x_rows, p->gather, 1, p->rows, p->k, a, sizing, x, s);
+}
+
+// w's strides along n, k and the groups, in place or of the copy.
+struct Weight {
+    const void *ptr;
+    int64_t n, k, g;
+};
+
+int carve_w(const spmm_linear *p, Arena &a, bool sizing, Weight &w, cudaStream_t s) {
+    const bool n_unit = p->w_n == 1;
+    Operand o;
+    SPMM_TRY(carve({p->w, n_unit ? p->w_k : p->w_n, p->w_g}, n_unit ? p->k : p->n, nullptr, p->groups,
+                   n_unit ? p->k : p->n, n_unit ? p->n : p->k, a, sizing, o, s));
+    w = n_unit ? Weight{o.ptr, 1, o.ld, o.gs} : Weight{o.ptr, o.ld, 1, o.gs};
     return SPMM_OK;
 }
 
@@ -259,17 +205,19 @@ Product base(const spmm_linear *p) {
 
 int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     Operand x;
+    Weight w;
     SPMM_TRY(carve_x(p, a, sizing, x, s));
+    SPMM_TRY(carve_w(p, a, sizing, w, s));
     if (sizing) return SPMM_OK;
     Product g = base(p);
     g.P = p->n;
     g.Q = p->rows;
     g.R = p->k;
     g.act = p->activation;
-    g.A = p->w;
-    g.a_p = p->w_n;
-    g.a_r = p->w_k;
-    g.a_g = p->w_g;
+    g.A = w.ptr;
+    g.a_p = w.n;
+    g.a_r = w.k;
+    g.a_g = w.g;
     g.B = x.ptr;
     g.b_q = x.ld;
     g.b_r = 1;
@@ -280,23 +228,26 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     g.residual = p->residual;
     g.residual_ld = p->residual_ld;
     g.slope = p->slope;
-    return launch_product(g, s);
+    return launch_product(g, true, p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT, s);
 }
 
 template <typename T>
 int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
-    Operand x{p->x, p->x_ld};
+    Operand x{}, dz{p->dy, p->dy_ld, 0};
+    Weight w{};
     if (p->dw) SPMM_TRY(carve_x(p, a, sizing, x, s));
-    Operand dz{p->dy, p->dy_ld};
+    if (p->dx) SPMM_TRY(carve_w(p, a, sizing, w, s));
     const int64_t tiles = ceil_div(p->rows, kDzRows) + (p->offsets ? p->groups + 1 : 0);
     if (tiles > 65535) return SPMM_EUNSUPPORTED;
     T *dzp = nullptr;
     float *part = nullptr, *dxs = nullptr;
-    const bool any = p->rows > 0 && p->n > 0;
+    const bool any = p->rows > 0 && p->n > 0, probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
     if (p->slope && any && (p->dx || p->dw)) {
         const int64_t ld = ceil_div(p->n, 8) * 8;
         dzp = a.take<T>(p->rows * ld);
-        dz = Operand{dzp, ld};
+        dz = Operand{dzp, ld, 0};
+    } else if (any && (p->dx || p->dw)) {
+        SPMM_TRY(carve(dz, p->rows, nullptr, 1, p->rows, p->n, a, sizing, dz, s));
     }
     if (p->dbias && any) part = a.take<float>(tiles * p->n);
     if (p->dx && p->gather) dxs = a.take<float>(p->rows * p->k);
@@ -318,17 +269,17 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
         g.P = p->k;
         g.Q = p->rows;
         g.R = p->n;
-        g.A = p->w;
-        g.a_p = p->w_k;
-        g.a_r = p->w_n;
-        g.a_g = p->w_g;
+        g.A = w.ptr;
+        g.a_p = w.k;
+        g.a_r = w.n;
+        g.a_g = w.g;
         g.B = dz.ptr;
         g.b_q = dz.ld;
         g.b_r = 1;
         g.C = dxs ? (void *)dxs : p->dx;
         g.c_q = dxs ? p->k : p->dx_ld;
         g.out_f32 = dxs != nullptr;
-        SPMM_TRY(launch_product(g, s));
+        SPMM_TRY(launch_product(g, true, probe, s));
         if (dxs)
             SPMM_TRY(launch_gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, p->dx, p->dx_ld, g.f16, s));
     }
@@ -348,7 +299,7 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
         g.C = p->dw;
         g.c_q = n_unit ? p->dw_k : p->dw_n;
         g.c_g = p->dw_g;
-        SPMM_TRY(launch_product(g, s));
+        SPMM_TRY(launch_product(g, !p->dx, probe, s));
     }
     return SPMM_OK;
 }
@@ -365,24 +316,13 @@ size_t sized(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool
     return (a.used + 255) & ~(size_t)255;
 }
 
-int clear_status(const spmm_linear *p, cudaStream_t s) {
-    if (!p->status) return SPMM_OK;
-    clear_status_kernel<<<1, 1, 0, s>>>(p->status);
-    SPMM_LAUNCH_CHECK();
+// The products clear the status word themselves; a call without any does it here.
+int clear_status(const spmm_linear *p, bool product, cudaStream_t s) {
+    if (p->status && !product) SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
     return SPMM_OK;
 }
 
 }  // namespace
-
-int launch_product(const Product &p, cudaStream_t s) {
-    if (p.P == 0 || p.Q == 0) return SPMM_OK;
-    const int64_t gy = p.red ? p.groups * ceil_div(p.Q, 64) : ceil_div(p.Q, 64) + (p.offsets ? p.groups + 1 : 0);
-    if (gy > 65535) return SPMM_EUNSUPPORTED;
-    const dim3 grid((unsigned)ceil_div(p.P, 64), (unsigned)gy);
-    if (p.f16) return p.out_f32 ? launch_act<__half, float>(p, grid, s) : launch_act<__half, __half>(p, grid, s);
-    return p.out_f32 ? launch_act<__nv_bfloat16, float>(p, grid, s)
-                     : launch_act<__nv_bfloat16, __nv_bfloat16>(p, grid, s);
-}
 
 int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,
                       void *out, int64_t out_ld, int f16, cudaStream_t s) {
@@ -412,7 +352,7 @@ extern "C" int spmm_linear_forward(const spmm_linear *p, spmm_stream_t stream) {
     const int64_t out = p->rows * p->n;
     if (out && !p->y) return SPMM_EINVAL;
     if (out && p->k && (!p->x || !p->w)) return SPMM_EINVAL;
-    SPMM_TRY(spmm::clear_status(p, (cudaStream_t)stream));
+    SPMM_TRY(spmm::clear_status(p, out > 0, (cudaStream_t)stream));
     spmm::Arena a(p->workspace, p->workspace_bytes);
     return spmm::forward(p, a, false, (cudaStream_t)stream);
 }
@@ -422,7 +362,8 @@ extern "C" int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream) 
     if (p->rows * p->n && !p->dy) return SPMM_EINVAL;
     if (p->dx && ((p->k * p->n && !p->w) || (p->gather && (!p->slots || p->top < 1)))) return SPMM_EINVAL;
     if (p->dw && ((p->rows * p->k && !p->x) || (p->dw_k != 1 && p->dw_n != 1))) return SPMM_EINVAL;
-    SPMM_TRY(spmm::clear_status(p, (cudaStream_t)stream));
+    const bool product = (p->dx && p->rows * p->k) || (!p->dx && p->dw && p->k * p->n);
+    SPMM_TRY(spmm::clear_status(p, product, (cudaStream_t)stream));
     spmm::Arena a(p->workspace, p->workspace_bytes);
     return spmm::backward(p, a, false, (cudaStream_t)stream);
 }

@@ -160,7 +160,8 @@ struct Product {
     int64_t wait_cycles;
 };
 
-int launch_product(const Product &p, cudaStream_t s);
+// `clear`: the kernel sets *status to 0 first (the first product of a call); `probe`: SPMM_CFG_EXPIRE_FIRST_WAIT.
+int launch_product(const Product &p, bool clear, bool probe, cudaStream_t s);
 
 // out[t] = sum_j weight * src[slots[t][j]] over float32 rows (the gradient of gathered rows).
 int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,

@@ -126,6 +126,6 @@ def test_route_and_combine_entries():
 
 
 def test_struct_sizes_match_the_header():
-    assert C.sizeof(_lib.Linear) == 4 * 4 + 8 * (5 + 3 + 1 + 10 + 13 + 3)
+    assert C.sizeof(_lib.Linear) == 6 * 4 + 8 * (5 + 3 + 1 + 10 + 13 + 3)
     assert C.sizeof(_lib.RouteArgs) == 4 * 4 + 8 * 3 + 8 * 3 + 8 + 8 * 8 + 8
     assert C.sizeof(_lib.CombineArgs) == 8 + 8 * 5 + 8 * 9 + 8 * 5

@@ -14,10 +14,13 @@ included):
        sums and u of the result
 """
 
+import ctypes as C
+
 import pytest
 import torch
 
 import spmm_b200 as S
+from spmm_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -264,6 +267,48 @@ def test_grouped_gather(cuda, tokens, experts, top, k, n, masked):
     close(dw, *ref['dw'], BF, 'dw')
     # the same as with the rows laid out by the caller
     assert torch.equal(y[gid >= 0], S.grouped_matmul(x[src], w, r, activation='silu')[gid >= 0])
+
+
+@pytest.mark.parametrize('t, k, n', [(3000, 256, 6200), (700, 2048, 4096), (5000, 520, 1500)])
+def test_many_tiles(cuda, t, k, n):
+    """More tiles than SMs: several per CTA, both accumulators in use."""
+    torch.manual_seed(t)
+    check_dense(normal(t, k), normal(k, n, scale=k ** -0.5), normal(n), normal(t, n), 'gelu_tanh')
+
+
+def test_many_ragged_groups(cuda):
+    torch.manual_seed(11)
+    G, k, n = 200, 192, 328
+    lens = [int(v) for v in torch.randint(0, 90, (G,))]
+    lens[17], lens[100] = 900, 0
+    offsets = torch.tensor([0] + lens).cumsum(0).int()
+    R = sum(lens) + 40
+    x, w, b, dy = normal(R, k), normal(G, k, n, scale=k ** -0.5), normal(G, n), normal(R, n)
+    ref = reference(x, w, group_of(offsets, R), torch.arange(R, device='cuda'), b, 'silu', dy)
+    go = offsets.cuda()
+    y, slope = S.grouped_matmul(x, w, go, b, activation='silu', return_slope=True)
+    close(y, *ref['y'], BF, 'y')
+    for name, got in zip(('dx', 'dw', 'dbias'), S.grouped_matmul_backward(dy, x, w, go, slope, bias=True)):
+        close(got, *ref[name], BF, name)
+
+
+def test_expired_wait_is_reported(cuda):
+    """A wait that nothing ends runs out after wait_us; the call's status says so and the next call is unharmed."""
+    x, w = normal(300, 256), normal(256, 512)
+    y = torch.zeros(300, 512, device='cuda', dtype=BF)
+    status = torch.full((1,), 7, dtype=torch.int32, device='cuda')
+    a = _lib.Linear()
+    a.version, a.dtype, a.rows, a.x_rows, a.k, a.n, a.groups = 1, _lib.DENSE_BF16, 300, 300, 256, 512, 1
+    a.x, a.x_ld, a.w, a.w_k, a.w_n, a.y, a.y_ld = x.data_ptr(), 256, w.data_ptr(), 512, 1, y.data_ptr(), 512
+    a.status, a.wait_us, a.flags = status.data_ptr(), 2000, _lib.SPMM_CFG_EXPIRE_FIRST_WAIT
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _lib.lib().spmm_linear_forward(C.byref(a), stream) == 0
+    torch.cuda.synchronize()
+    assert int(status) == _lib.SPMM_ETIMEOUT
+    a.flags = a.wait_us = 0
+    assert _lib.lib().spmm_linear_forward(C.byref(a), stream) == 0
+    torch.cuda.synchronize()
+    assert int(status) == 0 and torch.equal(y, S.dense_matmul(x, w))
 
 
 def test_wrong_offsets_stay_inside(cuda):
