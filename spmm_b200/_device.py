@@ -78,13 +78,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 def on_device(device: torch.device):
     """Context in which `device` is the current one; nothing when it is already."""
     if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _NOTHING
     return torch.cuda.device(device)
 
 

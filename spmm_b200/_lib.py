@@ -203,9 +203,9 @@ def lib() -> C.CDLL:
         L.spmm_hem_hierarchy.restype = C.c_int
         L.spmm_pbr_to_csr.restype = C.c_int
         for n in ('spmm_linear_forward', 'spmm_linear_backward'):
-            getattr(L, n).argtypes = [C.POINTER(Linear), C.c_void_p]
+            getattr(L, n).argtypes = [C.c_void_p, C.c_void_p]       # a Linear, or its bytes
             getattr(L, n).restype = C.c_int
-            getattr(L, n + '_workspace_size').argtypes = [C.POINTER(Linear)]
+            getattr(L, n + '_workspace_size').argtypes = [C.c_void_p]
             getattr(L, n + '_workspace_size').restype = C.c_size_t
         L.spmm_route_workspace_size.argtypes = [C.POINTER(RouteArgs)]
         L.spmm_route_workspace_size.restype = C.c_size_t

@@ -488,6 +488,8 @@ def product_status(y: torch.Tensor) -> int:
     status = getattr(y, '_spmm_status', None)
     if status is None:
         return 0
+    if status.dtype != torch.int32:      # the 4 bytes of a 16-bit product's word
+        status = status.view(torch.int32)
     return int(status.item())
 
 

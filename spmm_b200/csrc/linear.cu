@@ -39,47 +39,64 @@ __global__ void copy_rows_kernel(const uint16_t *src, int64_t src_ld, int64_t sr
 // ---- gradient of the activation and of the bias -------------------------------
 
 constexpr int kDzRows = 128;   // rows of a tile
-constexpr int kDzCols = 64;    // columns of a CTA
+constexpr int kDzCols = 256;   // columns of a CTA: 32 lanes of 8
 
 // dz = dy * act'(z) (rounded to the operands' type) and the tile's column sums
-// of the unrounded products.
-template <typename T>
+// of the unrounded products.  A warp takes a row at a time, a lane 16 bytes of
+// it; bound by reading dy and the slopes and writing dz once.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, const int16_t *slope, T *dz,
                                                  int64_t dz_ld, float *part, const int32_t *offsets, int64_t groups,
                                                  int64_t rows, int64_t n) {
     __shared__ float sums[8][kDzCols];
     const RowTile t = find_row_tile(offsets, groups, rows, kDzRows, blockIdx.y);
-    if (t.group > groups) return;
-    const bool tail = offsets && t.group == groups;
+    if (t.group > groups || (offsets && t.group == groups)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c0 = (int64_t)blockIdx.x * kDzCols;
-    float acc[2] = {0.f, 0.f};
-    if (!tail) {
+    const int64_t c0 = (int64_t)blockIdx.x * kDzCols + lane * 8;
+    const int cols = c0 >= n ? 0 : n - c0 < 8 ? (int)(n - c0) : 8;
+    float acc[8] = {};
+    if (cols) {
+#pragma unroll 4
         for (int i = warp; i < t.rows; i += 8) {
             const int64_t r = t.first + i;
+            float d[8];
+            if constexpr (VEC) {
+                unpack8<T>(__ldg((const uint4 *)(dy + r * dy_ld + c0)), d);
+                if (slope) {
+                    const uint4 v = __ldg((const uint4 *)(slope + r * n + c0));
+                    int16_t c[8];
+                    memcpy(c, &v, 16);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int64_t c = c0 + u * 32 + lane;
-                if (c < n) {
-                    float d = to_f32(dy[r * dy_ld + c]);
-                    if (slope) {
-                        d *= slope_value(slope[r * n + c]);
-                        if (dz) dz[r * dz_ld + c] = from_f32<T>(d);
+                    for (int e = 0; e < 8; ++e) d[e] *= slope_value(c[e]);
+                    if (dz) *(uint4 *)(dz + r * dz_ld + c0) = pack8<T>(d);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    d[e] = 0.f;
+                    if (e < cols) {
+                        d[e] = to_f32(dy[r * dy_ld + c0 + e]);
+                        if (slope) {
+                            d[e] *= slope_value(slope[r * n + c0 + e]);
+                            if (dz) dz[r * dz_ld + c0 + e] = from_f32<T>(d[e]);
+                        }
                     }
-                    acc[u] += d;
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += d[e];
         }
     }
     if (part == nullptr) return;
-    sums[warp][lane] = acc[0];
-    sums[warp][lane + 32] = acc[1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = acc[e];
     __syncthreads();
-    if (threadIdx.x < kDzCols && c0 + threadIdx.x < n) {
+    const int64_t c = (int64_t)blockIdx.x * kDzCols + threadIdx.x;
+    if (c < n) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x];
-        part[(int64_t)blockIdx.y * n + c0 + threadIdx.x] = v;
+        part[(int64_t)blockIdx.y * n + c] = v;
     }
 }
 
@@ -104,19 +121,55 @@ __global__ void dbias_kernel(const float *part, const int32_t *offsets, int64_t 
     out[g * out_g + c] = from_f32<T>(v);
 }
 
-// out[t] = sum_j src[slots[t][j]], in order of j.
-template <typename T>
-__global__ void gather_sum_kernel(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top,
-                                  int64_t n, T *out, int64_t out_ld) {
-    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-        for (int64_t c = threadIdx.x; c < n; c += blockDim.x) {
-            float v = 0.f;
-            for (int64_t j = 0; j < top; ++j) {
-                const int64_t s = __ldg(slots + t * top + j);
-                if (s >= 0 && s < rows) v += __ldg(src + s * n + c);
+// out[t] = sum_j src[slots[t][j]], in order of j: V values a thread, the rows of
+// four choices in flight.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) gather_sum_kernel(const float *src, int64_t rows, const int32_t *slots,
+                                                         int64_t tokens, int64_t top, int64_t n, T *out,
+                                                         int64_t out_ld) {
+    const int64_t per = n / V, items = tokens * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per, c = (i - t * per) * V;
+        float acc[V] = {};
+        for (int64_t j0 = 0; j0 < top; j0 += 4) {
+            float f[4][V];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t s = j0 + u < top ? __ldg(slots + t * top + j0 + u) : -1;
+                const bool in = s >= 0 && s < rows;
+                if constexpr (V == 4) {
+                    const float4 v = in ? __ldg((const float4 *)(src + s * n + c)) : float4{0.f, 0.f, 0.f, 0.f};
+                    f[u][0] = v.x, f[u][1] = v.y, f[u][2] = v.z, f[u][3] = v.w;
+                } else {
+                    f[u][0] = in ? __ldg(src + s * n + c) : 0.f;
+                }
             }
-            out[t * out_ld + c] = from_f32<T>(v);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += f[u][e];
         }
+        if constexpr (V == 4) {
+            T o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[e]);
+            memcpy(__builtin_assume_aligned(out + t * out_ld + c, 8), o, 8);
+        } else {
+            out[t * out_ld + c] = from_f32<T>(acc[0]);
+        }
+    }
+}
+
+template <typename T>
+int gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n, T *out,
+               int64_t out_ld, cudaStream_t s) {
+    const bool vec = n % 4 == 0 && out_ld % 4 == 0 && (uintptr_t)out % 8 == 0;
+    const int64_t blocks = ceil_div(tokens * (vec ? n / 4 : n), 256);
+    const unsigned grid = (unsigned)(blocks < 148 * 64 ? blocks : 148 * 64);
+    if (vec) gather_sum_kernel<T, 4><<<grid, 256, 0, s>>>(src, rows, slots, tokens, top, n, out, out_ld);
+    else gather_sum_kernel<T, 1><<<grid, 256, 0, s>>>(src, rows, slots, tokens, top, n, out, out_ld);
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -255,8 +308,14 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     if ((p->slope && any && (p->dx || p->dw) && !dzp) || (p->dbias && any && !part) || (p->dx && p->gather && !dxs))
         return SPMM_EWORKSPACE;
     if (dzp || part) {
-        dz_kernel<T><<<dim3((unsigned)ceil_div(p->n, kDzCols), (unsigned)tiles), 256, 0, s>>>(
-            (const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, p->offsets, p->groups, p->rows, p->n);
+        const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
+        const dim3 grid((unsigned)ceil_div(p->n, kDzCols), (unsigned)tiles);
+        if (vec)
+            dz_kernel<T, true><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, p->offsets,
+                                                    p->groups, p->rows, p->n);
+        else
+            dz_kernel<T, false><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part,
+                                                     p->offsets, p->groups, p->rows, p->n);
         SPMM_PRODUCT_LAUNCHED();
     }
     if (p->dbias && p->n) {
@@ -316,6 +375,12 @@ size_t sized(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool
     return (a.used + 255) & ~(size_t)255;
 }
 
+// Whether the workspace is too small: asked before anything is launched.
+bool short_of(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool, cudaStream_t)) {
+    const size_t need = sized(p, run);
+    return need && (!p->workspace || p->workspace_bytes < need);
+}
+
 // The products clear the status word themselves; a call without any does it here.
 int clear_status(const spmm_linear *p, bool product, cudaStream_t s) {
     if (p->status && !product) SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
@@ -327,13 +392,8 @@ int clear_status(const spmm_linear *p, bool product, cudaStream_t s) {
 int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,
                       void *out, int64_t out_ld, int f16, cudaStream_t s) {
     if (tokens == 0 || n == 0) return SPMM_OK;
-    const unsigned grid = (unsigned)(tokens < 65536 ? tokens : 65536);
-    if (f16)
-        gather_sum_kernel<<<grid, 256, 0, s>>>(src, rows, slots, tokens, top, n, (__half *)out, out_ld);
-    else
-        gather_sum_kernel<<<grid, 256, 0, s>>>(src, rows, slots, tokens, top, n, (__nv_bfloat16 *)out, out_ld);
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
+    return f16 ? gather_sum(src, rows, slots, tokens, top, n, (__half *)out, out_ld, s)
+               : gather_sum(src, rows, slots, tokens, top, n, (__nv_bfloat16 *)out, out_ld, s);
 }
 
 }  // namespace spmm
@@ -352,6 +412,7 @@ extern "C" int spmm_linear_forward(const spmm_linear *p, spmm_stream_t stream) {
     const int64_t out = p->rows * p->n;
     if (out && !p->y) return SPMM_EINVAL;
     if (out && p->k && (!p->x || !p->w)) return SPMM_EINVAL;
+    if (spmm::short_of(p, spmm::forward)) return SPMM_EWORKSPACE;
     SPMM_TRY(spmm::clear_status(p, out > 0, (cudaStream_t)stream));
     spmm::Arena a(p->workspace, p->workspace_bytes);
     return spmm::forward(p, a, false, (cudaStream_t)stream);
@@ -362,6 +423,7 @@ extern "C" int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream) 
     if (p->rows * p->n && !p->dy) return SPMM_EINVAL;
     if (p->dx && ((p->k * p->n && !p->w) || (p->gather && (!p->slots || p->top < 1)))) return SPMM_EINVAL;
     if (p->dw && ((p->rows * p->k && !p->x) || (p->dw_k != 1 && p->dw_n != 1))) return SPMM_EINVAL;
+    if (spmm::short_of(p, spmm::backward)) return SPMM_EWORKSPACE;
     const bool product = (p->dx && p->rows * p->k) || (!p->dx && p->dw && p->k * p->n);
     SPMM_TRY(spmm::clear_status(p, product, (cudaStream_t)stream));
     spmm::Arena a(p->workspace, p->workspace_bytes);

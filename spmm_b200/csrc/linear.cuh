@@ -95,44 +95,57 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t *offsets, int64_t
     return r;
 }
 
-// The activation and its derivative at z.  Both are bounded functions of z in
-// float32: exp and erf go through the CUDA library, 1/(1 + exp) cannot
-// overflow to NaN (exp(-z) = inf gives 0).
-struct ActValue {
-    float y, slope;
-};
-template <int ACT>
-__device__ __forceinline__ ActValue activate(float z) {
+// The activation and its derivative at z.  Exponentials and reciprocals are the
+// hardware's (about 2^-21 relative near 0, growing with |z|; far below a 16-bit
+// rounding): with expf and full divisions the epilogue of an 8192 x 16384 x 4096
+// product took longer than the product.  The error function is CUDA's, so gelu
+// is off by at most about 2^-24 |z|.  Far out each function is at its limit,
+// which also keeps 0 * inf away.
+__device__ __forceinline__ float sigmoid_fast(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
+
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float activate(float z, float &d) {
     if constexpr (ACT == SPMM_ACT_RELU) {
-        return {z > 0.f ? z : (z != z ? z : 0.f), z > 0.f ? 1.f : 0.f};
+        if constexpr (SLOPE) d = z > 0.f ? 1.f : 0.f;
+        return z < 0.f ? 0.f : z;                     // NaN stays
     } else if constexpr (ACT == SPMM_ACT_SILU) {
-        if (z == -INFINITY) return {0.f, 0.f};   // the limits; z * 0 would be NaN
-        const float s = 1.f / (1.f + expf(-z));
-        const float rest = z == INFINITY ? 0.f : z * (1.f - s);
-        return {z * s, s * (1.f + rest)};
+        const float s = sigmoid_fast(z), y = z < -100.f ? 0.f : z * s;
+        if constexpr (SLOPE) d = z > 80.f ? 1.f : fmaf(y, 1.f - s, s);
+        return y;
     } else if constexpr (ACT == SPMM_ACT_GELU) {
-        if (z == -INFINITY) return {0.f, 0.f};
-        const float cdf = 0.5f * erfcf(z * -0.70710678118654752f);
-        const float pdf = 0.3989422804014327f * expf(-0.5f * z * z);
-        return {z * cdf, cdf + (pdf > 0.f ? z * pdf : 0.f)};
+        const float cdf = fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f);
+        if constexpr (SLOPE) {
+            const float pdf = 0.3989422804014327f * __expf(-0.5f * z * z);
+            d = fabsf(z) > 12.f ? (z > 0.f ? 1.f : 0.f) : fmaf(z, pdf, cdf);
+        }
+        return z < -10.f ? 0.f : z * cdf;
     } else if constexpr (ACT == SPMM_ACT_GELU_TANH) {
-        // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u))
-        if (z == -INFINITY) return {0.f, 0.f};
+        // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), 2 u = 2 sqrt(2 / pi) (z + 0.044715 z^3)
         const float z2 = z * z;
-        const float u2 = 1.5957691216057308f * z * (1.f + 0.044715f * z2);
-        const float s = 1.f / (1.f + expf(-u2));
-        const float r = s * (1.f - s) * 1.5957691216057308f;
-        return {z * s, s + (r > 0.f ? z * r * (1.f + 0.134145f * z2) : 0.f)};
+        const float s = sigmoid_fast(1.5957691216057308f * z * fmaf(0.044715f, z2, 1.f));
+        const float y = z < -12.f ? 0.f : z * s;
+        if constexpr (SLOPE)
+            d = fabsf(z) > 12.f ? (z > 0.f ? 1.f : 0.f)
+                                : fmaf(y * (1.f - s), fmaf(0.21406859f, z2, 1.5957691216057308f), s);
+        return y;
     } else {
-        return {z, 1.f};
+        d = 1.f;
+        return z;
     }
 }
 
 // act'(z) in 16 bits.  It lies within (-2, 2), so fixed point in units of 2^-14
 // (off by at most 2^-15) keeps 4 to 30 times more of it than a 16-bit float
-// would; -32768 stands for NaN.
-__device__ __forceinline__ int16_t slope_code(float s) {
-    return s != s ? (int16_t)-32768 : (int16_t)__float2int_rn(s * 16384.f);
+// would; -32768 stands for NaN.  Adding 1.5 * 2^23 rounds to an integer in the
+// low bits.
+__device__ __forceinline__ uint16_t slope_code(float s) {
+    const uint32_t c = __float_as_uint(fmaf(s, 16384.f, 12582912.f));
+    return s != s ? (uint16_t)0x8000 : (uint16_t)c;
 }
 __device__ __forceinline__ float slope_value(int16_t c) {
     return c == -32768 ? __int_as_float(0x7fc00000) : (float)c * kSlopeUnit;
@@ -162,6 +175,10 @@ struct Product {
 
 // `clear`: the kernel sets *status to 0 first (the first product of a call); `probe`: SPMM_CFG_EXPIRE_FIRST_WAIT.
 int launch_product(const Product &p, bool clear, bool probe, cudaStream_t s);
+
+// The same for at most four rows per group on average (operands aligned, see skinny_fits).
+bool skinny_fits(const Product &p);
+int launch_skinny(const Product &p, bool clear, cudaStream_t s);
 
 // out[t] = sum_j weight * src[slots[t][j]] over float32 rows (the gradient of gathered rows).
 int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,

@@ -1,0 +1,226 @@
+// linear_skinny.cu -- products of a handful of rows: y[q][p] = sum_r A[p][r] B[q][r]
+// for one to four q per group, the single tokens of a decoding step.
+//
+// Every value of A (the weights) is used once per row, so the time is that of
+// reading A; what counts is many independent 16-byte loads from the first
+// microsecond on.  Plain loads and FMAs do that with less start-up than a ring
+// of bulk copies, barriers and tensor memory: 1 x 4096 x 4096 takes 7 us where
+// the tensor-core kernel needs 13.
+//
+// r contiguous: KS of a CTA's 8 warps share 4 p and take 256 r each in turn, a
+// lane 8 of them (KS = 1 where there are warps enough without: sharing costs a
+// barrier and leaves a warp little to stream).  p contiguous: a CTA owns 32 p; 4 lanes cover them, so a warp reads 8
+// rows r of 64 bytes at once and 16 warps take 128 r in turn.  Sums over lanes
+// by shuffles, over warps in shared memory, in a fixed order.
+#include "linear.cuh"
+
+namespace spmm {
+namespace {
+
+struct Rows {
+    int64_t q0, q1;
+    bool zero;
+};
+
+__device__ __forceinline__ Rows group_rows(const Product &p, int64_t g) {
+    if (!p.offsets) return {0, p.Q, false};
+    const int64_t a = group_first(p.offsets, g, p.Q), b = g < p.groups ? group_first(p.offsets, g + 1, p.Q) : p.Q;
+    return {a, b, g == p.groups};
+}
+
+template <typename T, typename O, int ACT>
+__device__ __forceinline__ void put_act(const Product &p, int64_t q, int64_t pp, float z) {
+    float d, y = activate<ACT, true>(z, d);
+    if (p.residual) y += to_f32(((const T *)p.residual)[q * p.residual_ld + pp]);
+    ((O *)p.C)[q * p.c_q + pp] = from_f32<O>(y);
+    if (p.slope) p.slope[q * p.P + pp] = (int16_t)slope_code(d);
+}
+
+template <typename T, typename O>
+__device__ __forceinline__ void put(const Product &p, int64_t g, int64_t q, int64_t pp, float z) {
+    if (p.bias) z += to_f32(((const T *)p.bias)[g * p.bias_g + pp]);
+    switch (p.act) {
+        case SPMM_ACT_NONE: put_act<T, O, SPMM_ACT_NONE>(p, q, pp, z); break;
+        case SPMM_ACT_RELU: put_act<T, O, SPMM_ACT_RELU>(p, q, pp, z); break;
+        case SPMM_ACT_GELU: put_act<T, O, SPMM_ACT_GELU>(p, q, pp, z); break;
+        case SPMM_ACT_GELU_TANH: put_act<T, O, SPMM_ACT_GELU_TANH>(p, q, pp, z); break;
+        default: put_act<T, O, SPMM_ACT_SILU>(p, q, pp, z); break;
+    }
+}
+
+// Rows behind the last group: zeros at this CTA's p.
+template <typename O>
+__device__ __forceinline__ void put_zeros(const Product &p, Rows w, int64_t p0, int np) {
+    for (int64_t i = threadIdx.x; i < (w.q1 - w.q0) * np; i += blockDim.x) {
+        const int64_t q = w.q0 + i / np, pp = p0 + i % np;
+        if (pp < p.P) {
+            ((O *)p.C)[q * p.c_q + pp] = from_f32<O>(0.f);
+            if (p.slope) p.slope[q * p.P + pp] = 0;
+        }
+    }
+}
+
+constexpr int kNP = 4;      // p of a CTA, r contiguous
+
+template <typename T, typename O, int R, int KS>
+__device__ __forceinline__ void rows_rmajor(const Product &p, int64_t g, int64_t q, int64_t p0, float *sm) {
+    const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % KS;
+    const T *A = (const T *)p.A + g * p.a_g, *B = (const T *)p.B + q * p.b_q;
+    const T *a[kNP];
+#pragma unroll
+    for (int i = 0; i < kNP; ++i) a[i] = A + (p0 + i < p.P ? p0 + i : p.P - 1) * p.a_p;
+    float acc[kNP][R] = {};
+#pragma unroll 2
+    for (int64_t r = part * 256 + lane * 8; r < p.R; r += KS * 256) {
+        uint4 w[kNP], x[R];
+#pragma unroll
+        for (int i = 0; i < kNP; ++i) w[i] = __ldg((const uint4 *)(a[i] + r));
+#pragma unroll
+        for (int j = 0; j < R; ++j) x[j] = __ldg((const uint4 *)(B + j * p.b_q + r));
+        float xf[R][8];
+#pragma unroll
+        for (int j = 0; j < R; ++j) unpack8<T>(x[j], xf[j]);
+#pragma unroll
+        for (int i = 0; i < kNP; ++i) {
+            float wf[8];
+            unpack8<T>(w[i], wf);
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[i][j] = fmaf(wf[e], xf[j][e], acc[i][j]);
+        }
+    }
+    float z = 0.f;           // lane i * R + j: sum (i, j)
+#pragma unroll
+    for (int i = 0; i < kNP; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            float v = acc[i][j];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+            if (lane == i * R + j) z = v;
+        }
+    const int64_t pp = p0 + lane / R;
+    if constexpr (KS > 1) {
+        const int warp = threadIdx.x >> 5;
+        if (lane < kNP * R) sm[warp * (kNP * R) + lane] = z;
+        __syncthreads();
+        if (part == 0 && lane < kNP * R) {
+            z = 0.f;
+#pragma unroll
+            for (int w = 0; w < KS; ++w) z += sm[(warp + w) * (kNP * R) + lane];
+        }
+    }
+    if (part == 0 && lane < kNP * R && pp < p.P) put<T, O>(p, g, q + lane % R, pp, z);
+    if constexpr (KS > 1) __syncthreads();
+}
+
+template <typename T, typename O, int KS>
+__global__ void __launch_bounds__(256) skinny_rmajor_kernel(const __grid_constant__ Product p, int clear) {
+    __shared__ float sm[8 * kNP * 4];
+    if (clear && p.status && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = 0;
+    const int64_t g = blockIdx.y;
+    const Rows w = group_rows(p, g);
+    if (w.zero) return put_zeros<O>(p, w, (int64_t)blockIdx.x * (kNP * 8 / KS), kNP * 8 / KS);
+    int64_t p0 = ((int64_t)blockIdx.x * (8 / KS) + (threadIdx.x >> 5) / KS) * kNP;
+    if (p0 >= p.P) {
+        if constexpr (KS == 1) return;
+        p0 = (p.P - 1) / kNP * kNP;          // walks along for the barriers, computing the last p once more
+    }
+    for (int64_t q = w.q0; q < w.q1;) {
+        const int64_t n = w.q1 - q;
+        if (n >= 4) rows_rmajor<T, O, 4, KS>(p, g, q, p0, sm), q += 4;
+        else if (n == 3) rows_rmajor<T, O, 3, KS>(p, g, q, p0, sm), q += 3;
+        else if (n == 2) rows_rmajor<T, O, 2, KS>(p, g, q, p0, sm), q += 2;
+        else rows_rmajor<T, O, 1, KS>(p, g, q, p0, sm), q += 1;
+    }
+}
+
+constexpr int kWP = 32;     // p of a CTA, p contiguous
+constexpr int kWarps = 16;
+
+template <typename T, typename O, int R>
+__device__ __forceinline__ void rows_pmajor(const Product &p, int64_t g, int64_t q, int64_t p0, float *sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t pl = p0 + (lane & 3) * 8;
+    const T *A = (const T *)p.A + g * p.a_g + (pl + 8 <= p.P ? pl : 0), *B = (const T *)p.B + q * p.b_q;
+    float acc[R][8] = {};
+#pragma unroll 4
+    for (int64_t r = warp * 8 + (lane >> 2); r < p.R; r += kWarps * 8) {
+        const uint4 w = __ldg((const uint4 *)(A + r * p.a_r));
+        float x[R], wf[8];
+#pragma unroll
+        for (int j = 0; j < R; ++j) x[j] = to_f32(B[j * p.b_q + r]);
+        unpack8<T>(w, wf);
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[j][e] = fmaf(wf[e], x[j], acc[j][e]);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v = acc[j][e];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(kFullMask, v, o);
+            if (lane < 4) sm[(warp * R + j) * kWP + lane * 8 + e] = v;
+        }
+    __syncthreads();
+    if (threadIdx.x < kWP * R) {
+        float z = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) z += sm[w * R * kWP + threadIdx.x];
+        const int64_t pp = p0 + threadIdx.x % kWP;
+        if (pp < p.P) put<T, O>(p, g, q + threadIdx.x / kWP, pp, z);
+    }
+    __syncthreads();
+}
+
+template <typename T, typename O>
+__global__ void __launch_bounds__(kWarps * 32) skinny_pmajor_kernel(const __grid_constant__ Product p, int clear) {
+    __shared__ float sm[kWarps * 4 * kWP];
+    if (clear && p.status && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = 0;
+    const int64_t g = blockIdx.y, p0 = (int64_t)blockIdx.x * kWP;
+    const Rows w = group_rows(p, g);
+    if (w.zero) return put_zeros<O>(p, w, p0, kWP);
+    for (int64_t q = w.q0; q < w.q1;) {
+        const int64_t n = w.q1 - q;
+        if (n >= 4) rows_pmajor<T, O, 4>(p, g, q, p0, sm), q += 4;
+        else if (n == 3) rows_pmajor<T, O, 3>(p, g, q, p0, sm), q += 3;
+        else if (n == 2) rows_pmajor<T, O, 2>(p, g, q, p0, sm), q += 2;
+        else rows_pmajor<T, O, 1>(p, g, q, p0, sm), q += 1;
+    }
+}
+
+template <typename T, typename O>
+int run(const Product &p, bool clear, cudaStream_t s) {
+    const unsigned gy = (unsigned)(p.offsets ? p.groups + 1 : 1);
+    if (p.a_r == 1) {
+        // warps of the whole call without sharing: 148 SMs hold about 4,700 at once
+        const int64_t quads = ceil_div(p.P, kNP), warps = quads * (p.Q < p.groups ? p.Q : p.groups);
+        if (warps >= 4096 || p.R <= 256)
+            skinny_rmajor_kernel<T, O, 1><<<dim3((unsigned)ceil_div(quads, 8), gy), 256, 0, s>>>(p, clear);
+        else if (warps >= 2048 || p.R <= 512)
+            skinny_rmajor_kernel<T, O, 2><<<dim3((unsigned)ceil_div(quads, 4), gy), 256, 0, s>>>(p, clear);
+        else
+            skinny_rmajor_kernel<T, O, 8><<<dim3((unsigned)quads, gy), 256, 0, s>>>(p, clear);
+    } else
+        skinny_pmajor_kernel<T, O><<<dim3((unsigned)ceil_div(p.P, kWP), gy), kWarps * 32, 0, s>>>(p, clear);
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
+}
+
+}  // namespace
+
+bool skinny_fits(const Product &p) {
+    if (p.red || p.Q > 4 * p.groups || p.b_r != 1) return false;
+    return p.a_r == 1 ? p.R % 8 == 0 : p.P % 8 == 0;
+}
+
+int launch_skinny(const Product &p, bool clear, cudaStream_t s) {
+    if (p.f16) return p.out_f32 ? run<__half, float>(p, clear, s) : run<__half, __half>(p, clear, s);
+    return p.out_f32 ? run<__nv_bfloat16, float>(p, clear, s) : run<__nv_bfloat16, __nv_bfloat16>(p, clear, s);
+}
+
+}  // namespace spmm

@@ -27,6 +27,9 @@
 // returns.
 #include <cuda.h>
 
+#include <atomic>
+#include <cmath>
+
 #include "linear.cuh"
 #include "ptx.cuh"
 
@@ -36,7 +39,9 @@ namespace {
 constexpr int kR = 64;              // r per stage: 128 bytes
 constexpr int kP = 128;             // p per CTA
 constexpr int kChunk = kR * 128;    // bytes of 64 rows of 128 bytes
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;     // 4 warps of roles, 8 of the epilogue
+constexpr int kEpiWarps = 8;
+constexpr int kPiece = kP * 36;     // floats of 32 columns of partial sums: 36 a row keeps 16-byte accesses apart
 constexpr int kBand = 8;            // q tiles that one sweep over p covers
 
 struct Maps {
@@ -46,7 +51,8 @@ struct Maps {
 struct TcArgs {
     Product p;
     int32_t a_kmajor, b_kmajor, a_grouped;   // a_grouped: the group is A's third coordinate
-    int32_t bf16, clear_status, expire_probe;
+    int32_t bf16, clear_status, expire_probe, splits;
+    int32_t vec_out, vec_slope, vec_residual;   // 16-byte aligned rows
 };
 
 template <int CG, int BQ>
@@ -54,11 +60,14 @@ struct Shape {
     static constexpr int kBRows = BQ / CG;                    // B rows of one CTA
     static constexpr int kStageBytes = kP * 128 + kBRows * 128;
     static constexpr int kStages = CG == 2 ? 6 : BQ == 256 ? 4 : BQ == 128 ? 6 : 8;
-    static constexpr int kBoxQ = kBRows < 64 ? kBRows : 64;   // rows of a K-major B box
+    // Rows of a K-major B box.  Few rows come in boxes of 16: one token then costs 2 KB a stage, not 8.
+    static constexpr int kBoxQ = BQ == 64 ? 16 : 64;
     static constexpr int kTmem = 2 * BQ;
     static constexpr int kTable = 2 * (SPMM_MAX_GROUPS + 2) * 4;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kTable + 512;
+    static constexpr int kRing = kStages * kStageBytes, kOut = kEpiWarps * 2048;
+    static constexpr int kSmem = 1024 + kRing + kOut + kTable + 512;
     static_assert(BQ % 64 == 0 && kTmem >= 32 && kTmem <= 512, "accumulators");
+    static_assert(BQ / 32 * kPiece * 4 <= kRing, "partial sums fit the ring");
     static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -71,12 +80,23 @@ struct Tile {
 
 struct Bars {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drain, never;
+    // Pairs, for a ragged last step in a stage: this CTA's copies have landed; the second CTA has zeroed its
+    // rows.  One per stage, as several short groups' last steps can be in the ring at once.
+    uint64_t tail[8], peer[8];
     uint32_t tmem;
     volatile int abort;
 };
 
 // ---- PTX ------------------------------------------------------------------------
 
+// One lane of a converged warp.  The compiler keeps operands of the issuing
+// instructions in uniform registers only behind an election: with `lane == 0`
+// four MMAs and a commit took 680 cycles to issue instead of under 100.
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -92,6 +112,13 @@ __device__ __forceinline__ void cluster_sync() {
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+    float4 f;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                 : "r"(addr));
+    return f;
 }
 template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
@@ -136,12 +163,12 @@ __device__ __forceinline__ void commit_local(uint64_t *bar) {
 }
 // Arrives on `bar` (of both CTAs of a pair) when the MMAs issued before are done.
 template <int CG>
-__device__ __forceinline__ void commit(uint64_t *bar) {
+__device__ __forceinline__ void commit(uint64_t *bar, uint16_t mask) {
     if constexpr (CG == 2)
         asm volatile(
             "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
                 smem_u32(bar)),
-            "h"((uint16_t)3)
+            "h"(mask)
             : "memory");
     else
         mma_commit(bar);
@@ -191,6 +218,10 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, Bars &s
             return false;
         }
     }
+}
+// The same for a converged warp: one answer for all lanes, so that they stay converged.
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, Bars &s, const TcArgs &a) {
+    return __all_sync(kFullMask, wait_bar(bar, parity, s, a));
 }
 // The same without the abort flag: for copies and MMAs already in flight.
 __device__ __forceinline__ bool drain_bar(uint64_t *bar, uint32_t parity) {
@@ -309,6 +340,14 @@ __device__ __forceinline__ bool get_tile(const Product &p, Table t, int64_t i, T
     return true;
 }
 
+// Part `part` of `splits` of a tile's steps.
+__device__ __forceinline__ void cut(Tile &t, int splits, int part) {
+    const int a = t.steps * part / splits, b = t.steps * (part + 1) / splits;
+    if (b < t.steps) t.last = 0;
+    t.r0 += (int64_t)a * kR;
+    t.steps = b - a;
+}
+
 // MMA columns of a tile: a multiple of 16 (of 32 for a pair, half from each CTA).
 template <int CG>
 __device__ __forceinline__ int mma_cols(int nq) {
@@ -317,75 +356,244 @@ __device__ __forceinline__ int mma_cols(int nq) {
 
 // ---- epilogue -----------------------------------------------------------------------
 
-template <typename T, typename O, int ACT>
-__device__ __forceinline__ void store_columns(const Product &p, const Tile &t, int64_t pp, float bias,
-                                              const uint32_t (&v)[32], int c0) {
-    const int n = t.nq - c0 < 32 ? t.nq - c0 : 32;
-    const int64_t q = t.q0 + c0;
-    O *out = (O *)p.C + (p.red ? t.group * p.c_g : 0) + q * p.c_q + pp;
-    const T *res = p.residual ? (const T *)p.residual + q * p.residual_ld + pp : nullptr;
-    int16_t *slope = p.slope ? p.slope + q * p.P + pp : nullptr;
+// A warp's 32 x 32 piece of the result goes through 2 KB of shared memory, so
+// that it leaves as 16-byte stores of 64 contiguous bytes a row: 2-byte stores
+// straight from the accumulator's layout (lane = p) cost 15 cycles each, 15,500
+// a 128 x 256 tile, as much as summing it over 2048.
+//
+// put(j) gives this lane's value of column j; the values of columns [0, n) are
+// stored at base + j * ld (lane 0's first).  `cols`: valid p from lane 0's on.
+template <typename O, typename F>
+__device__ __forceinline__ void store_piece(uint8_t *stage, O *base, int64_t ld, bool vec, int cols, int n, F put) {
+    constexpr int kPass = 2048 / (32 * sizeof(O));      // columns per pass
+    constexpr int kPer = 16 / sizeof(O), kLanes = 32 / kPer, kRows = 32 / kLanes;
+    const int lane = threadIdx.x & 31;
+    const int row = lane / kLanes, at = (lane % kLanes) * kPer;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        if (j >= n) break;
-        ActValue a = activate<ACT>(__uint_as_float(v[j]) + bias);
-        if (res) a.y += to_f32(res[j * p.residual_ld]);
-        if (t.zero) a.y = a.slope = 0.f;
-        out[j * p.c_q] = from_f32<O>(a.y);
-        if (slope) slope[j * p.P] = slope_code(a.slope);
+    for (int j0 = 0; j0 < 32; j0 += kPass) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kPass; ++j) ((O *)stage)[j * 32 + lane] = put(j0 + j);
+        __syncwarp();
+        if (vec && at + kPer <= cols) {
+#pragma unroll
+            for (int j = row; j < kPass; j += kRows) {
+                const uint4 v = *(const uint4 *)((O *)stage + j * 32 + at);
+                if (j0 + j < n) *(uint4 *)(base + (int64_t)(j0 + j) * ld + at) = v;
+            }
+        } else {                 // unaligned results and the last, partial 16 bytes
+            for (int j = row; j < kPass; j += kRows)
+                for (int e = 0; e < kPer; ++e)
+                    if (j0 + j < n && at + e < cols) base[(int64_t)(j0 + j) * ld + at + e] = ((O *)stage)[j * 32 + at + e];
+        }
     }
 }
 
-template <typename T, typename O>
-__device__ __forceinline__ void epilogue(const Product &p, const Tile &t, int64_t pp, uint32_t tmem, bool have) {
-    float bias = 0.f;
-    const bool in = pp < p.P;
-    if (in && p.bias && !t.zero) bias = to_f32(((const T *)p.bias)[t.group * p.bias_g + pp]);
-    for (int c0 = 0; c0 < t.nq; c0 += 32) {
-        uint32_t v[32];
-        if (have) {
-            __syncwarp();
-            tmem_ld32(tmem + c0, v);
-            tmem_wait_ld();
-        } else {
+// The other way: r[j] = column j's value at this lane, from base + j * ld.
+template <typename T>
+__device__ __forceinline__ void load_piece(uint8_t *stage, const T *base, int64_t ld, bool vec, int cols, int n,
+                                           float (&r)[32]) {
+    const int lane = threadIdx.x & 31, row = lane / 4, at = (lane % 4) * 8;
+    __syncwarp();
+    if (vec && at + 8 <= cols) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0u;
-        }
-        if (in) switch (p.act) {
-            case SPMM_ACT_NONE: store_columns<T, O, SPMM_ACT_NONE>(p, t, pp, bias, v, c0); break;
-            case SPMM_ACT_RELU: store_columns<T, O, SPMM_ACT_RELU>(p, t, pp, bias, v, c0); break;
-            case SPMM_ACT_GELU: store_columns<T, O, SPMM_ACT_GELU>(p, t, pp, bias, v, c0); break;
-            case SPMM_ACT_GELU_TANH: store_columns<T, O, SPMM_ACT_GELU_TANH>(p, t, pp, bias, v, c0); break;
-            default: store_columns<T, O, SPMM_ACT_SILU>(p, t, pp, bias, v, c0); break;
+        for (int j = row; j < 32; j += 8)
+            if (j < n) *(uint4 *)((T *)stage + j * 32 + at) = __ldg((const uint4 *)(base + (int64_t)j * ld + at));
+    } else {
+        for (int j = row; j < 32; j += 8)
+            for (int e = 0; e < 8; ++e)
+                if (j < n && at + e < cols) ((T *)stage)[j * 32 + at + e] = base[(int64_t)j * ld + at + e];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = to_f32(((const T *)stage)[j * 32 + lane]);
+}
+
+// Columns [c0, c0 + n) of a tile, n <= 32, for the warp whose first p is p0: v[j] is column c0 + j at this lane.
+template <typename T, typename O, int ACT, bool SLOPE>
+__device__ __forceinline__ void store_columns(const TcArgs &a, const Tile &t, uint8_t *stage, int64_t p0, float bias,
+                                              const float (&v)[32], int c0, int n) {
+    const Product &p = a.p;
+    const int64_t q = t.q0 + c0;
+    const int cols = p.P - p0 < 32 ? (int)(p.P - p0) : 32;
+    float y[32], d[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = activate<ACT, SLOPE>(v[j] + bias, d[j]);
+    if (p.residual) {
+        float r[32];
+        load_piece<T>(stage, (const T *)p.residual + q * p.residual_ld + p0, p.residual_ld, a.vec_residual, cols, n, r);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] += r[j];
+    }
+    store_piece<O>(stage, (O *)p.C + (p.red ? t.group * p.c_g : 0) + q * p.c_q + p0, p.c_q, a.vec_out, cols, n,
+                   [&](int j) { return from_f32<O>(y[j]); });
+    if constexpr (SLOPE)
+        store_piece<uint16_t>(stage, (uint16_t *)p.slope + q * p.P + p0, p.P, a.vec_slope, cols, n,
+                              [&](int j) { return slope_code(d[j]); });
+}
+
+template <typename T, typename O, int ACT>
+__device__ __forceinline__ void store_act(const TcArgs &a, const Tile &t, uint8_t *stage, int64_t p0, float bias,
+                                          const float (&v)[32], int c0, int n) {
+    if (a.p.slope) store_columns<T, O, ACT, true>(a, t, stage, p0, bias, v, c0, n);
+    else store_columns<T, O, ACT, false>(a, t, stage, p0, bias, v, c0, n);
+}
+
+template <typename T, typename O>
+__device__ __forceinline__ void finish_columns(const TcArgs &a, const Tile &t, uint8_t *stage, int64_t p0, float bias,
+                                               const float (&v)[32], int c0, int end) {
+    const Product &p = a.p;
+    if (p0 >= p.P) return;
+    const int n = end - c0 < 32 ? end - c0 : 32;
+    if (t.zero) {
+        const int64_t q = t.q0 + c0, pp = p0 + (threadIdx.x & 31);
+        if (pp < p.P)
+            for (int j = 0; j < n; ++j) {
+                ((O *)p.C)[(q + j) * p.c_q + pp] = from_f32<O>(0.f);
+                if (p.slope) p.slope[(q + j) * p.P + pp] = 0;
+            }
+        return;
+    }
+    if constexpr (sizeof(O) == 4) {     // the float32 result is a plain product
+        store_columns<T, O, SPMM_ACT_NONE, false>(a, t, stage, p0, bias, v, c0, n);
+    } else {
+        switch (p.act) {
+            case SPMM_ACT_NONE: store_columns<T, O, SPMM_ACT_NONE, false>(a, t, stage, p0, bias, v, c0, n); break;
+            case SPMM_ACT_RELU: store_act<T, O, SPMM_ACT_RELU>(a, t, stage, p0, bias, v, c0, n); break;
+            case SPMM_ACT_GELU: store_act<T, O, SPMM_ACT_GELU>(a, t, stage, p0, bias, v, c0, n); break;
+            case SPMM_ACT_GELU_TANH: store_act<T, O, SPMM_ACT_GELU_TANH>(a, t, stage, p0, bias, v, c0, n); break;
+            default: store_act<T, O, SPMM_ACT_SILU>(a, t, stage, p0, bias, v, c0, n); break;
         }
     }
+}
+
+// 32 columns from c0 of the accumulator at `tmem` (zeros where nothing was summed).  The whole warp.
+__device__ __forceinline__ void read_columns(uint32_t tmem, bool have, float (&v)[32]) {
+    __syncwarp();
+    uint32_t u[32];
+    if (have) {
+        tmem_ld32(tmem, u);
+        tmem_wait_ld();
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) u[j] = 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]);
+}
+
+template <typename T>
+__device__ __forceinline__ float load_bias(const Product &p, const Tile &t, int64_t pp) {
+    return p.bias && !t.zero && pp < p.P ? to_f32(((const T *)p.bias)[t.group * p.bias_g + pp]) : 0.f;
 }
 
 // ---- the kernel -----------------------------------------------------------------------
 
-template <int CG, int BQ, typename T, typename O>
+// Zeros in rows [last, next multiple of 16) of a stage of 64-row chunks, visible to the MMAs.  A whole warp.
+__device__ __forceinline__ void zero_rows(uint8_t *stage, int bytes, int last) {
+    const int rows = ((last + 15) & ~15) - last;
+    for (int c = 0; c < bytes; c += kChunk)
+        for (int x = threadIdx.x & 31; x < rows * 8; x += 32)
+            *(uint4 *)(stage + c + last * 128 + x * 16) = uint4{0, 0, 0, 0};
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// The producer: a step's boxes into the next stage of the ring.  Called by the
+// whole warp, an elected lane issues.
+template <int CG, int BQ>
+struct Loader {
+    const Maps &maps;
+    const TcArgs &a;
+    Bars &s;
+    uint8_t *ring;
+    uint32_t rank, lead;
+    uint32_t n, st, ph;      // steps issued; the next stage and its phase
+    uint32_t tails, odd;     // pairs: bit st, whether stage st has held a ragged last step; an odd number of them
+
+    __device__ __forceinline__ void step(const Tile &t, int k) {
+        using Sh = Shape<CG, BQ>;
+        if (elect()) {
+            const int mine = mma_cols<CG>(t.nq) / CG, box_rows = a.b_kmajor ? Sh::kBoxQ : 64;   // B rows of this CTA
+            const int boxes = (mine + box_rows - 1) / box_rows;
+            const uint32_t bytes = kP * 128 + boxes * box_rows * 128;
+            const int32_t pa = (int32_t)(t.p0 + rank * kP), qb = (int32_t)(t.q0 + rank * mine);
+            const int32_t g = a.a_grouped ? (int32_t)t.group : 0, r = (int32_t)(t.r0 + (int64_t)k * kR);
+            uint32_t bar = smem_u32(&s.full[st]);
+            if (CG == 2 && t.last && k == t.steps - 1) {   // each CTA has rows to zero first
+                bar = smem_u32(&s.tail[st]);
+                mbar_arrive_expect_tx(&s.tail[st], bytes);
+                if (rank == 0) mbar_arrive(&s.full[st]);
+            } else {
+                if (rank == 0) mbar_arrive_expect_tx(&s.full[st], bytes * CG);
+                if constexpr (CG == 2) bar = map_cta(bar, lead);
+            }
+            const uint32_t dst = smem_u32(ring + st * Sh::kStageBytes), db = dst + kP * 128;
+            if (a.a_kmajor) {
+                tma_load<CG>(dst, &maps.a, r, pa, g, bar);
+            } else {
+                tma_load<CG>(dst, &maps.a, pa, r, g, bar);
+                tma_load<CG>(dst + kChunk, &maps.a, pa + 64, r, g, bar);
+            }
+            if (a.b_kmajor) {
+#pragma unroll
+                for (int b = 0; b < Sh::kBRows / Sh::kBoxQ; ++b)
+                    if (b < boxes) tma_load<CG>(db + b * Sh::kBoxQ * 128, &maps.b, r, qb + b * Sh::kBoxQ, 0, bar);
+            } else {
+#pragma unroll
+                for (int b = 0; b < Sh::kBRows / 64; ++b)
+                    if (b < boxes) tma_load<CG>(db + b * kChunk, &maps.b, qb + b * 64, r, 0, bar);
+            }
+        }
+        __syncwarp();
+        if (CG == 2 && t.last && k == t.steps - 1) {
+            tails |= 1u << st;
+            odd ^= 1u << st;
+        }
+        ++n;
+        if (++st == Sh::kStages) {
+            st = 0;
+            ph ^= 1;
+        }
+    }
+};
+
+// SPLIT: a cluster of `splits` CTAs (pairs) shares one tile, each sums a part of
+// r, and the parts meet in shared memory: every CTA finishes a slice of the
+// columns, adding the parts in order.  One tile per cluster.
+template <int CG, int BQ, bool SPLIT, typename T, typename O>
 __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Maps maps,
                                                          const __grid_constant__ TcArgs a) {
     using Sh = Shape<CG, BQ>;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     Table table;
-    table.first = (int32_t *)(ring + Sh::kStages * Sh::kStageBytes);
+    uint8_t *stages = ring + Sh::kRing;      // the epilogue warps' 2 KB each
+    table.first = (int32_t *)(stages + Sh::kOut);
     table.qtiles = table.first + SPMM_MAX_GROUPS + 2;
     Bars &s = *(Bars *)((uint8_t *)table.first + Sh::kTable);
     const Product &p = a.p;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-    const int64_t first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+    const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t crank = CG == 2 || SPLIT ? cluster_rank() : 0;
+    const uint32_t rank = crank % CG, lead = crank - rank;     // within the pair; the pair's first CTA
+    const int splits = SPLIT ? a.splits : 1, part = SPLIT ? (int)(crank / CG) : 0;
+    const int64_t first_tile = blockIdx.x / (CG * splits);
+    const int64_t tile_step = SPLIT ? INT64_MAX / 2 : gridDim.x / CG;
 
     if (threadIdx.x == 0) {
+        if (p.R > 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
+        }
         for (int i = 0; i < Sh::kStages; ++i) {
             mbar_init(&s.full[i], 1);
             mbar_init(&s.empty[i], 1);
+            mbar_init(&s.tail[i], 1);
+            mbar_init(&s.peer[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.acc_full[i], 1);
-            mbar_init(&s.acc_empty[i], 4 * CG);
+            mbar_init(&s.acc_empty[i], kEpiWarps * CG);
         }
         mbar_init(&s.drain, 1);
         mbar_init(&s.never, 1);
@@ -394,143 +602,222 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         if (a.clear_status && blockIdx.x == 0 && p.status) *p.status = 0;
     }
     if (warp == 2) alloc_tmem<CG>(&s.tmem, Sh::kTmem);
+    Loader<CG, BQ> load{maps, a, s, ring, rank, lead, 0, 0, 0, 0, 0};
+    Tile t;
+    if (CG == 1 && warp == 0 && !p.offsets && !a.expire_probe) {   // fill the ring before anything else is ready
+        __syncwarp();
+        if (get_tile<CG, BQ>(p, table, first_tile, t)) {
+            if constexpr (SPLIT) cut(t, splits, part);
+            for (int k = 0; k < t.steps && k < Sh::kStages; ++k) load.step(t, k);
+        }
+    }
     fill_table<BQ>(p, table);
     tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2) cluster_sync();
+    if constexpr (CG == 2 || SPLIT) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    Tile t;
+    bool mine = false;       // SPLIT: this cluster has a tile
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t n = 0;      // steps issued
-            bool ok = true;
-            if (a.expire_probe) ok = wait_bar(&s.never, 0u, s, a);
-            for (int64_t i = first_tile; ok && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
-                const int cols = mma_cols<CG>(t.nq), mine = cols / CG;    // B rows of this CTA
-                const int boxes = (mine + (a.b_kmajor ? Sh::kBoxQ : 64) - 1) / (a.b_kmajor ? Sh::kBoxQ : 64);
-                const uint32_t bytes = kP * 128 + boxes * (a.b_kmajor ? Sh::kBoxQ * 128 : kChunk);
-                const int32_t pa = (int32_t)(t.p0 + rank * kP), qb = (int32_t)(t.q0 + rank * mine);
-                const int32_t g = a.a_grouped ? (int32_t)t.group : 0;
-                for (int k = 0; k < t.steps; ++k, ++n) {
-                    const uint32_t st = n % Sh::kStages, ph = (n / Sh::kStages) & 1;
-                    if (!wait_bar(&s.empty[st], ph ^ 1, s, a)) {
-                        ok = false;
-                        break;
-                    }
-                    uint32_t bar = smem_u32(&s.full[st]);
-                    if (rank == 0) mbar_arrive_expect_tx(&s.full[st], bytes * CG);
-                    if constexpr (CG == 2) bar = map_cta(bar, 0);
-                    const uint32_t dst = smem_u32(ring + st * Sh::kStageBytes);
-                    const int32_t r = (int32_t)(t.r0 + (int64_t)k * kR);
-                    if (a.a_kmajor) {
-                        tma_load<CG>(dst, &maps.a, r, pa, g, bar);
-                    } else {
-                        tma_load<CG>(dst, &maps.a, pa, r, g, bar);
-                        tma_load<CG>(dst + kChunk, &maps.a, pa + 64, r, g, bar);
-                    }
-                    for (int b = 0; b < boxes; ++b) {
-                        const uint32_t d = dst + kP * 128;
-                        if (a.b_kmajor) tma_load<CG>(d + b * Sh::kBoxQ * 128, &maps.b, r, qb + b * Sh::kBoxQ, 0, bar);
-                        else tma_load<CG>(d + b * kChunk, &maps.b, qb + b * 64, r, 0, bar);
-                    }
+        bool ok = true;
+        if (a.expire_probe) ok = wait_warp(&s.never, 0u, s, a);
+        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
+            if constexpr (SPLIT) cut(t, splits, part);
+            for (int k = i == first_tile ? (int)load.n : 0; k < t.steps; ++k) {
+                if (!wait_warp(&s.empty[load.st], load.ph ^ 1, s, a)) {
+                    ok = false;
+                    break;
                 }
+                load.step(t, k);
             }
-            if (ok) {               // every stage has been read: nothing arrives here after the CTA has left
-                for (uint32_t m = n > Sh::kStages ? n - Sh::kStages : 0; m < n; ++m)
-                    if (!wait_bar(&s.empty[m % Sh::kStages], (m / Sh::kStages) & 1, s, a)) {
-                        ok = false;
-                        break;
-                    }
-            }
-            if (!ok && rank == 0)   // copies in flight land before the CTA leaves
-                for (uint32_t m = n > Sh::kStages ? n - Sh::kStages : 0; m < n; ++m)
-                    if (!drain_bar(&s.full[m % Sh::kStages], (m / Sh::kStages) & 1)) break;
         }
+        const uint32_t n = load.n;
+        if (ok) {               // every stage has been read: nothing arrives here after the CTA has left
+            for (uint32_t m = n > Sh::kStages ? n - Sh::kStages : 0; m < n; ++m)
+                if (!wait_warp(&s.empty[m % Sh::kStages], (m / Sh::kStages) & 1, s, a)) {
+                    ok = false;
+                    break;
+                }
+        }
+        for (int i = 0; !ok && i < Sh::kStages; ++i)
+            if (load.tails >> i & 1) drain_bar(&s.tail[i], load.odd >> i & 1 ^ 1);
+        if (!ok && rank == 0)   // copies in flight land before the CTA leaves
+            for (uint32_t m = n > Sh::kStages ? n - Sh::kStages : 0; m < n; ++m)
+                if (!drain_bar(&s.full[m % Sh::kStages], (m / Sh::kStages) & 1)) break;
         __syncwarp();
     } else if (warp == 1 && rank == 0) {
-        uint32_t n = 0, acc = 0;   // steps, accumulators used
+        const uint16_t both = (uint16_t)(3u << lead);
+        uint32_t acc = 0, st = 0, ph = 0, odd = 0;   // accumulators used; stage and its phase; see Loader
         bool ok = true, issued = false;
         const uint32_t idesc0 = (1u << 4) | ((uint32_t)a.bf16 << 7) | ((uint32_t)a.bf16 << 10) |
                                 ((a.a_kmajor ? 0u : 1u) << 15) | ((a.b_kmajor ? 0u : 1u) << 16) |
                                 ((uint32_t)(kP * CG >> 4) << 24);
         const uint32_t a_adv = (a.a_kmajor ? 32 : 2048) >> 4, b_adv = (a.b_kmajor ? 32 : 2048) >> 4;
         for (int64_t i = first_tile; ok && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
+            if constexpr (SPLIT) cut(t, splits, part);
             if (t.steps == 0) continue;
             const uint32_t as = acc & 1, ap = (acc >> 1) & 1;
             ++acc;
-            if (lane == 0) ok = wait_bar(&s.acc_empty[as], ap ^ 1, s, a);
-            ok = __shfl_sync(kFullMask, ok, 0);
+            ok = wait_warp(&s.acc_empty[as], ap ^ 1, s, a);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t idesc = idesc0 | ((uint32_t)(mma_cols<CG>(t.nq) >> 3) << 17);
-            for (int k = 0; k < t.steps; ++k, ++n) {
-                const uint32_t st = n % Sh::kStages, ph = (n / Sh::kStages) & 1;
-                if (lane == 0) ok = wait_bar(&s.full[st], ph, s, a);
-                ok = __shfl_sync(kFullMask, ok, 0);
+            const uint32_t idesc = idesc0 | ((uint32_t)(mma_cols<CG>(t.nq) >> 3) << 17), d = tmem + as * BQ;
+            for (int k = 0; k < t.steps; ++k) {
+                ok = wait_warp(&s.full[st], ph, s, a);
                 if (!ok) break;
                 uint8_t *sa = ring + st * Sh::kStageBytes;
                 int chunks = kR / 16;
                 if (t.last && k == t.steps - 1) {   // rows behind the group: zeros up to the MMA's 16
                     chunks = (t.last + 15) / 16;
-                    const int rows = chunks * 16 - t.last;
-                    for (int c = 0; c < Sh::kStageBytes / kChunk; ++c)
-                        for (int x = lane; x < rows * 8; x += 32)
-                            *(uint4 *)(sa + c * kChunk + t.last * 128 + x * 16) = uint4{0, 0, 0, 0};
-                    fence_proxy_async_smem();
-                    __syncwarp();
+                    if constexpr (CG == 2) ok = wait_warp(&s.tail[st], odd >> st & 1, s, a);
+                    if (!ok) break;
+                    zero_rows(sa, Sh::kStageBytes, t.last);
+                    if constexpr (CG == 2) {
+                        ok = wait_warp(&s.peer[st], odd >> st & 1, s, a);
+                        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                    }
+                    if (!ok) break;
+                    odd ^= 1u << st;
                 }
-                if (lane == 0) {
-                    tc_fence_after();
+                tc_fence_after();
+                if (elect()) {
                     const uint64_t da = smem_desc(smem_u32(sa), a.a_kmajor);
                     const uint64_t db = smem_desc(smem_u32(sa + kP * 128), a.b_kmajor);
-                    for (int c = 0; c < chunks; ++c)
-                        mma_f16<CG>(tmem + as * BQ, da + (uint64_t)(c * a_adv), db + (uint64_t)(c * b_adv), idesc,
-                                    k > 0 || c > 0);
-                    commit<CG>(&s.empty[st]);
-                    if (k == t.steps - 1) commit<CG>(&s.acc_full[as]);
+#pragma unroll
+                    for (int c = 0; c < kR / 16; ++c)
+                        if (c < chunks)
+                            mma_f16<CG>(d, da + (uint64_t)(c * a_adv), db + (uint64_t)(c * b_adv), idesc,
+                                        k > 0 || c > 0);
+                    commit<CG>(&s.empty[st], both);
+                    if (k == t.steps - 1) commit<CG>(&s.acc_full[as], both);
                 }
                 issued = true;
                 __syncwarp();
+                if (++st == Sh::kStages) {
+                    st = 0;
+                    ph ^= 1;
+                }
             }
         }
-        if (!ok && issued && lane == 0) {   // MMAs in flight end before tensor memory is freed
-            commit_local<CG>(&s.drain);
+        if (!ok && issued) {   // MMAs in flight end before tensor memory is freed
+            if (elect()) commit_local<CG>(&s.drain);
+            __syncwarp();
             drain_bar(&s.drain, 0);
         }
         __syncwarp();
+    } else if (CG == 2 && warp == 1) {      // the pair's second CTA zeroes its rows of ragged last steps
+        uint32_t n = 0, odd = 0;
+        for (int64_t i = first_tile; p.red && p.offsets && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
+            if constexpr (SPLIT) cut(t, splits, part);
+            n += t.steps;
+            if (t.steps == 0 || t.last == 0) continue;
+            const uint32_t st = (n - 1) % Sh::kStages;
+            if (!wait_warp(&s.tail[st], odd >> st & 1, s, a)) break;
+            odd ^= 1u << st;
+            zero_rows(ring + st * Sh::kStageBytes, Sh::kStageBytes, t.last);
+            if (lane == 0) arrive_cluster(map_cta(smem_u32(&s.peer[st]), lead));
+        }
+        __syncwarp();
     } else if (warp >= 4) {
-        const int quad = warp & 3;
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        uint8_t *stage = stages + (warp - 4) * 2048;
         uint32_t acc = 0;
         for (int64_t i = first_tile; get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
+            mine = true;
+            const int64_t p0 = t.p0 + rank * kP + quad * 32;
+            if constexpr (SPLIT) cut(t, splits, part);
             const bool have = t.steps > 0;
-            uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
-            uint32_t as = 0;
+            const uint32_t as = acc & 1, at = lanes + as * BQ;
+            const float bias = SPLIT ? 0.f : load_bias<T>(p, t, p0 + lane);
             if (have) {
-                as = acc & 1;
                 const uint32_t ap = (acc >> 1) & 1;
                 ++acc;
-                at += as * BQ;
-                int ok = 1;
-                if (lane == 0) ok = wait_bar(&s.acc_full[as], ap, s, a);
-                if (!__shfl_sync(kFullMask, ok, 0)) break;
+                if (!wait_warp(&s.acc_full[as], ap, s, a)) break;
                 tc_fence_after();
             }
-            epilogue<T, O>(p, t, t.p0 + rank * kP + quad * 32 + lane, at, have);
+            float v[32];
+            for (int c0 = half * 32; c0 < t.nq; c0 += 64) {
+                read_columns(at + c0, have, v);
+                if constexpr (SPLIT) {       // the ring is free: partial sums, 32 columns a piece, a row per p
+                    float4 *o = (float4 *)((float *)ring + (c0 / 32) * kPiece + (quad * 32 + lane) * 36);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) o[j] = float4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
+                } else {
+                    finish_columns<T, O>(a, t, stage, p0, bias, v, c0, t.nq);
+                }
+            }
             if (have) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if constexpr (CG == 2) arrive_cluster(map_cta(smem_u32(&s.acc_empty[as]), 0));
+                    if constexpr (CG == 2) arrive_cluster(map_cta(smem_u32(&s.acc_empty[as]), lead));
                     else mbar_arrive(&s.acc_empty[as]);
                 }
+            }
+            if constexpr (SPLIT) break;
+        }
+    }
+    __syncwarp();
+    if constexpr (SPLIT) {
+        cluster_sync();
+        if (warp >= 4 && mine) {
+            // This CTA's slice of the columns, a multiple of 4, dealt to the two epilogue halves in runs of up to 32
+            // that stay within a piece.
+            const int quad = warp & 3, half = (warp - 4) >> 2;
+            const int64_t p0 = t.p0 + rank * kP + quad * 32;
+            uint8_t *stage = stages + (warp - 4) * 2048;
+            const float bias = load_bias<T>(p, t, p0 + lane);
+            const int per = ((t.nq + splits - 1) / splits + 3) & ~3, lo = part * per;
+            const int hi = lo + per < t.nq ? lo + per : t.nq;
+            int turn = 0;
+            for (int c0 = lo; c0 < hi; ++turn) {
+                int n = 32 - (c0 & 31);
+                if (n > hi - c0) n = hi - c0;
+                if (per <= 32 && n > (per / 2 + 3 & ~3)) n = per / 2 + 3 & ~3;
+                if ((turn & 1) == half) {
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                    const uint32_t own = smem_u32((float *)ring + (c0 / 32) * kPiece + (quad * 32 + lane) * 36 + (c0 & 31));
+                    for (int x = 0; x < splits; x += 2) {      // in order; two parts' loads in flight
+                        float4 f[2][8];
+                        if (n > 4) {
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const uint32_t src = map_cta(own, (x + u) * CG + rank);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)      // past n: other columns or padding, not stored
+                                    f[u][j] = ld_cluster(src + (4 * j < n ? j * 16 : 0));
+                            }
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                f[u][0] = ld_cluster(map_cta(own, (x + u) * CG + rank));
+#pragma unroll
+                                for (int j = 1; j < 8; ++j) f[u][j] = float4{0.f, 0.f, 0.f, 0.f};
+                            }
+                        }
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                v[4 * j] += f[u][j].x;
+                                v[4 * j + 1] += f[u][j].y;
+                                v[4 * j + 2] += f[u][j].z;
+                                v[4 * j + 3] += f[u][j].w;
+                            }
+                    }
+                    finish_columns<T, O>(a, t, stage, p0, bias, v, c0, c0 + n);
+                }
+                c0 += n;
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2) cluster_sync();
+    if constexpr (CG == 2 || SPLIT) cluster_sync();
     tc_fence_after();
     if (warp == 2) free_tmem<CG>(tmem, Sh::kTmem);
 }
@@ -569,8 +856,52 @@ int encode(CUtensorMap *m, const void *ptr, bool bf16, int64_t inner, int64_t ou
     return r == CUDA_SUCCESS ? SPMM_OK : SPMM_EALIGN;
 }
 
-template <int CG, int BQ, typename T, typename O>
-int launch(const Product &p, bool clear, bool probe, cudaStream_t s) {
+// Tile shape and splits by an estimate of the time: rounds of tiles over the
+// SMs, each its steps at the shape's measured cycles plus what a tile costs once.
+struct Choice {
+    int cg, bq, splits;
+};
+
+Choice choose(const Product &p, int sms) {
+    struct Cost {
+        int cg, bq;
+        double step, tile;
+    };
+    static const Cost costs[] = {{2, 256, 540, 6000}, {1, 128, 600, 3500}, {1, 64, 420, 2500}};
+    const double groups = (double)p.groups;
+    const double steps = (double)ceil_div(p.red && p.offsets ? ceil_div(p.R, p.groups) : p.R, kR);
+    Choice best{2, 256, 1};
+    double least = 1e300;
+    for (const Cost &c : costs) {
+        const double np = (double)ceil_div(p.P, kP * c.cg);
+        double nq;
+        if (p.red) nq = groups * (double)ceil_div(p.Q, c.bq);
+        else if (!p.offsets) nq = (double)ceil_div(p.Q, c.bq);
+        else {
+            const double per = (double)p.Q / groups;
+            nq = per < 1 ? (double)p.Q : groups * std::ceil(per / c.bq);
+            if (per > c.bq / 2) nq += groups * 0.5;
+        }
+        for (int s = 1; s <= 4 / c.cg; s *= 2) {        // clusters of 4 at most: larger ones leave SMs without any
+            if (s > 1 && (steps < 4 * s || np * nq * s * c.cg > sms * 7 / 8)) break;
+            const double rounds = std::ceil(np * nq * s * c.cg / sms);
+            const double t = rounds * (std::ceil(steps / s) * c.step + c.tile) + (s > 1 ? 5000 + c.bq * 30 : 0);
+            if (t < least) {
+                least = t;
+                best = Choice{c.cg, c.bq, s};
+            }
+        }
+    }
+    return best;
+}
+
+struct How {
+    bool clear, probe;
+    int splits, dev;
+};
+
+template <int CG, int BQ, bool SPLIT, typename T, typename O>
+int launch(const Product &p, const How &how, int sms, cudaStream_t s) {
     using Sh = Shape<CG, BQ>;
     Maps maps{};
     TcArgs a{};
@@ -578,8 +909,13 @@ int launch(const Product &p, bool clear, bool probe, cudaStream_t s) {
     a.a_kmajor = p.a_r == 1;
     a.b_kmajor = p.b_r == 1;
     a.bf16 = !p.f16;
-    a.clear_status = clear;
-    a.expire_probe = probe;
+    a.clear_status = how.clear;
+    a.expire_probe = how.probe;
+    a.splits = how.splits;
+    const int64_t per16 = 16 / sizeof(O);
+    a.vec_out = (uintptr_t)p.C % 16 == 0 && p.c_q % per16 == 0 && p.c_g % per16 == 0;
+    a.vec_slope = (uintptr_t)p.slope % 16 == 0 && p.P % 8 == 0;
+    a.vec_residual = (uintptr_t)p.residual % 16 == 0 && p.residual_ld % 8 == 0;
     if (p.R > 0) {
         const bool grouped = !p.red && p.groups > 1 && p.a_g != 0;
         a.a_grouped = grouped;
@@ -592,23 +928,25 @@ int launch(const Product &p, bool clear, bool probe, cudaStream_t s) {
     }
     const int64_t np = ceil_div(p.P, kP * CG);
     int64_t tiles = np * (p.red ? p.groups * ceil_div(p.Q, BQ) : ceil_div(p.Q, BQ) + (p.offsets ? p.groups : 0));
-    int dev = 0, sms = 0;
-    SPMM_CUDA_TRY(cudaGetDevice(&dev));
-    SPMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    if (tiles > sms / CG) tiles = sms / CG;
-    auto kernel = tc_kernel<CG, BQ, T, O>;
-    SPMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+    if (!SPLIT && tiles > sms / CG) tiles = sms / CG;
+    auto kernel = tc_kernel<CG, BQ, SPLIT, T, O>;
+    static std::atomic<uint64_t> ready{0};        // devices (below 64) on which the kernel may use its shared memory
+    const uint64_t bit = how.dev < 64 ? 1ull << how.dev : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * CG));
+    cfg.gridDim = dim3((unsigned)(tiles * CG * how.splits));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.x = CG * how.splits;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
+    cfg.numAttrs = CG * how.splits > 1 ? 1 : 0;
     if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
         (void)cudaGetLastError();
         return SPMM_ECUDA;
@@ -617,22 +955,34 @@ int launch(const Product &p, bool clear, bool probe, cudaStream_t s) {
     return SPMM_OK;
 }
 
+template <int CG, int BQ, typename T, typename O>
+int launch_split(const Product &p, const How &how, int sms, cudaStream_t s) {
+    return how.splits > 1 ? launch<CG, BQ, true, T, O>(p, how, sms, s) : launch<CG, BQ, false, T, O>(p, how, sms, s);
+}
+
 template <typename T, typename O>
-int by_shape(const Product &p, bool clear, bool probe, cudaStream_t s) {
-    const int64_t per = p.red ? p.Q : ceil_div(p.Q, p.groups);
-    if (per <= 64) return launch<1, 64, T, O>(p, clear, probe, s);
-    if (p.red) return launch<1, 256, T, O>(p, clear, probe, s);
-    return launch<2, 256, T, O>(p, clear, probe, s);
+int by_shape(const Product &p, How how, cudaStream_t s) {
+    int dev = 0, sms = 0;
+    SPMM_CUDA_TRY(cudaGetDevice(&dev));
+    SPMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const Choice c = choose(p, sms);
+    how.splits = c.splits;
+    how.dev = dev;
+    if (c.cg == 2) return launch_split<2, 256, T, O>(p, how, sms, s);
+    if (c.bq == 128) return launch_split<1, 128, T, O>(p, how, sms, s);
+    return launch_split<1, 64, T, O>(p, how, sms, s);
 }
 
 }  // namespace
 
 int launch_product(const Product &p, bool clear, bool probe, cudaStream_t s) {
     if (p.P == 0 || p.Q == 0 || (p.red && p.groups == 0)) return SPMM_OK;
-    if (p.f16) return p.out_f32 ? by_shape<__half, float>(p, clear, probe, s)
-                                : by_shape<__half, __half>(p, clear, probe, s);
-    return p.out_f32 ? by_shape<__nv_bfloat16, float>(p, clear, probe, s)
-                     : by_shape<__nv_bfloat16, __nv_bfloat16>(p, clear, probe, s);
+    if (!probe && skinny_fits(p)) return launch_skinny(p, clear, s);
+    const How how{clear, probe, 1, 0};
+    if (p.f16) return p.out_f32 ? by_shape<__half, float>(p, how, s)
+                                : by_shape<__half, __half>(p, how, s);
+    return p.out_f32 ? by_shape<__nv_bfloat16, float>(p, how, s)
+                     : by_shape<__nv_bfloat16, __nv_bfloat16>(p, how, s);
 }
 
 }  // namespace spmm

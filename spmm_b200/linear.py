@@ -14,33 +14,43 @@ of its bounded device waits (``product_status(y)``, ``check_product(y)``).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._device import on_device, ptr, stream_handle
+from ._device import on_device, stream_handle
 from .route import Routing, check_routing, need_cuda
 
 __all__ = ['dense_matmul', 'dense_matmul_backward', 'grouped_matmul', 'grouped_matmul_backward', 'ACTIVATIONS']
 
 ACTIVATIONS = ('none', 'relu', 'gelu', 'gelu_tanh', 'silu')
+_ACT = {name: i for i, name in enumerate(ACTIVATIONS)}
 _TYPES = {torch.bfloat16: _lib.DENSE_BF16, torch.float16: _lib.DENSE_F16}
+
+
+# spmm_linear (include/spmm_b200.h) packed in one go: filling a ctypes structure field by field cost as much
+# host time as launching the product
+_PACK = struct.Struct('@6i5q3Pq10P13qPQP').pack
+assert struct.calcsize('@6i5q3Pq10P13qPQP') == C.sizeof(_lib.Linear)
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _w_strides(w: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
-    """(w [G,K,N] with unit stride along k or n, the two strides)."""
-    k, n = w.shape[1], w.shape[2]
-    if w.stride(2) == 1 or n <= 1:
-        return w, w.stride(1) if k > 1 else max(n, 1), 1
-    if w.stride(1) == 1 or k <= 1:
-        return w, 1, w.stride(2) if n > 1 else max(k, 1)
-    w = w.contiguous()
-    return w, w.stride(1), 1
+def _w_strides(w: torch.Tensor):
+    """(w [..., K, N] with unit stride along k or n, the strides along k, n and the groups)."""
+    k, n = w.shape[-2], w.shape[-1]
+    st = w.stride()
+    if st[-1] != 1 and n > 1 and st[-2] != 1 and k > 1:
+        w = w.contiguous()
+        st = w.stride()
+    sg = st[0] if len(st) == 3 else 0
+    if st[-1] == 1 or n <= 1:
+        return w, (st[-2] if k > 1 else max(n, 1), 1, sg)
+    return w, (1, st[-1] if n > 1 else max(k, 1), sg)
 
 
 class _Groups:
@@ -51,81 +61,83 @@ class _Groups:
     def __init__(self, offsets, gather, slots, rows, count):
         self.offsets, self.gather, self.slots, self.rows, self.count = offsets, gather, slots, rows, count
 
-
-def _struct(x, w, g):
-    """spmm_linear with everything both directions share (x [R,K] and w [G,K,N] prepared)."""
-    w, sk, sn = _w_strides(w)
-    a = _lib.Linear()
-    a.version, a.dtype = 1, _TYPES[x.dtype]
-    a.rows, a.k, a.n, a.groups, a.x_rows = g.rows, w.shape[1], w.shape[2], g.count, x.shape[0]
-    a.offsets, a.gather = ptr(g.offsets), ptr(g.gather)
-    if g.slots is not None:
-        a.slots, a.top = ptr(g.slots), g.slots.shape[1]
-    a.x, a.x_ld = ptr(x), x.stride(0)
-    a.w, a.w_k, a.w_n, a.w_g = ptr(w), sk, sn, w.stride(0)
-    return a, w
+    def pointers(self):
+        """offsets, gather, slots, top."""
+        if self.offsets is None:
+            return 0, 0, 0, 0
+        if self.gather is None:
+            return self.offsets.data_ptr(), 0, 0, 0
+        return self.offsets.data_ptr(), self.gather.data_ptr(), self.slots.data_ptr(), self.slots.shape[1]
 
 
-def _scratch(a, size, device):
-    n = (size + 255) // 256 * 256
-    buf = torch.empty(n + 256, dtype=torch.uint8, device=device)
-    p = buf.data_ptr()
-    a.workspace, a.workspace_bytes, a.status = p if size else None, size, p + n
-    return buf, buf[n:n + 4].view(torch.int32)
+def _call(name, fixed, x, where):
+    """Runs a C entry on x's device and stream; returns the call's status word.  A call that needs scratch says
+    so before it does anything and is repeated with it."""
+    L = _lib.lib()
+    run = getattr(L, name)
+    stream = stream_handle(x.device)
+    word = x.new_empty(2)                       # 4 bytes
+    rc = run(_PACK(*fixed, 0, 0, word.data_ptr()), stream)
+    if rc == _lib.SPMM_EWORKSPACE:
+        n = getattr(L, name + '_workspace_size')(_PACK(*fixed, 0, 0, 0))
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        rc = run(_PACK(*fixed, ws.data_ptr(), n, word.data_ptr()), stream)
+    if rc:
+        _lib.check(rc, where)
+    return word
 
 
 def _forward(x, w, g, bias, residual, activation, want_slope):
-    device = x.device
+    """x [rows, K], w [K,N] or [G,K,N], bias [N] or [G,N], residual [rows, N]."""
     x = _unit_rows(x)
-    a, w = _struct(x, w, g)
-    a.activation = ACTIVATIONS.index(activation)
-    L = _lib.lib()
-    with on_device(device):
-        y = torch.empty((g.rows, w.shape[2]), dtype=x.dtype, device=device)
-        a.y, a.y_ld = ptr(y), y.stride(0)
-        if bias is not None:
-            bias = _unit_rows(bias)
-            a.bias, a.bias_g = ptr(bias), bias.stride(0)
-        if residual is not None:
-            residual = _unit_rows(residual)
-            a.residual, a.residual_ld = ptr(residual), residual.stride(0)
+    w, (sk, sn, sg) = _w_strides(w)
+    k, n = w.shape[-2:]
+    rows = g.rows
+    with on_device(x.device):
+        y = x.new_empty((rows, n))
         slope = None
         if want_slope and activation != 'none':
-            slope = torch.empty(y.shape, dtype=torch.int16, device=device)
-            a.slope = ptr(slope)
-        keep, status = _scratch(a, L.spmm_linear_forward_workspace_size(C.byref(a)), device)
-        _lib.check(L.spmm_linear_forward(C.byref(a), stream_handle(device)), 'matmul')
-        del keep
+            slope = torch.empty((rows, n), dtype=torch.int16, device=x.device)
+        bias_g = res_ld = 0
+        if bias is not None:
+            bias = _unit_rows(bias)
+            bias_g = bias.stride(0) if bias.dim() == 2 else 0
+        if residual is not None:
+            residual = _unit_rows(residual)
+            res_ld = residual.stride(0)
+        status = _call('spmm_linear_forward', (
+            1, _TYPES[x.dtype], _ACT[activation], 0, 0, 0, rows, k, n, g.count, x.shape[0], *g.pointers(),
+            x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            0 if residual is None else residual.data_ptr(), y.data_ptr(), 0 if slope is None else slope.data_ptr(),
+            0, 0, 0, 0, x.stride(0), sk, sn, sg, bias_g, res_ld, n, 0, 0, 0, 0, 0, 0), x, 'matmul')
     return y, slope, status
 
 
 def _backward(dy, x, w, g, slope, need_dx, need_dw, need_dbias):
-    device = x.device
     x, dy = _unit_rows(x), _unit_rows(dy)
-    a, w = _struct(x, w, g)
-    L = _lib.lib()
-    with on_device(device):
-        a.dy, a.dy_ld = ptr(dy), dy.stride(0)
-        a.slope = ptr(slope)
+    w, (sk, sn, sg) = _w_strides(w)
+    k, n = w.shape[-2:]
+    with on_device(x.device):
         dx = dw = dbias = None
+        dw_k = dw_n = 0
         if need_dx:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-            a.dx, a.dx_ld = ptr(dx), dx.stride(0)
+            dx = x.new_empty(x.shape)
         if need_dw:
-            count, k, n = w.shape
-            if a.w_n == 1:
-                dw = torch.empty((count, k, n), dtype=x.dtype, device=device)
-                a.dw_k, a.dw_n = max(n, 1), 1
+            lead = w.shape[:-2]
+            if sn == 1:
+                dw = x.new_empty(lead + (k, n))
+                dw_k, dw_n = max(n, 1), 1
             else:
-                dw = torch.empty((count, n, k), dtype=x.dtype, device=device).transpose(1, 2)
-                a.dw_k, a.dw_n = 1, max(k, 1)
-            a.dw, a.dw_g = ptr(dw), k * n
+                dw = x.new_empty(lead + (n, k)).transpose(-2, -1)
+                dw_k, dw_n = 1, max(k, 1)
         if need_dbias:
-            dbias = torch.empty((g.count, w.shape[2]), dtype=x.dtype, device=device)
-            a.dbias, a.dbias_g = ptr(dbias), dbias.stride(0)
-        keep, status = _scratch(a, L.spmm_linear_backward_workspace_size(C.byref(a)), device)
-        _lib.check(L.spmm_linear_backward(C.byref(a), stream_handle(device)), 'matmul_backward')
-        del keep
+            dbias = x.new_empty(w.shape[:-2] + (n,))
+        status = _call('spmm_linear_backward', (
+            1, _TYPES[x.dtype], 0, 0, 0, 0, g.rows, k, n, g.count, x.shape[0], *g.pointers(),
+            x.data_ptr(), w.data_ptr(), 0, 0, 0, 0 if slope is None else slope.data_ptr(), dy.data_ptr(),
+            0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+            0 if dbias is None else dbias.data_ptr(), x.stride(0), sk, sn, sg, 0, 0, 0, dy.stride(0), k, dw_k, dw_n,
+            k * n, n), x, 'matmul_backward')
     for t in (dx, dw, dbias):
         if t is not None:
             t._spmm_status = status
@@ -217,12 +229,11 @@ def dense_matmul(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] 
     if residual is not None:
         _check_like('residual', residual, x, shape)
     need_cuda(x, 'x')
-    x2 = x.reshape(_rows(x), x.shape[-1])
-    res = None if residual is None else residual.reshape(x2.shape[0], w.shape[1])
-    g = _Groups(None, None, None, x2.shape[0], 1)
-    out = _run(x2, w.unsqueeze(0), g, None if bias is None else bias.unsqueeze(0), res, activation, return_slope)
     if x.dim() == 2:
-        return out
+        return _run(x, w, _Groups(None, None, None, x.shape[0], 1), bias, residual, activation, return_slope)
+    rows = _rows(x)
+    out = _run(x.reshape(rows, x.shape[-1]), w, _Groups(None, None, None, rows, 1), bias,
+               None if residual is None else residual.reshape(rows, w.shape[1]), activation, return_slope)
     y = out[0] if return_slope else out
     status = y._spmm_status
     y = y.reshape(shape)
@@ -251,12 +262,13 @@ def dense_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sl
     _check_slope(slope, (rows, w.shape[1]), x)
     need_cuda(x, 'x')
     g = _Groups(None, None, None, rows, 1)
-    x2 = x.reshape(rows, x.shape[-1])
-    dx, dw, db = _backward(dy.reshape(rows, w.shape[1]), x2, w.unsqueeze(0), g, slope, True, True, bias)
+    if x.dim() == 2:
+        return _backward(dy, x, w, g, slope, True, True, bias)
+    dx, dw, db = _backward(dy.reshape(rows, w.shape[1]), x.reshape(rows, x.shape[-1]), w, g, slope, True, True, bias)
     status = dx._spmm_status
-    dx, dw = dx.reshape(x.shape), dw.squeeze(0)
-    dx._spmm_status = dw._spmm_status = status
-    return dx, dw, None if db is None else db.squeeze(0)
+    dx = dx.reshape(x.shape)
+    dx._spmm_status = status
+    return dx, dw, db
 
 
 def _groups(x, w, groups, gather):
