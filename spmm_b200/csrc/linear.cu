@@ -6,6 +6,8 @@
 //
 // All three products are one form, D[p][q] = sum_r A[p][r] B[q][r] (linear.cuh),
 // with groups that are ragged in q (forward, dx) or in r (dw).
+#include <type_traits>
+
 #include "linear.cuh"
 
 namespace spmm {
@@ -13,26 +15,33 @@ namespace {
 
 // ---- operand copies -----------------------------------------------------------
 
-// dst[i][c] = src[map ? map[i] : i][c], rows of `cols` 16-bit values, destination rows `dst_ld` apart; a map
-// value outside [0, src_rows) gives zeros.  Blocks of src_gs / dst_gs (groups) in blockIdx.z.
-__global__ void copy_rows_kernel(const uint16_t *src, int64_t src_ld, int64_t src_gs, int64_t src_rows,
-                                 const int32_t *map, uint16_t *dst, int64_t dst_ld, int64_t dst_gs, int64_t rows,
-                                 int64_t cols, int vec) {
-    src += blockIdx.z * src_gs;
-    dst += blockIdx.z * dst_gs;
-    const int64_t per = vec ? cols / 8 : cols;
-    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-        const int64_t from = map ? __ldg(map + i) : i;
+// dst[i][c] = src[map ? map[i] : i][c], rows of `cols` 16-bit values in pieces of
+// 8 (16 bytes, aligned in dst, whose rows are padded), read W values at a time;
+// a map value outside [0, src_rows) gives zeros.  A block of rows per group
+// (blockIdx.y), src_gs / dst_gs apart.
+template <int W>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t *src, int64_t src_ld, int64_t src_gs,
+                                                        int64_t src_rows, const int32_t *map, uint16_t *dst,
+                                                        int64_t dst_ld, int64_t dst_gs, int64_t rows, int64_t cols) {
+    using V = typename std::conditional<W == 8, uint4, typename std::conditional<W == 4, uint2,
+              typename std::conditional<W == 2, uint32_t, uint16_t>::type>::type>::type;
+    src += blockIdx.y * src_gs;
+    dst += blockIdx.y * dst_gs;
+    const int64_t per = dst_ld / 8, items = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per, c = (i - r * per) * 8;
+        const int64_t from = map ? __ldg(map + r) : r;
+        uint16_t v[8];
         const bool in = from >= 0 && from < src_rows;
-        for (int64_t c = threadIdx.x; c < per; c += blockDim.x) {
-            if (vec) {
-                uint4 v{0, 0, 0, 0};
-                if (in) v = __ldg(reinterpret_cast<const uint4 *>(src + from * src_ld) + c);
-                reinterpret_cast<uint4 *>(dst + i * dst_ld)[c] = v;
-            } else {
-                dst[i * dst_ld + c] = in ? __ldg(src + from * src_ld + c) : (uint16_t)0;
-            }
+#pragma unroll
+        for (int u = 0; u < 8 / W; ++u) {
+            V x{};
+            if (in && c + u * W < cols) x = __ldg(reinterpret_cast<const V *>(src + from * src_ld + c + u * W));
+            memcpy(v + u * W, &x, sizeof(V));
         }
+        uint4 o;
+        memcpy(&o, v, 16);
+        *reinterpret_cast<uint4 *>(dst + r * dst_ld + c) = o;
     }
 }
 
@@ -215,12 +224,17 @@ int carve(const Operand src, int64_t src_rows, const int32_t *map, int64_t group
     if (sizing) return SPMM_OK;
     if (!buf) return SPMM_EWORKSPACE;
     out.ptr = buf;
-    const int vec = cols % 8 == 0 && in_place(src.ptr, src.ld, src.gs, cols);
-    const int64_t per = vec ? cols / 8 : cols;
-    const int threads = per >= 256 ? 256 : (int)ceil_div(per, 32) * 32;
-    const dim3 grid((unsigned)(rows < 65536 ? rows : 65536), 1, (unsigned)copies);
-    copy_rows_kernel<<<grid, threads, 0, s>>>((const uint16_t *)src.ptr, src.ld, src.gs, src_rows, map, buf, ld,
-                                              out.gs, rows, cols, vec);
+    const int64_t blocks = ceil_div(rows * (ld / 8), 256);
+    const dim3 grid((unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), (unsigned)copies);
+    const int64_t all = (int64_t)((uintptr_t)src.ptr / 2) | src.ld | (copies > 1 ? src.gs : 0) | cols;
+#define SPMM_COPY(W)                                                                                             \
+    copy_rows_kernel<W><<<grid, 256, 0, s>>>((const uint16_t *)src.ptr, src.ld, src.gs, src_rows, map, buf, ld, \
+                                             out.gs, rows, cols)
+    if (all % 8 == 0) SPMM_COPY(8);
+    else if (all % 4 == 0) SPMM_COPY(4);
+    else if (all % 2 == 0) SPMM_COPY(2);
+    else SPMM_COPY(1);
+#undef SPMM_COPY
     SPMM_PRODUCT_LAUNCHED();
     return SPMM_OK;
 }
@@ -261,7 +275,6 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     Weight w;
     SPMM_TRY(carve_x(p, a, sizing, x, s));
     SPMM_TRY(carve_w(p, a, sizing, w, s));
-    if (sizing) return SPMM_OK;
     Product g = base(p);
     g.P = p->n;
     g.Q = p->rows;
@@ -281,7 +294,7 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     g.residual = p->residual;
     g.residual_ld = p->residual_ld;
     g.slope = p->slope;
-    return launch_product(g, true, p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT, s);
+    return launch_product(g, a, sizing, true, p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT, s);
 }
 
 template <typename T>
@@ -304,10 +317,9 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     }
     if (p->dbias && any) part = a.take<float>(tiles * p->n);
     if (p->dx && p->gather) dxs = a.take<float>(p->rows * p->k);
-    if (sizing) return SPMM_OK;
-    if ((p->slope && any && (p->dx || p->dw) && !dzp) || (p->dbias && any && !part) || (p->dx && p->gather && !dxs))
+    if (!sizing && ((p->slope && any && (p->dx || p->dw) && !dzp) || (p->dbias && any && !part) || (p->dx && p->gather && !dxs)))
         return SPMM_EWORKSPACE;
-    if (dzp || part) {
+    if (!sizing && (dzp || part)) {
         const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
         const dim3 grid((unsigned)ceil_div(p->n, kDzCols), (unsigned)tiles);
         if (vec)
@@ -318,7 +330,7 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
                                                      p->offsets, p->groups, p->rows, p->n);
         SPMM_PRODUCT_LAUNCHED();
     }
-    if (p->dbias && p->n) {
+    if (!sizing && p->dbias && p->n) {
         dbias_kernel<T><<<dim3((unsigned)ceil_div(p->n, 128), (unsigned)p->groups), 128, 0, s>>>(
             part, p->offsets, any ? p->rows : 0, p->n, (T *)p->dbias, p->dbias_g);
         SPMM_PRODUCT_LAUNCHED();
@@ -335,11 +347,11 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
         g.B = dz.ptr;
         g.b_q = dz.ld;
         g.b_r = 1;
-        g.C = dxs ? (void *)dxs : p->dx;
-        g.c_q = dxs ? p->k : p->dx_ld;
-        g.out_f32 = dxs != nullptr;
-        SPMM_TRY(launch_product(g, true, probe, s));
-        if (dxs)
+        g.C = p->gather ? (void *)dxs : p->dx;
+        g.c_q = p->gather ? p->k : p->dx_ld;
+        g.out_f32 = p->gather != nullptr;
+        SPMM_TRY(launch_product(g, a, sizing, true, probe, s));
+        if (p->gather && !sizing)
             SPMM_TRY(launch_gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, p->dx, p->dx_ld, g.f16, s));
     }
     if (p->dw) {
@@ -358,7 +370,7 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
         g.C = p->dw;
         g.c_q = n_unit ? p->dw_k : p->dw_n;
         g.c_g = p->dw_g;
-        SPMM_TRY(launch_product(g, !p->dx, probe, s));
+        SPMM_TRY(launch_product(g, a, sizing, !p->dx, probe, s));
     }
     return SPMM_OK;
 }

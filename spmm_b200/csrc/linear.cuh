@@ -174,7 +174,8 @@ struct Product {
 };
 
 // `clear`: the kernel sets *status to 0 first (the first product of a call); `probe`: SPMM_CFG_EXPIRE_FIRST_WAIT.
-int launch_product(const Product &p, bool clear, bool probe, cudaStream_t s);
+// Scratch comes from `arena`; `sizing` only counts it.
+int launch_product(const Product &p, Arena &arena, bool sizing, bool clear, bool probe, cudaStream_t s);
 
 // The same for at most four rows per group on average (operands aligned, see skinny_fits).
 bool skinny_fits(const Product &p);

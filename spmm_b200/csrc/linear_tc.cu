@@ -41,7 +41,6 @@ constexpr int kP = 128;             // p per CTA
 constexpr int kChunk = kR * 128;    // bytes of 64 rows of 128 bytes
 constexpr int kThreads = 384;     // 4 warps of roles, 8 of the epilogue
 constexpr int kEpiWarps = 8;
-constexpr int kPiece = kP * 36;     // floats of 32 columns of partial sums: 36 a row keeps 16-byte accesses apart
 constexpr int kBand = 8;            // q tiles that one sweep over p covers
 
 struct Maps {
@@ -53,6 +52,7 @@ struct TcArgs {
     int32_t a_kmajor, b_kmajor, a_grouped;   // a_grouped: the group is A's third coordinate
     int32_t bf16, clear_status, expire_probe, splits;
     int32_t vec_out, vec_slope, vec_residual;   // 16-byte aligned rows
+    int64_t part_stride;                        // between the partial results of one group's split sum
 };
 
 template <int CG, int BQ>
@@ -67,13 +67,13 @@ struct Shape {
     static constexpr int kRing = kStages * kStageBytes, kOut = kEpiWarps * 2048;
     static constexpr int kSmem = 1024 + kRing + kOut + kTable + 512;
     static_assert(BQ % 64 == 0 && kTmem >= 32 && kTmem <= 512, "accumulators");
-    static_assert(BQ / 32 * kPiece * 4 <= kRing, "partial sums fit the ring");
     static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 };
 
 struct Tile {
     int64_t group, p0, q0, r0;
     int nq, steps;       // columns; steps of kR
+    int part;            // of the sum over r (TcArgs::splits)
     int last;            // rows of r in the last step when it is ragged, else 0
     bool zero;           // rows behind the last group: written as zeros
 };
@@ -112,13 +112,6 @@ __device__ __forceinline__ void cluster_sync() {
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
-    float4 f;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
-                 : "r"(addr));
-    return f;
 }
 template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
@@ -289,26 +282,26 @@ __device__ __forceinline__ void raster(int64_t i, int64_t np, int64_t nq, int64_
 
 // Tile number i; false behind the last one.
 template <int CG, int BQ>
-__device__ __forceinline__ bool get_tile(const Product &p, Table t, int64_t i, Tile &o) {
+__device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, int64_t i, Tile &o) {
+    const Product &p = a.p;
     const int64_t np = (p.P + kP * CG - 1) / (kP * CG);
     int64_t pt, qt;
     o.zero = false;
     o.r0 = 0;
     o.last = 0;
     int64_t len = p.R;
-    if (p.red) {
+    o.part = 0;
+    if (p.red && p.offsets) {
         const int64_t nq = (p.Q + BQ - 1) / BQ, per = np * nq;
         o.group = i / per;
         if (o.group >= p.groups) return false;
         raster(i - o.group * per, np, nq, pt, qt);
         o.q0 = qt * BQ;
         o.nq = (int)(p.Q - o.q0 < BQ ? p.Q - o.q0 : BQ);
-        if (p.offsets) {
-            o.r0 = t.first[o.group];
-            len = t.first[o.group + 1] - o.r0;
-            if (len < 0) len = 0;
-            o.last = (int)(len & (kR - 1));
-        }
+        o.r0 = t.first[o.group];
+        len = t.first[o.group + 1] - o.r0;
+        if (len < 0) len = 0;
+        o.last = (int)(len & (kR - 1));
     } else if (p.offsets) {
         const int G = (int)p.groups;
         const int64_t nq = t.qtiles[G + 1];
@@ -328,24 +321,22 @@ __device__ __forceinline__ bool get_tile(const Product &p, Table t, int64_t i, T
             len = 0;
         }
     } else {
-        const int64_t nq = (p.Q + BQ - 1) / BQ;
-        if (i >= np * nq) return false;
-        raster(i, np, nq, pt, qt);
+        const int64_t nq = (p.Q + BQ - 1) / BQ, all = np * nq;
+        if (i >= all * a.splits) return false;
+        o.part = (int)(i / all);
+        raster(i - o.part * all, np, nq, pt, qt);
         o.group = 0;
         o.q0 = qt * BQ;
         o.nq = (int)(p.Q - o.q0 < BQ ? p.Q - o.q0 : BQ);
     }
     o.p0 = pt * kP * CG;
     o.steps = (int)((len + kR - 1) / kR);
+    if (a.splits > 1) {
+        const int lo = (int)((int64_t)o.steps * o.part / a.splits);
+        o.steps = (int)((int64_t)o.steps * (o.part + 1) / a.splits) - lo;
+        o.r0 = (int64_t)lo * kR;
+    }
     return true;
-}
-
-// Part `part` of `splits` of a tile's steps.
-__device__ __forceinline__ void cut(Tile &t, int splits, int part) {
-    const int a = t.steps * part / splits, b = t.steps * (part + 1) / splits;
-    if (b < t.steps) t.last = 0;
-    t.r0 += (int64_t)a * kR;
-    t.steps = b - a;
 }
 
 // MMA columns of a tile: a multiple of 16 (of 32 for a pair, half from each CTA).
@@ -425,7 +416,7 @@ __device__ __forceinline__ void store_columns(const TcArgs &a, const Tile &t, ui
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] += r[j];
     }
-    store_piece<O>(stage, (O *)p.C + (p.red ? t.group * p.c_g : 0) + q * p.c_q + p0, p.c_q, a.vec_out, cols, n,
+    store_piece<O>(stage, (O *)p.C + (p.red ? t.group * p.c_g : 0) + t.part * a.part_stride + q * p.c_q + p0, p.c_q, a.vec_out, cols, n,
                    [&](int j) { return from_f32<O>(y[j]); });
     if constexpr (SLOPE)
         store_piece<uint16_t>(stage, (uint16_t *)p.slope + q * p.P + p0, p.P, a.vec_slope, cols, n,
@@ -558,10 +549,7 @@ struct Loader {
     }
 };
 
-// SPLIT: a cluster of `splits` CTAs (pairs) shares one tile, each sums a part of
-// r, and the parts meet in shared memory: every CTA finishes a slice of the
-// columns, adding the parts in order.  One tile per cluster.
-template <int CG, int BQ, bool SPLIT, typename T, typename O>
+template <int CG, int BQ, typename T, typename O>
 __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ Maps maps,
                                                          const __grid_constant__ TcArgs a) {
     using Sh = Shape<CG, BQ>;
@@ -574,11 +562,9 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     Bars &s = *(Bars *)((uint8_t *)table.first + Sh::kTable);
     const Product &p = a.p;
     const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const uint32_t crank = CG == 2 || SPLIT ? cluster_rank() : 0;
+    const uint32_t crank = CG == 2 ? cluster_rank() : 0;
     const uint32_t rank = crank % CG, lead = crank - rank;     // within the pair; the pair's first CTA
-    const int splits = SPLIT ? a.splits : 1, part = SPLIT ? (int)(crank / CG) : 0;
-    const int64_t first_tile = blockIdx.x / (CG * splits);
-    const int64_t tile_step = SPLIT ? INT64_MAX / 2 : gridDim.x / CG;
+    const int64_t first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
         if (p.R > 0) {
@@ -606,24 +592,21 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     Tile t;
     if (CG == 1 && warp == 0 && !p.offsets && !a.expire_probe) {   // fill the ring before anything else is ready
         __syncwarp();
-        if (get_tile<CG, BQ>(p, table, first_tile, t)) {
-            if constexpr (SPLIT) cut(t, splits, part);
+        if (get_tile<CG, BQ>(a, table, first_tile, t)) {
             for (int k = 0; k < t.steps && k < Sh::kStages; ++k) load.step(t, k);
         }
     }
     fill_table<BQ>(p, table);
     tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2 || SPLIT) cluster_sync();
+    if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
-    bool mine = false;       // SPLIT: this cluster has a tile
 
     if (warp == 0) {
         bool ok = true;
         if (a.expire_probe) ok = wait_warp(&s.never, 0u, s, a);
-        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
-            if constexpr (SPLIT) cut(t, splits, part);
+        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             for (int k = i == first_tile ? (int)load.n : 0; k < t.steps; ++k) {
                 if (!wait_warp(&s.empty[load.st], load.ph ^ 1, s, a)) {
                     ok = false;
@@ -654,8 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                                 ((a.a_kmajor ? 0u : 1u) << 15) | ((a.b_kmajor ? 0u : 1u) << 16) |
                                 ((uint32_t)(kP * CG >> 4) << 24);
         const uint32_t a_adv = (a.a_kmajor ? 32 : 2048) >> 4, b_adv = (a.b_kmajor ? 32 : 2048) >> 4;
-        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
-            if constexpr (SPLIT) cut(t, splits, part);
+        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             if (t.steps == 0) continue;
             const uint32_t as = acc & 1, ap = (acc >> 1) & 1;
             ++acc;
@@ -708,8 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         __syncwarp();
     } else if (CG == 2 && warp == 1) {      // the pair's second CTA zeroes its rows of ragged last steps
         uint32_t n = 0, odd = 0;
-        for (int64_t i = first_tile; p.red && p.offsets && get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
-            if constexpr (SPLIT) cut(t, splits, part);
+        for (int64_t i = first_tile; p.red && p.offsets && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             n += t.steps;
             if (t.steps == 0 || t.last == 0) continue;
             const uint32_t st = (n - 1) % Sh::kStages;
@@ -724,13 +705,11 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         uint8_t *stage = stages + (warp - 4) * 2048;
         uint32_t acc = 0;
-        for (int64_t i = first_tile; get_tile<CG, BQ>(p, table, i, t); i += tile_step) {
-            mine = true;
+        for (int64_t i = first_tile; get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             const int64_t p0 = t.p0 + rank * kP + quad * 32;
-            if constexpr (SPLIT) cut(t, splits, part);
             const bool have = t.steps > 0;
             const uint32_t as = acc & 1, at = lanes + as * BQ;
-            const float bias = SPLIT ? 0.f : load_bias<T>(p, t, p0 + lane);
+            const float bias = load_bias<T>(p, t, p0 + lane);
             if (have) {
                 const uint32_t ap = (acc >> 1) & 1;
                 ++acc;
@@ -740,13 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             float v[32];
             for (int c0 = half * 32; c0 < t.nq; c0 += 64) {
                 read_columns(at + c0, have, v);
-                if constexpr (SPLIT) {       // the ring is free: partial sums, 32 columns a piece, a row per p
-                    float4 *o = (float4 *)((float *)ring + (c0 / 32) * kPiece + (quad * 32 + lane) * 36);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = float4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
-                } else {
-                    finish_columns<T, O>(a, t, stage, p0, bias, v, c0, t.nq);
-                }
+                finish_columns<T, O>(a, t, stage, p0, bias, v, c0, t.nq);
             }
             if (have) {
                 tc_fence_before();
@@ -756,68 +729,12 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     else mbar_arrive(&s.acc_empty[as]);
                 }
             }
-            if constexpr (SPLIT) break;
         }
     }
     __syncwarp();
-    if constexpr (SPLIT) {
-        cluster_sync();
-        if (warp >= 4 && mine) {
-            // This CTA's slice of the columns, a multiple of 4, dealt to the two epilogue halves in runs of up to 32
-            // that stay within a piece.
-            const int quad = warp & 3, half = (warp - 4) >> 2;
-            const int64_t p0 = t.p0 + rank * kP + quad * 32;
-            uint8_t *stage = stages + (warp - 4) * 2048;
-            const float bias = load_bias<T>(p, t, p0 + lane);
-            const int per = ((t.nq + splits - 1) / splits + 3) & ~3, lo = part * per;
-            const int hi = lo + per < t.nq ? lo + per : t.nq;
-            int turn = 0;
-            for (int c0 = lo; c0 < hi; ++turn) {
-                int n = 32 - (c0 & 31);
-                if (n > hi - c0) n = hi - c0;
-                if (per <= 32 && n > (per / 2 + 3 & ~3)) n = per / 2 + 3 & ~3;
-                if ((turn & 1) == half) {
-                    float v[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
-                    const uint32_t own = smem_u32((float *)ring + (c0 / 32) * kPiece + (quad * 32 + lane) * 36 + (c0 & 31));
-                    for (int x = 0; x < splits; x += 2) {      // in order; two parts' loads in flight
-                        float4 f[2][8];
-                        if (n > 4) {
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const uint32_t src = map_cta(own, (x + u) * CG + rank);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)      // past n: other columns or padding, not stored
-                                    f[u][j] = ld_cluster(src + (4 * j < n ? j * 16 : 0));
-                            }
-                        } else {
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                f[u][0] = ld_cluster(map_cta(own, (x + u) * CG + rank));
-#pragma unroll
-                                for (int j = 1; j < 8; ++j) f[u][j] = float4{0.f, 0.f, 0.f, 0.f};
-                            }
-                        }
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                v[4 * j] += f[u][j].x;
-                                v[4 * j + 1] += f[u][j].y;
-                                v[4 * j + 2] += f[u][j].z;
-                                v[4 * j + 3] += f[u][j].w;
-                            }
-                    }
-                    finish_columns<T, O>(a, t, stage, p0, bias, v, c0, c0 + n);
-                }
-                c0 += n;
-            }
-        }
-    }
     tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2 || SPLIT) cluster_sync();
+    if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
     if (warp == 2) free_tmem<CG>(tmem, Sh::kTmem);
 }
@@ -856,8 +773,9 @@ int encode(CUtensorMap *m, const void *ptr, bool bf16, int64_t inner, int64_t ou
     return r == CUDA_SUCCESS ? SPMM_OK : SPMM_EALIGN;
 }
 
-// Tile shape and splits by an estimate of the time: rounds of tiles over the
-// SMs, each its steps at the shape's measured cycles plus what a tile costs once.
+// Tile shape and splits by an estimate of the time in cycles: rounds of tiles
+// over the SMs, each its steps at the shape's measured rate plus what a tile
+// costs once; a split adds a second kernel that reads every part.
 struct Choice {
     int cg, bq, splits;
 };
@@ -882,10 +800,11 @@ Choice choose(const Product &p, int sms) {
             nq = per < 1 ? (double)p.Q : groups * std::ceil(per / c.bq);
             if (per > c.bq / 2) nq += groups * 0.5;
         }
-        for (int s = 1; s <= 4 / c.cg; s *= 2) {        // clusters of 4 at most: larger ones leave SMs without any
-            if (s > 1 && (steps < 4 * s || np * nq * s * c.cg > sms * 7 / 8)) break;
+        for (int s = 1; s <= 16; ++s) {
+            if (s > 1 && (p.offsets || p.out_f32 || steps < 4 * s || np * nq * s * c.cg > sms)) break;
             const double rounds = std::ceil(np * nq * s * c.cg / sms);
-            const double t = rounds * (std::ceil(steps / s) * c.step + c.tile) + (s > 1 ? 5000 + c.bq * 30 : 0);
+            double t = rounds * (std::ceil(steps / s) * c.step + c.tile);
+            if (s > 1) t += 4000 + (double)p.P * (double)p.Q * s * 4 / 4000;
             if (t < least) {
                 least = t;
                 best = Choice{c.cg, c.bq, s};
@@ -895,13 +814,76 @@ Choice choose(const Product &p, int sms) {
     return best;
 }
 
+// Partial results of a split sum: C = finish(sum over parts, in order).  Eight p a thread.
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Product p, const float *parts, int splits) {
+    constexpr int V = VEC ? 8 : 1;
+    const int64_t per = p.P / V, items = p.Q * per;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= items) return;
+    const int64_t q = i / per, pp = (i - q * per) * V;
+    float z[V] = {}, d[V];
+    const float *src = parts + q * p.P + pp;
+#pragma unroll 4
+    for (int x = 0; x < splits; ++x, src += p.P * p.Q) {
+        if constexpr (VEC) {
+            const float4 a = __ldcg((const float4 *)src), b = __ldcg((const float4 *)src + 1);
+            z[0] += a.x, z[1] += a.y, z[2] += a.z, z[3] += a.w, z[4] += b.x, z[5] += b.y, z[6] += b.z, z[7] += b.w;
+        } else {
+            z[0] += __ldcg(src);
+        }
+    }
+    if (p.bias) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] += to_f32(((const T *)p.bias)[pp + e]);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) z[e] = activate<ACT, true>(z[e], d[e]);
+    if (p.residual) {
+        const T *r = (const T *)p.residual + q * p.residual_ld + pp;
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[e] += to_f32(r[e]);
+    }
+    T *out = (T *)p.C + q * p.c_q + pp;
+    if constexpr (VEC) *(uint4 *)out = pack8<T>(z);
+    else out[0] = from_f32<T>(z[0]);
+    if (p.slope) {
+        uint16_t c[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) c[e] = slope_code(d[e]);
+        if constexpr (VEC) memcpy(__builtin_assume_aligned(p.slope + q * p.P + pp, 16), c, 16);
+        else p.slope[q * p.P + pp] = (int16_t)c[0];
+    }
+}
+
+template <typename T>
+int join(const Product &p, const float *parts, int splits, cudaStream_t s) {
+    const bool vec = p.P % 8 == 0 && (uintptr_t)p.C % 16 == 0 && p.c_q % 8 == 0 && (uintptr_t)p.slope % 16 == 0;
+    const unsigned grid = (unsigned)ceil_div(p.Q * (vec ? p.P / 8 : p.P), 256);
+#define SPMM_JOIN(ACT)                                                                       \
+    do {                                                                                     \
+        if (vec) join_kernel<T, ACT, true><<<grid, 256, 0, s>>>(p, parts, splits);           \
+        else join_kernel<T, ACT, false><<<grid, 256, 0, s>>>(p, parts, splits);              \
+    } while (0)
+    switch (p.act) {
+        case SPMM_ACT_NONE: SPMM_JOIN(SPMM_ACT_NONE); break;
+        case SPMM_ACT_RELU: SPMM_JOIN(SPMM_ACT_RELU); break;
+        case SPMM_ACT_GELU: SPMM_JOIN(SPMM_ACT_GELU); break;
+        case SPMM_ACT_GELU_TANH: SPMM_JOIN(SPMM_ACT_GELU_TANH); break;
+        default: SPMM_JOIN(SPMM_ACT_SILU); break;
+    }
+#undef SPMM_JOIN
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
+}
+
 struct How {
     bool clear, probe;
-    int splits, dev;
+    int splits, dev, sms;
 };
 
-template <int CG, int BQ, bool SPLIT, typename T, typename O>
-int launch(const Product &p, const How &how, int sms, cudaStream_t s) {
+template <int CG, int BQ, typename T, typename O>
+int launch(const Product &p, const How &how, cudaStream_t s) {
     using Sh = Shape<CG, BQ>;
     Maps maps{};
     TcArgs a{};
@@ -912,8 +894,10 @@ int launch(const Product &p, const How &how, int sms, cudaStream_t s) {
     a.clear_status = how.clear;
     a.expire_probe = how.probe;
     a.splits = how.splits;
+    a.part_stride = p.P * p.Q;
     const int64_t per16 = 16 / sizeof(O);
-    a.vec_out = (uintptr_t)p.C % 16 == 0 && p.c_q % per16 == 0 && p.c_g % per16 == 0;
+    a.vec_out = (uintptr_t)p.C % 16 == 0 && p.c_q % per16 == 0 && p.c_g % per16 == 0 &&
+                (how.splits == 1 || a.part_stride % per16 == 0);
     a.vec_slope = (uintptr_t)p.slope % 16 == 0 && p.P % 8 == 0;
     a.vec_residual = (uintptr_t)p.residual % 16 == 0 && p.residual_ld % 8 == 0;
     if (p.R > 0) {
@@ -928,8 +912,9 @@ int launch(const Product &p, const How &how, int sms, cudaStream_t s) {
     }
     const int64_t np = ceil_div(p.P, kP * CG);
     int64_t tiles = np * (p.red ? p.groups * ceil_div(p.Q, BQ) : ceil_div(p.Q, BQ) + (p.offsets ? p.groups : 0));
-    if (!SPLIT && tiles > sms / CG) tiles = sms / CG;
-    auto kernel = tc_kernel<CG, BQ, SPLIT, T, O>;
+    tiles *= how.splits;
+    if (tiles > how.sms / CG) tiles = how.sms / CG;
+    auto kernel = tc_kernel<CG, BQ, T, O>;
     static std::atomic<uint64_t> ready{0};        // devices (below 64) on which the kernel may use its shared memory
     const uint64_t bit = how.dev < 64 ? 1ull << how.dev : 0;
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
@@ -937,16 +922,16 @@ int launch(const Product &p, const How &how, int sms, cudaStream_t s) {
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * CG * how.splits));
+    cfg.gridDim = dim3((unsigned)(tiles * CG));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG * how.splits;
+    at[0].val.clusterDim.x = CG;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = CG * how.splits > 1 ? 1 : 0;
+    cfg.numAttrs = CG > 1 ? 1 : 0;
     if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
         (void)cudaGetLastError();
         return SPMM_ECUDA;
@@ -955,34 +940,45 @@ int launch(const Product &p, const How &how, int sms, cudaStream_t s) {
     return SPMM_OK;
 }
 
-template <int CG, int BQ, typename T, typename O>
-int launch_split(const Product &p, const How &how, int sms, cudaStream_t s) {
-    return how.splits > 1 ? launch<CG, BQ, true, T, O>(p, how, sms, s) : launch<CG, BQ, false, T, O>(p, how, sms, s);
+template <typename T, typename O>
+int by_shape(const Product &p, const Choice &c, const How &how, cudaStream_t s) {
+    if (c.cg == 2) return launch<2, 256, T, O>(p, how, s);
+    if (c.bq == 128) return launch<1, 128, T, O>(p, how, s);
+    return launch<1, 64, T, O>(p, how, s);
 }
 
-template <typename T, typename O>
-int by_shape(const Product &p, How how, cudaStream_t s) {
-    int dev = 0, sms = 0;
-    SPMM_CUDA_TRY(cudaGetDevice(&dev));
-    SPMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    const Choice c = choose(p, sms);
+template <typename T>
+int run(const Product &p, Arena &arena, bool sizing, How how, cudaStream_t s) {
+    const Choice c = choose(p, how.sms);
     how.splits = c.splits;
-    how.dev = dev;
-    if (c.cg == 2) return launch_split<2, 256, T, O>(p, how, sms, s);
-    if (c.bq == 128) return launch_split<1, 128, T, O>(p, how, sms, s);
-    return launch_split<1, 64, T, O>(p, how, sms, s);
+    if (c.splits == 1) {
+        if (sizing) return SPMM_OK;
+        return p.out_f32 ? by_shape<T, float>(p, c, how, s) : by_shape<T, T>(p, c, how, s);
+    }
+    float *parts = arena.take<float>(p.P * p.Q * c.splits);
+    if (sizing) return SPMM_OK;
+    if (!parts) return SPMM_EWORKSPACE;
+    Product raw = p;          // plain float32 sums of each part
+    raw.C = parts;
+    raw.c_q = p.P;
+    raw.c_g = 0;
+    raw.out_f32 = 1;
+    raw.act = SPMM_ACT_NONE;
+    raw.bias = raw.residual = nullptr;
+    raw.slope = nullptr;
+    SPMM_TRY((by_shape<T, float>(raw, c, how, s)));
+    return join<T>(p, parts, c.splits, s);
 }
 
 }  // namespace
 
-int launch_product(const Product &p, bool clear, bool probe, cudaStream_t s) {
+int launch_product(const Product &p, Arena &arena, bool sizing, bool clear, bool probe, cudaStream_t s) {
     if (p.P == 0 || p.Q == 0 || (p.red && p.groups == 0)) return SPMM_OK;
-    if (!probe && skinny_fits(p)) return launch_skinny(p, clear, s);
-    const How how{clear, probe, 1, 0};
-    if (p.f16) return p.out_f32 ? by_shape<__half, float>(p, how, s)
-                                : by_shape<__half, __half>(p, how, s);
-    return p.out_f32 ? by_shape<__nv_bfloat16, float>(p, how, s)
-                     : by_shape<__nv_bfloat16, __nv_bfloat16>(p, how, s);
+    if (!probe && skinny_fits(p)) return sizing ? SPMM_OK : launch_skinny(p, clear, s);
+    How how{clear, probe, 1, 0, 148};
+    SPMM_CUDA_TRY(cudaGetDevice(&how.dev));
+    SPMM_CUDA_TRY(cudaDeviceGetAttribute(&how.sms, cudaDevAttrMultiProcessorCount, how.dev));
+    return p.f16 ? run<__half>(p, arena, sizing, how, s) : run<__nv_bfloat16>(p, arena, sizing, how, s);
 }
 
 }  // namespace spmm

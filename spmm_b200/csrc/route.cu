@@ -12,6 +12,8 @@
 // first positions, and a CTA per chunk places its choices in order (ranks
 // within a warp by match, warps by a prefix over their counts).  Integer sums
 // only: the result does not depend on the order of the atomics.
+#include <type_traits>
+
 #include "linear.cuh"
 
 namespace spmm {
@@ -26,6 +28,20 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     if (v != v) return kNone;
     const uint32_t u = __float_as_uint(v + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// The same in 16 bits for a 16-bit value, and the key of its -inf.
+template <typename T>
+__device__ __forceinline__ uint32_t half_key(float v) {
+    if (v != v) v = -INFINITY;
+    const T h = from_f32<T>(v + 0.f);
+    uint16_t u;
+    memcpy(&u, &h, 2);
+    return u & 0x8000u ? (uint16_t)~u : u | 0x8000u;
+}
+template <typename T>
+__host__ __device__ constexpr uint32_t half_floor() {
+    return sizeof(T) == 2 ? (std::is_same<T, __half>::value ? 0x03FFu : 0x007Fu) : 0u;
 }
 
 // A logit as the weights use it: +inf as the largest float, NaN as -inf.
@@ -66,7 +82,12 @@ __device__ __forceinline__ void load_row(const T *row, int experts, int lane, fl
 __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
 
 // One token: lane j < top ends with choice j in (expert, weight).
-template <typename T, int V>
+//
+// PACKED (16-bit logits without bias): a 16-bit key with the expert below it
+// makes one 32-bit word, so that a round is a maximum tree, one reduction and
+// V selects; otherwise the key needs all 32 bits and the expert a second
+// reduction.
+template <typename T, int V, bool PACKED>
 __device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int lane, int &expert, float &weight) {
     const int experts = (int)p.experts, top = (int)p.top;
     float l[V];
@@ -75,41 +96,52 @@ __device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int 
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int e = v * 32 + lane;
-        key[v] = e >= experts ? 0u : order_key(p.bias ? l[v] + __ldg(p.bias + e) : l[v]);
+        if constexpr (PACKED) {
+            key[v] = e >= experts ? 0u : half_key<T>(l[v]) << 16 | (0xFFFFu - e);
+        } else {
+            key[v] = e >= experts ? 0u : order_key(p.bias ? l[v] + __ldg(p.bias + e) : l[v]);
+        }
         l[v] = clean_logit(l[v]);
     }
     expert = -1;
     float mine = -INFINITY;   // the logit of this lane's choice
     for (int j = 0; j < top; ++j) {
-        uint32_t best = 0u;
-        int at = 0;
+        int e;
+        if constexpr (PACKED) {
+            uint32_t best = key[0];
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (key[v] > best) {
-                best = key[v];
-                at = v;
-            }
-        const uint32_t m = __reduce_max_sync(kFullMask, best);
-        if (m <= kNone) break;
-        const int e = (int)__reduce_min_sync(kFullMask, best == m ? (unsigned)(at * 32 + lane) : ~0u);
-        float val = 0.f;
+            for (int v = 1; v < V; ++v) best = best > key[v] ? best : key[v];
+            const uint32_t m = __reduce_max_sync(kFullMask, best);
+            if (m >> 16 <= half_floor<T>()) break;
+            e = (int)(0xFFFFu - (m & 0xFFFFu));
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (v * 32 + lane == e) {
-                key[v] = 0u;
-                val = l[v];
-            }
-        val = __shfl_sync(kFullMask, val, e & 31);
-        if (lane == j) {
-            expert = e;
-            mine = val;
+            for (int v = 0; v < V; ++v) key[v] = key[v] == m ? 0u : key[v];
+        } else {
+            uint32_t best = 0u;
+            int at = 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (key[v] > best) {
+                    best = key[v];
+                    at = v;
+                }
+            const uint32_t m = __reduce_max_sync(kFullMask, best);
+            if (m <= kNone) break;
+            e = (int)__reduce_min_sync(kFullMask, best == m ? (unsigned)(at * 32 + lane) : ~0u);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v * 32 + lane == e) key[v] = 0u;
         }
+        if (lane == j) expert = e;
     }
+    // each choice's logit, from the row just read
+    if (expert >= 0) mine = clean_logit(to_f32(((const T *)p.logits)[t * p.logits_ld + expert]));
+    __syncwarp();
     // weights
     if (p.scoring == SPMM_SCORE_SOFTMAX) {
         Row r;
         if (p.renormalize) {   // relative to the chosen ones alone
-            float c[1] = {expert >= 0 ? mine : -INFINITY};
+            float c[1] = {mine};
             r = softmax_row<1>(c);
         } else {
             r = softmax_row<V>(l);
@@ -128,13 +160,13 @@ __device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int 
 }
 
 // Choices of the tokens [t0, t1) of this CTA, and their counts per expert in `count`.
-template <typename T, int V>
+template <typename T, int V, bool PACKED>
 __device__ __forceinline__ void choose_chunk(const spmm_route_args &p, int64_t t0, int64_t t1, int *count) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     for (int64_t t = t0 + warp; t < t1; t += warps) {
         int e;
         float w;
-        choose<T, V>(p, t, lane, e, w);
+        choose<T, V, PACKED>(p, t, lane, e, w);
         if (lane < p.top) {
             p.weights[t * p.top + lane] = w;
             p.experts_out[t * p.top + lane] = e;
@@ -220,7 +252,7 @@ __device__ __forceinline__ void place(const spmm_route_args &p, int64_t i0, int6
 }
 
 // Everything in one CTA: for few tokens, where launches are what it costs.
-template <typename T, int V>
+template <typename T, int V, bool PACKED>
 __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_route_args p) {
     extern __shared__ int sm[];
     __shared__ int tmp[33];
@@ -228,7 +260,7 @@ __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_r
     int *count = sm, *wcount = sm + experts;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) count[e] = 0;
     __syncthreads();
-    choose_chunk<T, V>(p, 0, p.tokens, count);
+    choose_chunk<T, V, PACKED>(p, 0, p.tokens, count);
     __syncthreads();
     const int total = cta_exclusive(count, experts, tmp);
     for (int e = threadIdx.x; e < experts; e += blockDim.x) p.offsets[e] = count[e];
@@ -238,14 +270,14 @@ __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_r
     place(p, 0, all, count, wcount);
 }
 
-template <typename T, int V>
+template <typename T, int V, bool PACKED>
 __global__ void __launch_bounds__(kWarps * 32) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
     extern __shared__ int sm[];
     const int experts = (int)p.experts;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) sm[e] = 0;
     __syncthreads();
     const int64_t t0 = blockIdx.x * chunk, t1 = t0 + chunk < p.tokens ? t0 + chunk : p.tokens;
-    choose_chunk<T, V>(p, t0, t1, sm);
+    choose_chunk<T, V, PACKED>(p, t0, t1, sm);
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[(int64_t)blockIdx.x * experts + e] = sm[e];
 }
@@ -401,32 +433,45 @@ __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC]) {
     }
 }
 
+// A warp per (token, 32 VEC columns): lane j holds choice j's slot and weight, so
+// the chosen rows' loads are issued together, eight at a time, after one load
+// latency.  Bound by reading each chosen row once.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_kernel(spmm_combine_args p, int64_t per) {
-    const int64_t items = p.tokens * per, step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += step) {
-        const int64_t t = i / per, c = (i - t * per) * VEC;
+__global__ void __launch_bounds__(256) combine_kernel(spmm_combine_args p, int chunks) {
+    const int lane = threadIdx.x & 31, top = (int)p.top;
+    const int64_t step = (int64_t)gridDim.x * 8;
+    int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    for (; i < p.tokens * chunks; i += step) {
+        const int64_t t = i / chunks, c = ((i - t * chunks) * 32 + lane) * VEC;
+        const bool in = c < p.n;
         float acc[VEC] = {};
-        for (int64_t j0 = 0; j0 < p.top; j0 += 4) {
-            float f[4][VEC], w[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                w[u] = 0.f;
-#pragma unroll
-                for (int x = 0; x < VEC; ++x) f[u][x] = 0.f;
-                if (j0 + u < p.top) {
-                    const int64_t s = __ldg(p.slots + t * p.top + j0 + u);
-                    if (s >= 0 && s < p.rows) {
-                        w[u] = __ldg(p.weights + t * p.top + j0 + u);
-                        load_vec<T, VEC>((const T *)p.y + s * p.y_ld + c, f[u]);
-                    }
-                }
+        for (int j0 = 0; j0 < top; j0 += 32) {
+            int slot = -1;
+            float weight = 0.f;
+            if (j0 + lane < top) {
+                slot = __ldg(p.slots + t * top + j0 + lane);
+                weight = __ldg(p.weights + t * top + j0 + lane);
+                if (slot >= p.rows) slot = -1;
             }
+            const int n = top - j0 < 32 ? top - j0 : 32;
+            for (int j1 = 0; j1 < n; j1 += 8) {
+                float f[8][VEC], w[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < 8; ++u) {
+                    const int s = __shfl_sync(kFullMask, slot, j1 + u);      // lanes past top hold -1
+                    w[u] = __shfl_sync(kFullMask, weight, j1 + u);
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) acc[x] = fmaf(w[u], f[u][x], acc[x]);
+                    for (int x = 0; x < VEC; ++x) f[u][x] = 0.f;
+                    if (s >= 0 && in) load_vec<T, VEC>((const T *)p.y + s * p.y_ld + c, f[u]);
+                    else w[u] = 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int x = 0; x < VEC; ++x) acc[x] = fmaf(w[u], f[u][x], acc[x]);
+            }
         }
+        if (!in) continue;
         if (p.residual) {
             float f[VEC];
             load_vec<T, VEC>((const T *)p.residual + t * p.residual_ld + c, f);
@@ -437,39 +482,66 @@ __global__ void __launch_bounds__(256) combine_kernel(spmm_combine_args p, int64
     }
 }
 
-// A warp per token: dout's row against each chosen row of y.
+// A warp per token: dout's row, read once per eight choices, against their rows
+// of y, with eight sums in registers.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) combine_backward_kernel(spmm_combine_args p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t per = p.n / VEC, step = (int64_t)gridDim.x * 8;
+    const int lane = threadIdx.x & 31, top = (int)p.top;
+    const int64_t step = (int64_t)gridDim.x * 8;
     const int64_t w0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     for (int64_t t = w0; t < p.tokens; t += step) {
-        for (int64_t j = 0; j < p.top; ++j) {
-            const int64_t s = __ldg(p.slots + t * p.top + j);
-            const bool in = s >= 0 && s < p.rows;
-            float dot = 0.f;
-            if (in) {
-                const float w = p.dy ? __ldg(p.weights + t * p.top + j) : 0.f;
-                for (int64_t c = lane; c < per; c += 32) {
-                    float d[VEC];
-                    load_vec<T, VEC>((const T *)p.dout + t * p.dout_ld + c * VEC, d);
-                    if (p.dweights) {
-                        float y[VEC];
-                        load_vec<T, VEC>((const T *)p.y + s * p.y_ld + c * VEC, y);
+        for (int j0 = 0; j0 < top; j0 += 8) {
+            int slot = -1;
+            float weight = 0.f;
+            if (lane < 8 && j0 + lane < top) {
+                slot = __ldg(p.slots + t * top + j0 + lane);
+                weight = __ldg(p.weights + t * top + j0 + lane);
+                if (slot >= p.rows) slot = -1;
+            }
+            int s[8];
+            float w[8], dot[8] = {};
 #pragma unroll
-                        for (int x = 0; x < VEC; ++x) dot = fmaf(d[x], y[x], dot);
-                    }
-                    if (p.dy) {
+            for (int u = 0; u < 8; ++u) {
+                s[u] = __shfl_sync(kFullMask, slot, u);
+                w[u] = __shfl_sync(kFullMask, weight, u);
+            }
+            for (int64_t c = lane * VEC; c < p.n; c += 32 * VEC) {
+                float d[VEC], y[8][VEC];
+                load_vec<T, VEC>((const T *)p.dout + t * p.dout_ld + c, d);
+                if (p.dweights) {
 #pragma unroll
-                        for (int x = 0; x < VEC; ++x) d[x] *= w;
-                        store_vec<T, VEC>((T *)p.dy + s * p.dy_ld + c * VEC, d);
+                    for (int u = 0; u < 8; ++u) {
+#pragma unroll
+                        for (int x = 0; x < VEC; ++x) y[u][x] = 0.f;
+                        if (s[u] >= 0) load_vec<T, VEC>((const T *)p.y + s[u] * p.y_ld + c, y[u]);
                     }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (s[u] >= 0)
+#pragma unroll
+                            for (int x = 0; x < VEC; ++x) dot[u] = fmaf(d[x], y[u][x], dot[u]);
+                }
+                if (p.dy) {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (s[u] >= 0) {
+                            float o[VEC];
+#pragma unroll
+                            for (int x = 0; x < VEC; ++x) o[x] = w[u] * d[x];
+                            store_vec<T, VEC>((T *)p.dy + s[u] * p.dy_ld + c, o);
+                        }
                 }
             }
             if (p.dweights) {
+                float mine = 0.f;
 #pragma unroll
-                for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
-                if (lane == 0) p.dweights[t * p.top + j] = dot;
+                for (int u = 0; u < 8; ++u) {
+                    float v = dot[u];
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+                    if (lane == u) mine = v;
+                }
+                if (lane < 8 && j0 + lane < top) p.dweights[t * top + j0 + lane] = mine;
             }
         }
     }
@@ -501,20 +573,20 @@ int64_t chunk_tokens(const spmm_route_args *p) {
     return c < 32 ? 32 : c;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool PACKED>
 int run_route(const spmm_route_args &p, cudaStream_t s) {
     const int e4 = (int)p.experts * 4;
     if (small_route(&p)) {
         const int most = V <= 8 ? 32 : 16;   // registers: V logits and keys a thread
         int warps = (int)(p.tokens < 1 ? 1 : p.tokens < most ? p.tokens : most);
         while (warps > 1 && (warps + 1) * e4 > 40 * 1024) --warps;   // below 48 KB with the static part
-        route_small_kernel<T, V><<<1, warps * 32, (warps + 1) * e4, s>>>(p);
+        route_small_kernel<T, V, PACKED><<<1, warps * 32, (warps + 1) * e4, s>>>(p);
         SPMM_PRODUCT_LAUNCHED();
         return SPMM_OK;
     }
     const int64_t chunk = chunk_tokens(&p), chunks = ceil_div(p.tokens, chunk);
     int *counts = (int *)p.workspace, *totals = counts + chunks * p.experts;
-    route_choose_kernel<T, V><<<(unsigned)chunks, kWarps * 32, e4, s>>>(p, chunk, counts);
+    route_choose_kernel<T, V, PACKED><<<(unsigned)chunks, kWarps * 32, e4, s>>>(p, chunk, counts);
     SPMM_PRODUCT_LAUNCHED();
     route_scan_kernel<<<(unsigned)ceil_div(p.experts, 32), 1024, 0, s>>>(counts, (int)chunks, (int)p.experts, totals);
     SPMM_PRODUCT_LAUNCHED();
@@ -534,7 +606,13 @@ int run_route_backward(const spmm_route_args &p, cudaStream_t s) {
 
 template <typename T>
 int by_width(const spmm_route_args &p, bool backward, cudaStream_t s) {
-#define SPMM_ROUTE_V(V) return backward ? run_route_backward<T, V>(p, s) : run_route<T, V>(p, s)
+#define SPMM_ROUTE_V(V)                                         \
+    do {                                                        \
+        if (backward) return run_route_backward<T, V>(p, s);    \
+        if constexpr (sizeof(T) == 2)                           \
+            if (!p.bias) return run_route<T, V, true>(p, s);    \
+        return run_route<T, V, false>(p, s);                    \
+    } while (0)
     if (p.experts <= 32) SPMM_ROUTE_V(1);
     if (p.experts <= 64) SPMM_ROUTE_V(2);
     if (p.experts <= 128) SPMM_ROUTE_V(4);
@@ -555,6 +633,7 @@ int check_combine(const spmm_combine_args *p) {
     if (p->dtype != SPMM_DENSE_F32 && p->dtype != SPMM_DENSE_BF16 && p->dtype != SPMM_DENSE_F16)
         return SPMM_EUNSUPPORTED;
     if (p->tokens < 0 || p->top < 1 || p->rows < 0 || p->n < 0) return SPMM_EINVAL;
+    if (p->rows > INT32_MAX || p->top > INT32_MAX) return SPMM_EUNSUPPORTED;
     return SPMM_OK;
 }
 
@@ -574,11 +653,12 @@ int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
         if (vec) combine_backward_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p);
         else combine_backward_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
     } else {
-        const int64_t per = vec ? p.n / W : p.n;
-        int64_t grid = ceil_div(p.tokens * per, 256);
-        if (grid > 148 * 32) grid = 148 * 32;
-        if (vec) combine_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p, per);
-        else combine_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p, per);
+        const int64_t chunks = ceil_div(p.n, vec ? 32 * W : 32);
+        if (chunks > INT32_MAX) return SPMM_EUNSUPPORTED;
+        int64_t grid = ceil_div(p.tokens * chunks, 8);
+        if (grid > 148 * 64) grid = 148 * 64;
+        if (vec) combine_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p, (int)chunks);
+        else combine_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p, (int)chunks);
     }
     SPMM_PRODUCT_LAUNCHED();
     return SPMM_OK;

@@ -301,6 +301,8 @@ def test_expired_wait_is_reported(cuda):
     a.version, a.dtype, a.rows, a.x_rows, a.k, a.n, a.groups = 1, _lib.DENSE_BF16, 300, 300, 256, 512, 1
     a.x, a.x_ld, a.w, a.w_k, a.w_n, a.y, a.y_ld = x.data_ptr(), 256, w.data_ptr(), 512, 1, y.data_ptr(), 512
     a.status, a.wait_us, a.flags = status.data_ptr(), 2000, _lib.SPMM_CFG_EXPIRE_FIRST_WAIT
+    ws = torch.empty(_lib.lib().spmm_linear_forward_workspace_size(C.byref(a)) + 256, device='cuda', dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     stream = torch.cuda.current_stream().cuda_stream
     assert _lib.lib().spmm_linear_forward(C.byref(a), stream) == 0
     torch.cuda.synchronize()
