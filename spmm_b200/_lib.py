@@ -207,11 +207,10 @@ def lib() -> C.CDLL:
             getattr(L, n).restype = C.c_int
             getattr(L, n + '_workspace_size').argtypes = [C.c_void_p]
             getattr(L, n + '_workspace_size').restype = C.c_size_t
-        L.spmm_route_workspace_size.argtypes = [C.POINTER(RouteArgs)]
+        L.spmm_route_workspace_size.argtypes = [C.c_void_p]
         L.spmm_route_workspace_size.restype = C.c_size_t
-        for n, t in (('spmm_route', RouteArgs), ('spmm_route_backward', RouteArgs), ('spmm_combine', CombineArgs),
-                     ('spmm_combine_backward', CombineArgs)):
-            getattr(L, n).argtypes = [C.POINTER(t), C.c_void_p]
+        for n in ('spmm_route', 'spmm_route_backward', 'spmm_combine', 'spmm_combine_backward'):
+            getattr(L, n).argtypes = [C.c_void_p, C.c_void_p]       # a RouteArgs or CombineArgs, or its bytes
             getattr(L, n).restype = C.c_int
         for n in ('spmm_boo_build_analyze', 'spmm_boo_build_emit', 'spmm_pbr_build_analyze',
                   'spmm_pbr_build_emit', 'spmm_boo_matmul', 'spmm_pbr_matmul'):

@@ -273,7 +273,6 @@ Product base(const spmm_linear *p) {
 int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     Operand x;
     Weight w;
-    SPMM_TRY(carve_x(p, a, sizing, x, s));
     SPMM_TRY(carve_w(p, a, sizing, w, s));
     Product g = base(p);
     g.P = p->n;
@@ -284,9 +283,16 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     g.a_p = w.n;
     g.a_r = w.k;
     g.a_g = w.g;
+    g.b_r = 1;
+    if (p->gather && skinny_fits(g) && in_place(p->x, p->x_ld, 0, p->k)) {   // reads the gathered rows itself
+        g.gather = p->gather;
+        g.gather_rows = p->x_rows;
+        x = Operand{p->x, p->x_ld, 0};
+    } else {
+        SPMM_TRY(carve_x(p, a, sizing, x, s));
+    }
     g.B = x.ptr;
     g.b_q = x.ld;
-    g.b_r = 1;
     g.C = p->y;
     g.c_q = p->y_ld;
     g.bias = p->bias;

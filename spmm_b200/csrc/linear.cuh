@@ -169,6 +169,9 @@ struct Product {
     const void *residual;
     int64_t residual_ld;
     int16_t *slope;              // [Q][P]
+    // A handful of rows: row q of B is row gather[q] of the operand, zeros where that lies outside [0, gather_rows).
+    const int32_t *gather;
+    int64_t gather_rows;
     int32_t *status;
     int64_t wait_cycles;
 };

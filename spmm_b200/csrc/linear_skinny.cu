@@ -28,6 +28,16 @@ __device__ __forceinline__ Rows group_rows(const Product &p, int64_t g) {
     return {a, b, g == p.groups};
 }
 
+// Row q of B (null: zeros).
+template <typename T>
+__device__ __forceinline__ const T *row_of(const Product &p, int64_t q) {
+    if (p.gather) {
+        q = __ldg(p.gather + q);
+        if (q < 0 || q >= p.gather_rows) return nullptr;
+    }
+    return (const T *)p.B + q * p.b_q;
+}
+
 template <typename T, typename O, int ACT>
 __device__ __forceinline__ void put_act(const Product &p, int64_t q, int64_t pp, float z) {
     float d, y = activate<ACT, true>(z, d);
@@ -65,7 +75,9 @@ constexpr int kNP = 4;      // p of a CTA, r contiguous
 template <typename T, typename O, int R, int KS>
 __device__ __forceinline__ void rows_rmajor(const Product &p, int64_t g, int64_t q, int64_t p0, float *sm) {
     const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % KS;
-    const T *A = (const T *)p.A + g * p.a_g, *B = (const T *)p.B + q * p.b_q;
+    const T *A = (const T *)p.A + g * p.a_g, *b[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) b[j] = row_of<T>(p, q + j);
     const T *a[kNP];
 #pragma unroll
     for (int i = 0; i < kNP; ++i) a[i] = A + (p0 + i < p.P ? p0 + i : p.P - 1) * p.a_p;
@@ -76,7 +88,7 @@ __device__ __forceinline__ void rows_rmajor(const Product &p, int64_t g, int64_t
 #pragma unroll
         for (int i = 0; i < kNP; ++i) w[i] = __ldg((const uint4 *)(a[i] + r));
 #pragma unroll
-        for (int j = 0; j < R; ++j) x[j] = __ldg((const uint4 *)(B + j * p.b_q + r));
+        for (int j = 0; j < R; ++j) x[j] = b[j] ? __ldg((const uint4 *)(b[j] + r)) : uint4{0, 0, 0, 0};
         float xf[R][8];
 #pragma unroll
         for (int j = 0; j < R; ++j) unpack8<T>(x[j], xf[j]);
@@ -143,14 +155,16 @@ template <typename T, typename O, int R>
 __device__ __forceinline__ void rows_pmajor(const Product &p, int64_t g, int64_t q, int64_t p0, float *sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t pl = p0 + (lane & 3) * 8;
-    const T *A = (const T *)p.A + g * p.a_g + (pl + 8 <= p.P ? pl : 0), *B = (const T *)p.B + q * p.b_q;
+    const T *A = (const T *)p.A + g * p.a_g + (pl + 8 <= p.P ? pl : 0), *b[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) b[j] = row_of<T>(p, q + j);
     float acc[R][8] = {};
 #pragma unroll 4
     for (int64_t r = warp * 8 + (lane >> 2); r < p.R; r += kWarps * 8) {
         const uint4 w = __ldg((const uint4 *)(A + r * p.a_r));
         float x[R], wf[8];
 #pragma unroll
-        for (int j = 0; j < R; ++j) x[j] = to_f32(B[j * p.b_q + r]);
+        for (int j = 0; j < R; ++j) x[j] = b[j] ? to_f32(b[j][r]) : 0.f;
         unpack8<T>(w, wf);
 #pragma unroll
         for (int j = 0; j < R; ++j)

@@ -19,7 +19,8 @@
 namespace spmm {
 namespace {
 
-constexpr int kWarps = 8;                  // warps of a routing CTA
+constexpr int kWarps = 8;                  // warps of a CTA that places or differentiates
+constexpr int kChooseWarps = 16;           // of one that chooses: two tokens a warp at 32 tokens a chunk
 constexpr int kMaxExperts = SPMM_MAX_GROUPS;
 constexpr uint32_t kNone = 0x007FFFFFu;    // key of -inf: not selectable, like every smaller key
 
@@ -81,12 +82,30 @@ __device__ __forceinline__ void load_row(const T *row, int experts, int lane, fl
 
 __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
 
+// Descending, by Batcher's odd-even merge network.
+template <int V>
+__device__ __forceinline__ void sort_descending(uint32_t (&k)[V]) {
+#pragma unroll
+    for (int p = 1; p < V; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t a = k[i + j], b = k[i + j + q];
+                        k[i + j] = a > b ? a : b;
+                        k[i + j + q] = a > b ? b : a;
+                    }
+}
+
 // One token: lane j < top ends with choice j in (expert, weight).
 //
 // PACKED (16-bit logits without bias): a 16-bit key with the expert below it
-// makes one 32-bit word, so that a round is a maximum tree, one reduction and
-// V selects; otherwise the key needs all 32 bits and the expert a second
-// reduction.
+// makes one 32-bit word; each lane sorts its words once, and a round is one
+// reduction of the lanes' first ones and a shift in the lane that won.
+// Otherwise the key needs all 32 bits and the expert a second reduction.
 template <typename T, int V, bool PACKED>
 __device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int lane, int &expert, float &weight) {
     const int experts = (int)p.experts, top = (int)p.top;
@@ -103,19 +122,18 @@ __device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int 
         }
         l[v] = clean_logit(l[v]);
     }
+    if constexpr (PACKED) sort_descending(key);
     expert = -1;
     float mine = -INFINITY;   // the logit of this lane's choice
     for (int j = 0; j < top; ++j) {
         int e;
         if constexpr (PACKED) {
-            uint32_t best = key[0];
-#pragma unroll
-            for (int v = 1; v < V; ++v) best = best > key[v] ? best : key[v];
-            const uint32_t m = __reduce_max_sync(kFullMask, best);
+            const uint32_t m = __reduce_max_sync(kFullMask, key[0]);
             if (m >> 16 <= half_floor<T>()) break;
             e = (int)(0xFFFFu - (m & 0xFFFFu));
+            const bool won = key[0] == m;
 #pragma unroll
-            for (int v = 0; v < V; ++v) key[v] = key[v] == m ? 0u : key[v];
+            for (int v = 0; v < V; ++v) key[v] = won ? (v + 1 < V ? key[v + 1] : 0u) : key[v];
         } else {
             uint32_t best = 0u;
             int at = 0;
@@ -271,7 +289,7 @@ __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_r
 }
 
 template <typename T, int V, bool PACKED>
-__global__ void __launch_bounds__(kWarps * 32) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
+__global__ void __launch_bounds__(kChooseWarps * 32) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
     extern __shared__ int sm[];
     const int experts = (int)p.experts;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) sm[e] = 0;
@@ -405,20 +423,25 @@ __global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(spmm_route_
 
 // ---- combine --------------------------------------------------------------------
 
-template <typename T, int VEC> struct Pack { T v[VEC]; };
+// VEC values as they lie in memory: loads are issued together and converted
+// afterwards, or each would be waited for in turn.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T *p, float (&f)[VEC]) {
-    if constexpr (VEC * sizeof(T) == 16) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+struct Raw {
+    typename std::conditional<VEC * sizeof(T) == 16, uint4, T>::type v;
+    static_assert(VEC * sizeof(T) == 16 || VEC == 1, "one value or 16 bytes");
+
+    __device__ __forceinline__ void clear() { memset(&v, 0, sizeof(v)); }
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC * sizeof(T) == 16) v = __ldg(reinterpret_cast<const uint4 *>(p));
+        else v = p[0];
+    }
+    __device__ __forceinline__ void get(float (&f)[VEC]) const {
         T t[VEC];
-        memcpy(t, &u, 16);
+        memcpy(t, &v, sizeof(t));
 #pragma unroll
         for (int i = 0; i < VEC; ++i) f[i] = to_f32(t[i]);
-    } else {
-        static_assert(VEC == 1, "one value or 16 bytes");
-        f[0] = to_f32(p[0]);
     }
-}
+};
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC]) {
     T t[VEC];
@@ -433,59 +456,87 @@ __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC]) {
     }
 }
 
-// A warp per (token, 32 VEC columns): lane j holds choice j's slot and weight, so
-// the chosen rows' loads are issued together, eight at a time, after one load
-// latency.  Bound by reading each chosen row once.
+// A warp per token, or per part of its columns where tokens are few: lane j
+// holds choice j's slot and weight, and the chosen rows' loads are issued eight
+// at a time.  Bound by reading each chosen row once.  A warp per 32 VEC columns
+// whatever the tokens, each fetching the slots anew, took twice as long
+// (16384 tokens x 8 rows of 4 KB: 229 us).
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_kernel(spmm_combine_args p, int chunks) {
+__global__ void __launch_bounds__(256, 3) combine_kernel(const __grid_constant__ spmm_combine_args p, int parts,
+                                                         int part_cols) {
     const int lane = threadIdx.x & 31, top = (int)p.top;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    for (; i < p.tokens * chunks; i += step) {
-        const int64_t t = i / chunks, c = ((i - t * chunks) * 32 + lane) * VEC;
-        const bool in = c < p.n;
-        float acc[VEC] = {};
-        for (int j0 = 0; j0 < top; j0 += 32) {
-            int slot = -1;
-            float weight = 0.f;
-            if (j0 + lane < top) {
-                slot = __ldg(p.slots + t * top + j0 + lane);
-                weight = __ldg(p.weights + t * top + j0 + lane);
-                if (slot >= p.rows) slot = -1;
+    const int64_t items = p.tokens * parts, step = (int64_t)gridDim.x * 8;
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < items; i += step) {
+        const int64_t t = i / parts, c0 = (i - t * parts) * part_cols;
+        const int64_t end = c0 + part_cols < p.n ? c0 + part_cols : p.n;
+        int slot = -1;
+        float weight = 0.f;
+        if (lane < top) {
+            slot = __ldg(p.slots + t * top + lane);
+            weight = __ldg(p.weights + t * top + lane);
+            if (slot >= p.rows) slot = -1;
+        }
+        int s[8];
+        float w[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            s[u] = __shfl_sync(kFullMask, slot, u);
+            w[u] = __shfl_sync(kFullMask, weight, u);
+        }
+        for (int64_t cb = c0; cb < end; cb += 32 * VEC) {      // the whole warp
+            const int64_t c = cb + lane * VEC;
+            const bool in = c < end;
+            Raw<T, VEC> residual, y[8];
+            if (p.residual && in) residual.load((const T *)p.residual + t * p.residual_ld + c);
+            float acc[VEC] = {};
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                y[u].clear();
+                if (s[u] >= 0 && in) y[u].load((const T *)p.y + s[u] * p.y_ld + c);
             }
-            const int n = top - j0 < 32 ? top - j0 : 32;
-            for (int j1 = 0; j1 < n; j1 += 8) {
-                float f[8][VEC], w[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int s = __shfl_sync(kFullMask, slot, j1 + u);      // lanes past top hold -1
-                    w[u] = __shfl_sync(kFullMask, weight, j1 + u);
+            for (int u = 0; u < 8; ++u)
+                if (s[u] >= 0) {
+                    float f[VEC];
+                    y[u].get(f);
 #pragma unroll
-                    for (int x = 0; x < VEC; ++x) f[u][x] = 0.f;
-                    if (s >= 0 && in) load_vec<T, VEC>((const T *)p.y + s * p.y_ld + c, f[u]);
-                    else w[u] = 0.f;
+                    for (int x = 0; x < VEC; ++x) acc[x] = fmaf(w[u], f[x], acc[x]);
+                }
+            for (int j = 8; j < top; j += 4) {                 // more than eight choices
+                Raw<T, VEC> z[4];
+                int sj[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    sj[u] = j + u < top ? __ldg(p.slots + t * top + j + u) : -1;
+                    z[u].clear();
+                    if (sj[u] >= 0 && sj[u] < p.rows && in) z[u].load((const T *)p.y + sj[u] * p.y_ld + c);
                 }
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int u = 0; u < 4; ++u)
+                    if (sj[u] >= 0 && sj[u] < p.rows) {
+                        const float wj = __ldg(p.weights + t * top + j + u);
+                        float f[VEC];
+                        z[u].get(f);
 #pragma unroll
-                    for (int x = 0; x < VEC; ++x) acc[x] = fmaf(w[u], f[u][x], acc[x]);
+                        for (int x = 0; x < VEC; ++x) acc[x] = fmaf(wj, f[x], acc[x]);
+                    }
             }
-        }
-        if (!in) continue;
-        if (p.residual) {
-            float f[VEC];
-            load_vec<T, VEC>((const T *)p.residual + t * p.residual_ld + c, f);
+            if (!in) continue;
+            if (p.residual) {
+                float f[VEC];
+                residual.get(f);
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) acc[x] += f[x];
+                for (int x = 0; x < VEC; ++x) acc[x] += f[x];
+            }
+            store_vec<T, VEC>((T *)p.out + t * p.out_ld + c, acc);
         }
-        store_vec<T, VEC>((T *)p.out + t * p.out_ld + c, acc);
     }
 }
 
 // A warp per token: dout's row, read once per eight choices, against their rows
 // of y, with eight sums in registers.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_backward_kernel(spmm_combine_args p) {
+__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const __grid_constant__ spmm_combine_args p) {
     const int lane = threadIdx.x & 31, top = (int)p.top;
     const int64_t step = (int64_t)gridDim.x * 8;
     const int64_t w0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -506,20 +557,26 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(spmm_combine_args
                 w[u] = __shfl_sync(kFullMask, weight, u);
             }
             for (int64_t c = lane * VEC; c < p.n; c += 32 * VEC) {
-                float d[VEC], y[8][VEC];
-                load_vec<T, VEC>((const T *)p.dout + t * p.dout_ld + c, d);
+                Raw<T, VEC> dr, y[8];
+                dr.load((const T *)p.dout + t * p.dout_ld + c);
                 if (p.dweights) {
 #pragma unroll
                     for (int u = 0; u < 8; ++u) {
-#pragma unroll
-                        for (int x = 0; x < VEC; ++x) y[u][x] = 0.f;
-                        if (s[u] >= 0) load_vec<T, VEC>((const T *)p.y + s[u] * p.y_ld + c, y[u]);
+                        y[u].clear();
+                        if (s[u] >= 0) y[u].load((const T *)p.y + s[u] * p.y_ld + c);
                     }
+                }
+                float d[VEC];
+                dr.get(d);
+                if (p.dweights) {
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
-                        if (s[u] >= 0)
+                        if (s[u] >= 0) {
+                            float f[VEC];
+                            y[u].get(f);
 #pragma unroll
-                            for (int x = 0; x < VEC; ++x) dot[u] = fmaf(d[x], y[u][x], dot[u]);
+                            for (int x = 0; x < VEC; ++x) dot[u] = fmaf(d[x], f[x], dot[u]);
+                        }
                 }
                 if (p.dy) {
 #pragma unroll
@@ -586,7 +643,7 @@ int run_route(const spmm_route_args &p, cudaStream_t s) {
     }
     const int64_t chunk = chunk_tokens(&p), chunks = ceil_div(p.tokens, chunk);
     int *counts = (int *)p.workspace, *totals = counts + chunks * p.experts;
-    route_choose_kernel<T, V, PACKED><<<(unsigned)chunks, kWarps * 32, e4, s>>>(p, chunk, counts);
+    route_choose_kernel<T, V, PACKED><<<(unsigned)chunks, kChooseWarps * 32, e4, s>>>(p, chunk, counts);
     SPMM_PRODUCT_LAUNCHED();
     route_scan_kernel<<<(unsigned)ceil_div(p.experts, 32), 1024, 0, s>>>(counts, (int)chunks, (int)p.experts, totals);
     SPMM_PRODUCT_LAUNCHED();
@@ -653,12 +710,16 @@ int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
         if (vec) combine_backward_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p);
         else combine_backward_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
     } else {
-        const int64_t chunks = ceil_div(p.n, vec ? 32 * W : 32);
-        if (chunks > INT32_MAX) return SPMM_EUNSUPPORTED;
-        int64_t grid = ceil_div(p.tokens * chunks, 8);
-        if (grid > 148 * 64) grid = 148 * 64;
-        if (vec) combine_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p, (int)chunks);
-        else combine_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p, (int)chunks);
+        const int64_t wide = vec ? 32 * W : 32, chunks = ceil_div(p.n, wide);
+        if (p.n > INT32_MAX - 1024) return SPMM_EUNSUPPORTED;
+        int64_t parts = ceil_div(148 * 24, p.tokens);          // 24 warps an SM are resident
+        if (parts > chunks) parts = chunks;
+        const int64_t cols = ceil_div(chunks, parts) * wide;
+        parts = ceil_div(p.n, cols);
+        int64_t grid = ceil_div(p.tokens * parts, 8);
+        if (grid > 148 * 12) grid = 148 * 12;
+        if (vec) combine_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p, (int)parts, (int)cols);
+        else combine_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p, (int)parts, (int)cols);
     }
     SPMM_PRODUCT_LAUNCHED();
     return SPMM_OK;

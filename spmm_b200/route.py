@@ -9,13 +9,14 @@ stays on the device: no call waits for the GPU.  Not in the reference.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._device import on_device, ptr, stream_handle
+from ._device import on_device, stream_handle
 
 __all__ = ['Routing', 'route_topk', 'route_topk_backward', 'route_combine', 'route_combine_backward', 'SCORINGS']
 
@@ -84,45 +85,47 @@ def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _route_args(logits, top, scoring, renormalize, scale, bias):
-    a = _lib.RouteArgs()
-    a.version, a.dtype = 1, _TYPES[logits.dtype]
-    a.scoring, a.renormalize = SCORINGS.index(scoring), int(bool(renormalize))
-    a.tokens, a.experts, a.top = logits.shape[0], logits.shape[1], top
-    a.logits, a.logits_ld = ptr(logits), logits.stride(0)
-    a.bias, a.scale = ptr(bias), scale
-    return a
+# spmm_route_args and spmm_combine_args (include/spmm_b200.h) packed in one go, see linear.py
+_ROUTE = struct.Struct('@4i3qPqPfi8PQ').pack
+_COMBINE = struct.Struct('@2i5q9P5q').pack
+assert struct.calcsize('@4i3qPqPfi8PQ') == C.sizeof(_lib.RouteArgs)
+assert struct.calcsize('@2i5q9P5q') == C.sizeof(_lib.CombineArgs)
 
 
 def _topk(logits, top, scoring, renormalize, scale, bias):
     logits = _unit_rows(logits)
     device = logits.device
     tokens, experts = logits.shape
-    a = _route_args(logits, top, scoring, renormalize, scale, bias)
     L = _lib.lib()
+    head = (1, _TYPES[logits.dtype], SCORINGS.index(scoring), int(bool(renormalize)), tokens, experts, top,
+            logits.data_ptr(), logits.stride(0), 0 if bias is None else bias.data_ptr(), scale, 0)
     with on_device(device):
-        weights = torch.empty((tokens, top), dtype=torch.float32, device=device)
-        chosen = torch.empty((tokens, top), dtype=torch.int32, device=device)
-        slots = torch.empty((tokens, top), dtype=torch.int32, device=device)
-        rows = torch.empty(tokens * top, dtype=torch.int32, device=device)
-        offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
-        a.weights, a.experts_out, a.slots, a.rows = ptr(weights), ptr(chosen), ptr(slots), ptr(rows)
-        a.offsets = ptr(offsets)
-        n = L.spmm_route_workspace_size(C.byref(a))
-        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        a.workspace, a.workspace_bytes = ptr(ws), n
-        _lib.check(L.spmm_route(C.byref(a), stream_handle(device)), 'route_topk')
+        weights = logits.new_empty((tokens, top), dtype=torch.float32)
+        chosen = logits.new_empty((tokens, top), dtype=torch.int32)
+        slots = torch.empty_like(chosen)
+        rows = chosen.new_empty(tokens * top)
+        offsets = chosen.new_empty(experts + 1)
+        args = head + (weights.data_ptr(), chosen.data_ptr(), slots.data_ptr(), rows.data_ptr(), offsets.data_ptr(),
+                       0, 0)
+        stream = stream_handle(device)
+        rc = L.spmm_route(_ROUTE(*args, 0, 0), stream)
+        if rc == _lib.SPMM_EWORKSPACE:         # said before anything is launched
+            n = L.spmm_route_workspace_size(_ROUTE(*args, 0, 0))
+            ws = torch.empty(n, dtype=torch.uint8, device=device)
+            rc = L.spmm_route(_ROUTE(*args, ws.data_ptr(), n), stream)
+        _lib.check(rc, 'route_topk')
     return weights, chosen, slots, rows, offsets
 
 
 def _topk_backward(dweights, logits, experts, scoring, renormalize, scale):
     logits, dweights = _unit_rows(logits), dweights.contiguous()
     device = logits.device
-    a = _route_args(logits, experts.shape[1], scoring, renormalize, scale, None)
     with on_device(device):
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-        a.experts_out, a.dweights, a.dlogits = ptr(experts), ptr(dweights), ptr(out)
-        _lib.check(_lib.lib().spmm_route_backward(C.byref(a), stream_handle(device)), 'route_topk_backward')
+        out = logits.new_empty(logits.shape)
+        args = _ROUTE(1, _TYPES[logits.dtype], SCORINGS.index(scoring), int(bool(renormalize)), *logits.shape,
+                      experts.shape[1], logits.data_ptr(), logits.stride(0), 0, scale, 0, 0, experts.data_ptr(), 0, 0,
+                      0, dweights.data_ptr(), out.data_ptr(), 0, 0)
+        _lib.check(_lib.lib().spmm_route_backward(args, stream_handle(device)), 'route_topk_backward')
     return out
 
 
@@ -187,41 +190,34 @@ def route_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, routing: R
     return _topk_backward(dweights, logits, routing.experts, scoring, renormalize, float(scale))
 
 
-def _combine_args(y, routing, weights):
-    a = _lib.CombineArgs()
-    a.version, a.dtype = 1, _TYPES[y.dtype]
-    a.tokens, a.top, a.rows, a.n = routing.tokens, routing.top, y.shape[0], y.shape[1]
-    a.experts = routing.num_experts
-    a.slots, a.offsets, a.weights = ptr(routing.slots), ptr(routing.offsets), ptr(weights)
-    a.y, a.y_ld = ptr(y), y.stride(0)
-    return a
-
-
 def _combine(y, routing, weights, residual):
     y, weights = _unit_rows(y), weights.contiguous()
-    device = y.device
-    a = _combine_args(y, routing, weights)
-    with on_device(device):
-        out = torch.empty((routing.tokens, y.shape[1]), dtype=y.dtype, device=device)
-        a.out, a.out_ld = ptr(out), out.stride(0)
+    slots, n = routing.slots, y.shape[1]
+    tokens, top = slots.shape
+    with on_device(y.device):
+        out = y.new_empty((tokens, n))
+        res, res_ld = 0, 0
         if residual is not None:
             residual = _unit_rows(residual)
-            a.residual, a.residual_ld = ptr(residual), residual.stride(0)
-        _lib.check(_lib.lib().spmm_combine(C.byref(a), stream_handle(device)), 'route_combine')
+            res, res_ld = residual.data_ptr(), residual.stride(0)
+        args = _COMBINE(1, _TYPES[y.dtype], tokens, top, y.shape[0], n, routing.num_experts, slots.data_ptr(),
+                        routing.offsets.data_ptr(), weights.data_ptr(), y.data_ptr(), res, out.data_ptr(), 0, 0, 0,
+                        y.stride(0), res_ld, n, 0, 0)
+        _lib.check(_lib.lib().spmm_combine(args, stream_handle(y.device)), 'route_combine')
     return out
 
 
 def _combine_backward(dout, y, routing, weights, need_dy=True, need_dweights=True):
     y, dout, weights = _unit_rows(y), _unit_rows(dout), weights.contiguous()
-    device = y.device
-    a = _combine_args(y, routing, weights)
-    with on_device(device):
-        dy = torch.empty(y.shape, dtype=y.dtype, device=device) if need_dy else None
-        dw = torch.empty(weights.shape, dtype=torch.float32, device=device) if need_dweights else None
-        a.dout, a.dout_ld = ptr(dout), dout.stride(0)
-        a.dy, a.dy_ld = ptr(dy), dy.stride(0) if need_dy else 0
-        a.dweights = ptr(dw)
-        _lib.check(_lib.lib().spmm_combine_backward(C.byref(a), stream_handle(device)), 'route_combine_backward')
+    slots, n = routing.slots, y.shape[1]
+    with on_device(y.device):
+        dy = y.new_empty(y.shape) if need_dy else None
+        dw = weights.new_empty(weights.shape) if need_dweights else None
+        args = _COMBINE(1, _TYPES[y.dtype], *slots.shape, y.shape[0], n, routing.num_experts, slots.data_ptr(),
+                        routing.offsets.data_ptr(), weights.data_ptr(), y.data_ptr(), 0, 0, dout.data_ptr(),
+                        dy.data_ptr() if need_dy else 0, dw.data_ptr() if need_dweights else 0, y.stride(0), 0, 0,
+                        dout.stride(0), n)
+        _lib.check(_lib.lib().spmm_combine_backward(args, stream_handle(y.device)), 'route_combine_backward')
     return dy, dw
 
 

@@ -249,13 +249,16 @@ def test_grouped(cuda, lens, tail, k, n, dtype, act, w_t):
 
 @pytest.mark.parametrize('tokens, experts, top, k, n, masked', [
     (1, 4, 1, 64, 64, 0), (3, 8, 8, 40, 24, 1), (50, 16, 3, 136, 72, 5), (200, 64, 6, 256, 128, 0),
-    (600, 5, 2, 65, 130, 20)])
-def test_grouped_gather(cuda, tokens, experts, top, k, n, masked):
+    (600, 5, 2, 65, 130, 20), (2500, 9, 4, 328, 392, 77), (900, 64, 8, 192, 264, 0)])
+@pytest.mark.parametrize('w_t', [False, True])
+def test_grouped_gather(cuda, tokens, experts, top, k, n, masked, w_t):
     torch.manual_seed(tokens)
     logits = torch.randn(tokens, experts, device='cuda')
     logits[tokens - masked:] = float('-inf')
     weights, r = S.route_topk(logits, top)
     x, w = normal(tokens, k), normal(experts, k, n, scale=k ** -0.5)
+    if w_t:
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
     dy = normal(tokens * top, n)
     gid = group_of(r.offsets.cpu(), tokens * top)
     src = r.rows.long().clamp(min=0)
