@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t *src, int
 
 // ---- gradient of the activation and of the bias -------------------------------
 
-constexpr int kDzRows = 128;   // rows of a tile
+constexpr int kDzRows = 64;    // rows of a tile
 constexpr int kDzCols = 256;   // columns of a CTA: 32 lanes of 8
 
 // dz = dy * act'(z) (rounded to the operands' type) and the tile's column sums

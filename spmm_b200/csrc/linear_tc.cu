@@ -196,14 +196,27 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
         : "r"(t));
 }
 
+// One poll during which the thread may sleep in the hardware until the phase completes (2 us at most): eight
+// epilogue warps wait for most of a tile's time, and polling costs power that the tensor cores could use.
+__device__ __forceinline__ bool poll_asleep(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait for the phase of `bar` with the given parity; false on abort or expiry.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, Bars &s, const TcArgs &a) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     for (;;) {
 #pragma unroll 1
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
+        for (int i = 0; i < 16; ++i)
+            if (poll_asleep(bar, parity)) return true;
         if (s.abort) return false;
         if (clock64() - t0 > a.p.wait_cycles) {
             s.abort = 1;
