@@ -86,7 +86,7 @@ _NOTHING = contextlib.nullcontext()
 
 def on_device(device: torch.device):
     """Context in which `device` is the current one; nothing when it is already."""
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         return _NOTHING
     return torch.cuda.device(device)
 

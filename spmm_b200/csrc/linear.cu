@@ -16,33 +16,71 @@ namespace {
 // ---- operand copies -----------------------------------------------------------
 
 // dst[i][c] = src[map ? map[i] : i][c], rows of `cols` 16-bit values in pieces of
-// 8 (16 bytes, aligned in dst, whose rows are padded), read W values at a time;
-// a map value outside [0, src_rows) gives zeros.  A block of rows per group
-// (blockIdx.y), src_gs / dst_gs apart.
+// 8 (16 bytes, aligned in dst, whose rows are padded), read `width` values at a
+// time; a map value outside [0, src_rows) gives zeros.  `copies` blocks of rows,
+// src_gs / dst_gs apart.
+struct CopyJob {
+    const uint16_t *src;
+    int64_t src_ld, src_gs, src_rows;
+    const int32_t *map;
+    uint16_t *dst;
+    int64_t dst_ld, dst_gs, rows, cols, copies;
+    int32_t width;
+};
+struct Copies {          // the operands of a call that are copied, in one launch
+    CopyJob job[3];
+    int count;
+};
+
 template <int W>
-__global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t *src, int64_t src_ld, int64_t src_gs,
-                                                        int64_t src_rows, const int32_t *map, uint16_t *dst,
-                                                        int64_t dst_ld, int64_t dst_gs, int64_t rows, int64_t cols) {
+__device__ __forceinline__ void copy_piece(const uint16_t *row, int64_t c, int64_t cols, uint16_t (&v)[8]) {
     using V = typename std::conditional<W == 8, uint4, typename std::conditional<W == 4, uint2,
               typename std::conditional<W == 2, uint32_t, uint16_t>::type>::type>::type;
-    src += blockIdx.y * src_gs;
-    dst += blockIdx.y * dst_gs;
-    const int64_t per = dst_ld / 8, items = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per, c = (i - r * per) * 8;
-        const int64_t from = map ? __ldg(map + r) : r;
-        uint16_t v[8];
-        const bool in = from >= 0 && from < src_rows;
 #pragma unroll
-        for (int u = 0; u < 8 / W; ++u) {
-            V x{};
-            if (in && c + u * W < cols) x = __ldg(reinterpret_cast<const V *>(src + from * src_ld + c + u * W));
-            memcpy(v + u * W, &x, sizeof(V));
+    for (int u = 0; u < 8 / W; ++u) {
+        V x{};
+        if (c + u * W < cols) x = __ldg(reinterpret_cast<const V *>(row + c + u * W));
+        memcpy(v + u * W, &x, sizeof(V));
+    }
+}
+
+// I: 32-bit piece numbers where they suffice; two 64-bit divisions a piece took longer than moving it.
+template <typename I>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ Copies all) {
+    const CopyJob &j = all.job[blockIdx.y];
+    const I per = (I)(j.dst_ld / 8), block = (I)j.rows * per, items = block * (I)j.copies;
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < items; i += (I)gridDim.x * 256) {
+        const I g = i / block, k = i - g * block, row_in = k / per;
+        const int64_t r = row_in, c = (int64_t)(k - row_in * per) * 8;
+        const int64_t from = j.map ? __ldg(j.map + r) : r;
+        uint16_t v[8] = {};
+        if (from >= 0 && from < j.src_rows) {
+            const uint16_t *row = j.src + g * j.src_gs + from * j.src_ld;
+            if (j.width == 8) copy_piece<8>(row, c, j.cols, v);
+            else if (j.width == 4) copy_piece<4>(row, c, j.cols, v);
+            else if (j.width == 2) copy_piece<2>(row, c, j.cols, v);
+            else copy_piece<1>(row, c, j.cols, v);
         }
         uint4 o;
         memcpy(&o, v, 16);
-        *reinterpret_cast<uint4 *>(dst + r * dst_ld + c) = o;
+        *reinterpret_cast<uint4 *>(j.dst + g * j.dst_gs + r * j.dst_ld + c) = o;
     }
+}
+
+int run_copies(const Copies &all, cudaStream_t s) {
+    if (all.count == 0) return SPMM_OK;
+    int64_t most = 1, pieces = 0;
+    for (int i = 0; i < all.count; ++i) {
+        const CopyJob &j = all.job[i];
+        const int64_t blocks = ceil_div(j.copies * j.rows * (j.dst_ld / 8), 256);
+        most = blocks > most ? blocks : most;
+        pieces = j.copies * j.rows * (j.dst_ld / 8) > pieces ? j.copies * j.rows * (j.dst_ld / 8) : pieces;
+    }
+    const dim3 grid((unsigned)(most < 148 * 32 ? most : 148 * 32), (unsigned)all.count);
+    if (pieces < INT32_MAX) copy_rows_kernel<uint32_t><<<grid, 256, 0, s>>>(all);
+    else copy_rows_kernel<int64_t><<<grid, 256, 0, s>>>(all);
+    SPMM_PRODUCT_LAUNCHED();
+    return SPMM_OK;
 }
 
 // ---- gradient of the activation and of the bias -------------------------------
@@ -55,13 +93,13 @@ constexpr int kDzCols = 256;   // columns of a CTA: 32 lanes of 8
 // it; bound by reading dy and the slopes and writing dz once.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, const int16_t *slope, T *dz,
-                                                 int64_t dz_ld, float *part, const int32_t *offsets, int64_t groups,
-                                                 int64_t rows, int64_t n) {
+                                                 int64_t dz_ld, float *part, T *dbias, const int32_t *offsets,
+                                                 int64_t groups, int64_t rows, int64_t n) {
     __shared__ float sums[8][kDzCols];
-    const RowTile t = find_row_tile(offsets, groups, rows, kDzRows, blockIdx.y);
+    const RowTile t = find_row_tile(offsets, groups, rows, kDzRows, blockIdx.x);
     if (t.group > groups || (offsets && t.group == groups)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c0 = (int64_t)blockIdx.x * kDzCols + lane * 8;
+    const int64_t c0 = (int64_t)blockIdx.y * kDzCols + lane * 8;
     const int cols = c0 >= n ? 0 : n - c0 < 8 ? (int)(n - c0) : 8;
     float acc[8] = {};
     if (cols) {
@@ -96,16 +134,17 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, con
             for (int e = 0; e < 8; ++e) acc[e] += d[e];
         }
     }
-    if (part == nullptr) return;
+    if (part == nullptr && dbias == nullptr) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = acc[e];
     __syncthreads();
-    const int64_t c = (int64_t)blockIdx.x * kDzCols + threadIdx.x;
+    const int64_t c = (int64_t)blockIdx.y * kDzCols + threadIdx.x;
     if (c < n) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x];
-        part[(int64_t)blockIdx.y * n + c] = v;
+        if (dbias) dbias[c] = from_f32<T>(v);       // the only tile of the only group
+        else part[(int64_t)blockIdx.x * n + c] = v;
     }
 }
 
@@ -208,39 +247,31 @@ bool in_place(const void *p, int64_t ld, int64_t gs, int64_t cols) {
     return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && gs % 8 == 0 && ld >= cols;
 }
 
-// `rows` x `cols` values (per group), gathered by `map` or copied where they are not aligned.
+// `rows` x `cols` values (per group): in place, or a copy (gathered by `map`) that run_copies makes.
 int carve(const Operand src, int64_t src_rows, const int32_t *map, int64_t groups, int64_t rows, int64_t cols,
-          Arena &a, bool sizing, Operand &out, cudaStream_t s) {
+          Arena &a, bool sizing, Operand &out, Copies &copies) {
     out = src;
     if (rows == 0 || cols == 0) return SPMM_OK;
     const int64_t ld = ceil_div(cols, 8) * 8;
     if (rows == 1) out.ld = ld;         // one row: its stride is never used
     if (groups == 1) out.gs = 0;
     if (!map && in_place(src.ptr, out.ld, out.gs, cols)) return SPMM_OK;
-    const int64_t copies = groups > 1 && src.gs == 0 ? 1 : groups;   // a block shared by all groups
+    const int64_t blocks = groups > 1 && src.gs == 0 ? 1 : groups;   // one block shared by all groups
     out.ld = ld;
-    out.gs = copies > 1 ? rows * ld : 0;
-    uint16_t *buf = a.take<uint16_t>(copies * rows * ld);
+    out.gs = blocks > 1 ? rows * ld : 0;
+    uint16_t *buf = a.take<uint16_t>(blocks * rows * ld);
     if (sizing) return SPMM_OK;
     if (!buf) return SPMM_EWORKSPACE;
     out.ptr = buf;
-    const int64_t blocks = ceil_div(rows * (ld / 8), 256);
-    const dim3 grid((unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), (unsigned)copies);
-    const int64_t all = (int64_t)((uintptr_t)src.ptr / 2) | src.ld | (copies > 1 ? src.gs : 0) | cols;
-#define SPMM_COPY(W)                                                                                             \
-    copy_rows_kernel<W><<<grid, 256, 0, s>>>((const uint16_t *)src.ptr, src.ld, src.gs, src_rows, map, buf, ld, \
-                                             out.gs, rows, cols)
-    if (all % 8 == 0) SPMM_COPY(8);
-    else if (all % 4 == 0) SPMM_COPY(4);
-    else if (all % 2 == 0) SPMM_COPY(2);
-    else SPMM_COPY(1);
-#undef SPMM_COPY
-    SPMM_PRODUCT_LAUNCHED();
+    const int64_t all = (int64_t)((uintptr_t)src.ptr / 2) | src.ld | (blocks > 1 ? src.gs : 0) | cols;
+    const int32_t width = all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+    copies.job[copies.count++] = CopyJob{(const uint16_t *)src.ptr, src.ld, src.gs, src_rows, map, buf,
+                                         ld, out.gs, rows, cols, blocks, width};
     return SPMM_OK;
 }
 
-int carve_x(const spmm_linear *p, Arena &a, bool sizing, Operand &x, cudaStream_t s) {
-    return carve({p->x, p->x_ld, 0}, p->x_rows, p->gather, 1, p->rows, p->k, a, sizing, x, s);
+int carve_x(const spmm_linear *p, Arena &a, bool sizing, Operand &x, Copies &copies) {
+    return carve({p->x, p->x_ld, 0}, p->x_rows, p->gather, 1, p->rows, p->k, a, sizing, x, copies);
 }
 
 // w's strides along n, k and the groups, in place or of the copy.
@@ -249,11 +280,11 @@ struct Weight {
     int64_t n, k, g;
 };
 
-int carve_w(const spmm_linear *p, Arena &a, bool sizing, Weight &w, cudaStream_t s) {
+int carve_w(const spmm_linear *p, Arena &a, bool sizing, Weight &w, Copies &copies) {
     const bool n_unit = p->w_n == 1;
     Operand o;
     SPMM_TRY(carve({p->w, n_unit ? p->w_k : p->w_n, p->w_g}, n_unit ? p->k : p->n, nullptr, p->groups,
-                   n_unit ? p->k : p->n, n_unit ? p->n : p->k, a, sizing, o, s));
+                   n_unit ? p->k : p->n, n_unit ? p->n : p->k, a, sizing, o, copies));
     w = n_unit ? Weight{o.ptr, 1, o.ld, o.gs} : Weight{o.ptr, o.ld, 1, o.gs};
     return SPMM_OK;
 }
@@ -273,7 +304,8 @@ Product base(const spmm_linear *p) {
 int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     Operand x;
     Weight w;
-    SPMM_TRY(carve_w(p, a, sizing, w, s));
+    Copies copies{};
+    SPMM_TRY(carve_w(p, a, sizing, w, copies));
     Product g = base(p);
     g.P = p->n;
     g.Q = p->rows;
@@ -289,8 +321,9 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
         g.gather_rows = p->x_rows;
         x = Operand{p->x, p->x_ld, 0};
     } else {
-        SPMM_TRY(carve_x(p, a, sizing, x, s));
+        SPMM_TRY(carve_x(p, a, sizing, x, copies));
     }
+    SPMM_TRY(run_copies(copies, s));
     g.B = x.ptr;
     g.b_q = x.ld;
     g.C = p->y;
@@ -307,39 +340,46 @@ template <typename T>
 int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     Operand x{}, dz{p->dy, p->dy_ld, 0};
     Weight w{};
-    if (p->dw) SPMM_TRY(carve_x(p, a, sizing, x, s));
-    if (p->dx) SPMM_TRY(carve_w(p, a, sizing, w, s));
+    Copies copies{};
+    if (p->dw) SPMM_TRY(carve_x(p, a, sizing, x, copies));
+    if (p->dx) SPMM_TRY(carve_w(p, a, sizing, w, copies));
     const int64_t tiles = ceil_div(p->rows, kDzRows) + (p->offsets ? p->groups + 1 : 0);
-    if (tiles > 65535) return SPMM_EUNSUPPORTED;
+    const bool any = p->rows > 0 && p->n > 0, probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
+    const bool make_dz = p->slope && any && (p->dx || p->dw);
+    const bool one_tile = p->dbias && any && tiles == 1 && !p->offsets;
+    const bool parts = p->dbias && any && !one_tile, sums = p->dx && p->gather;
+    if (ceil_div(p->n, kDzCols) > 65535) return SPMM_EUNSUPPORTED;
     T *dzp = nullptr;
     float *part = nullptr, *dxs = nullptr;
-    const bool any = p->rows > 0 && p->n > 0, probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
-    if (p->slope && any && (p->dx || p->dw)) {
+    if (make_dz) {
         const int64_t ld = ceil_div(p->n, 8) * 8;
         dzp = a.take<T>(p->rows * ld);
         dz = Operand{dzp, ld, 0};
     } else if (any && (p->dx || p->dw)) {
-        SPMM_TRY(carve(dz, p->rows, nullptr, 1, p->rows, p->n, a, sizing, dz, s));
+        SPMM_TRY(carve(dz, p->rows, nullptr, 1, p->rows, p->n, a, sizing, dz, copies));
     }
-    if (p->dbias && any) part = a.take<float>(tiles * p->n);
-    if (p->dx && p->gather) dxs = a.take<float>(p->rows * p->k);
-    if (!sizing && ((p->slope && any && (p->dx || p->dw) && !dzp) || (p->dbias && any && !part) || (p->dx && p->gather && !dxs)))
-        return SPMM_EWORKSPACE;
-    if (!sizing && (dzp || part)) {
-        const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
-        const dim3 grid((unsigned)ceil_div(p->n, kDzCols), (unsigned)tiles);
-        if (vec)
-            dz_kernel<T, true><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, p->offsets,
-                                                    p->groups, p->rows, p->n);
-        else
-            dz_kernel<T, false><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part,
-                                                     p->offsets, p->groups, p->rows, p->n);
-        SPMM_PRODUCT_LAUNCHED();
-    }
-    if (!sizing && p->dbias && p->n) {
-        dbias_kernel<T><<<dim3((unsigned)ceil_div(p->n, 128), (unsigned)p->groups), 128, 0, s>>>(
-            part, p->offsets, any ? p->rows : 0, p->n, (T *)p->dbias, p->dbias_g);
-        SPMM_PRODUCT_LAUNCHED();
+    if (parts) part = a.take<float>(tiles * p->n);
+    if (sums) dxs = a.take<float>(p->rows * p->k);
+    if (!sizing) {
+        if ((make_dz && !dzp) || (parts && !part) || (sums && !dxs)) return SPMM_EWORKSPACE;
+        SPMM_TRY(run_copies(copies, s));
+        if (make_dz || parts || one_tile) {
+            const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
+            const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p->n, kDzCols));
+            T *direct = one_tile ? (T *)p->dbias : nullptr;
+            if (vec)
+                dz_kernel<T, true><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct,
+                                                        p->offsets, p->groups, p->rows, p->n);
+            else
+                dz_kernel<T, false><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part,
+                                                         direct, p->offsets, p->groups, p->rows, p->n);
+            SPMM_PRODUCT_LAUNCHED();
+        }
+        if (p->dbias && p->n && !one_tile) {
+            dbias_kernel<T><<<dim3((unsigned)ceil_div(p->n, 128), (unsigned)p->groups), 128, 0, s>>>(
+                part, p->offsets, any ? p->rows : 0, p->n, (T *)p->dbias, p->dbias_g);
+            SPMM_PRODUCT_LAUNCHED();
+        }
     }
     if (p->dx) {
         Product g = base(p);
@@ -430,6 +470,7 @@ extern "C" int spmm_linear_forward(const spmm_linear *p, spmm_stream_t stream) {
     const int64_t out = p->rows * p->n;
     if (out && !p->y) return SPMM_EINVAL;
     if (out && p->k && (!p->x || !p->w)) return SPMM_EINVAL;
+    if (p->rows > 1 && p->y_ld < p->n) return SPMM_EINVAL;
     if (spmm::short_of(p, spmm::forward)) return SPMM_EWORKSPACE;
     SPMM_TRY(spmm::clear_status(p, out > 0, (cudaStream_t)stream));
     spmm::Arena a(p->workspace, p->workspace_bytes);
@@ -441,6 +482,7 @@ extern "C" int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream) 
     if (p->rows * p->n && !p->dy) return SPMM_EINVAL;
     if (p->dx && ((p->k * p->n && !p->w) || (p->gather && (!p->slots || p->top < 1)))) return SPMM_EINVAL;
     if (p->dw && ((p->rows * p->k && !p->x) || (p->dw_k != 1 && p->dw_n != 1))) return SPMM_EINVAL;
+    if (p->dx && p->x_rows > 1 && p->dx_ld < p->k) return SPMM_EINVAL;
     if (spmm::short_of(p, spmm::backward)) return SPMM_EWORKSPACE;
     const bool product = (p->dx && p->rows * p->k) || (!p->dx && p->dw && p->k * p->n);
     SPMM_TRY(spmm::clear_status(p, product, (cudaStream_t)stream));

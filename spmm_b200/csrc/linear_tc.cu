@@ -361,34 +361,67 @@ __device__ __forceinline__ int mma_cols(int nq) {
 // ---- epilogue -----------------------------------------------------------------------
 
 // A warp's 32 x 32 piece of the result goes through 2 KB of shared memory, so
-// that it leaves as 16-byte stores of 64 contiguous bytes a row: 2-byte stores
-// straight from the accumulator's layout (lane = p) cost 15 cycles each, 15,500
-// a 128 x 256 tile, as much as summing it over 2048.
+// that it leaves as runs of 64 contiguous bytes a row: 2-byte stores straight
+// from the accumulator's layout (lane = p) cost 15 cycles each, 15,500 a 128 x
+// 256 tile, as much as summing it over 2048.  16-bit values travel as words of
+// two neighbouring columns, which halves the shared-memory accesses: the MMAs'
+// operands and the copies already take nearly all of its bandwidth.
 //
 // put(j) gives this lane's value of column j; the values of columns [0, n) are
 // stored at base + j * ld (lane 0's first).  `cols`: valid p from lane 0's on.
 template <typename O, typename F>
 __device__ __forceinline__ void store_piece(uint8_t *stage, O *base, int64_t ld, bool vec, int cols, int n, F put) {
-    constexpr int kPass = 2048 / (32 * sizeof(O));      // columns per pass
-    constexpr int kPer = 16 / sizeof(O), kLanes = 32 / kPer, kRows = 32 / kLanes;
-    const int lane = threadIdx.x & 31;
-    const int row = lane / kLanes, at = (lane % kLanes) * kPer;
-#pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += kPass) {
+    const int lane = threadIdx.x & 31, row = lane >> 3, at = (lane & 7) * 4;   // a lane moves 4 p
+    if constexpr (sizeof(O) == 2) {
+        uint32_t *word = (uint32_t *)stage;
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < kPass; ++j) ((O *)stage)[j * 32 + lane] = put(j0 + j);
+        for (int j = 0; j < 16; ++j) word[j * 32 + lane] = put(2 * j);
         __syncwarp();
-        if (vec && at + kPer <= cols) {
 #pragma unroll
-            for (int j = row; j < kPass; j += kRows) {
-                const uint4 v = *(const uint4 *)((O *)stage + j * 32 + at);
-                if (j0 + j < n) *(uint4 *)(base + (int64_t)(j0 + j) * ld + at) = v;
+        for (int i = 0; i < 4; ++i) {
+            const int j = i * 4 + row;
+            const uint4 w = *(const uint4 *)(word + j * 32 + at);
+            const uint2 even{__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410)};
+            const uint2 odd{__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632)};
+            O *out = base + (int64_t)(2 * j) * ld + at;
+            if (vec && at + 4 <= cols) {
+                if (2 * j < n) *(uint2 *)out = even;
+                if (2 * j + 1 < n) *(uint2 *)(out + ld) = odd;
+            } else {             // unaligned results and the last, partial run
+                O e[4], o[4];
+                memcpy(e, &even, 8);
+                memcpy(o, &odd, 8);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if (2 * j < n && at + x < cols) out[x] = e[x];
+                    if (2 * j + 1 < n && at + x < cols) out[ld + x] = o[x];
+                }
             }
-        } else {                 // unaligned results and the last, partial 16 bytes
-            for (int j = row; j < kPass; j += kRows)
-                for (int e = 0; e < kPer; ++e)
-                    if (j0 + j < n && at + e < cols) base[(int64_t)(j0 + j) * ld + at + e] = ((O *)stage)[j * 32 + at + e];
+        }
+    } else {
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 16) {
+            float *value = (float *)stage;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) value[j * 32 + lane] = put(j0 + j);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = i * 4 + row;
+                const float4 v = *(const float4 *)(value + j * 32 + at);
+                O *out = base + (int64_t)(j0 + j) * ld + at;
+                if (j0 + j >= n) continue;
+                if (vec && at + 4 <= cols) {
+                    *(float4 *)out = v;
+                } else {
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (at + x < cols) out[x] = e[x];
+                }
+            }
         }
     }
 }
@@ -397,20 +430,63 @@ __device__ __forceinline__ void store_piece(uint8_t *stage, O *base, int64_t ld,
 template <typename T>
 __device__ __forceinline__ void load_piece(uint8_t *stage, const T *base, int64_t ld, bool vec, int cols, int n,
                                            float (&r)[32]) {
-    const int lane = threadIdx.x & 31, row = lane / 4, at = (lane % 4) * 8;
-    __syncwarp();
-    if (vec && at + 8 <= cols) {
+    const int lane = threadIdx.x & 31, row = lane >> 3, at = (lane & 7) * 4;
+    uint32_t *word = (uint32_t *)stage;
+    uint2 v[8];
 #pragma unroll
-        for (int j = row; j < 32; j += 8)
-            if (j < n) *(uint4 *)((T *)stage + j * 32 + at) = __ldg((const uint4 *)(base + (int64_t)j * ld + at));
-    } else {
-        for (int j = row; j < 32; j += 8)
-            for (int e = 0; e < 8; ++e)
-                if (j < n && at + e < cols) ((T *)stage)[j * 32 + at + e] = base[(int64_t)j * ld + at + e];
+    for (int i = 0; i < 8; ++i) {
+        const int j = (i >> 1) * 8 + row * 2 + (i & 1);
+        const T *src = base + (int64_t)j * ld + at;
+        v[i] = uint2{0, 0};
+        if (vec && at + 4 <= cols) {
+            if (j < n) v[i] = __ldg((const uint2 *)src);
+        } else {
+            T e[4] = {};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (j < n && at + x < cols) e[x] = src[x];
+            memcpy(&v[i], e, 8);
+        }
     }
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = to_f32(((const T *)stage)[j * 32 + lane]);
+    for (int i = 0; i < 4; ++i) {
+        const uint2 a = v[2 * i], b = v[2 * i + 1];
+        *(uint4 *)(word + (i * 4 + row) * 32 + at) =
+            uint4{__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410),
+                  __byte_perm(a.y, b.y, 0x7632)};
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const uint32_t w = word[j * 32 + lane];
+        T e[2];
+        memcpy(e, &w, 4);
+        r[2 * j] = to_f32(e[0]);
+        r[2 * j + 1] = to_f32(e[1]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    T e[2] = {from_f32<T>(a), from_f32<T>(b)};
+    uint32_t w;
+    memcpy(&w, e, 4);
+    return w;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    uint32_t w;
+    memcpy(&w, &v, 4);
+    return w;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    uint32_t w;
+    memcpy(&w, &v, 4);
+    return w;
 }
 
 // Columns [c0, c0 + n) of a tile, n <= 32, for the warp whose first p is p0: v[j] is column c0 + j at this lane.
@@ -430,10 +506,13 @@ __device__ __forceinline__ void store_columns(const TcArgs &a, const Tile &t, ui
         for (int j = 0; j < 32; ++j) y[j] += r[j];
     }
     store_piece<O>(stage, (O *)p.C + (p.red ? t.group * p.c_g : 0) + t.part * a.part_stride + q * p.c_q + p0, p.c_q, a.vec_out, cols, n,
-                   [&](int j) { return from_f32<O>(y[j]); });
+                   [&](int j) {
+                       if constexpr (sizeof(O) == 2) return pack2<O>(y[j], y[j + 1]);
+                       else return y[j];
+                   });
     if constexpr (SLOPE)
         store_piece<uint16_t>(stage, (uint16_t *)p.slope + q * p.P + p0, p.P, a.vec_slope, cols, n,
-                              [&](int j) { return slope_code(d[j]); });
+                              [&](int j) { return (uint32_t)slope_code(d[j]) | (uint32_t)slope_code(d[j + 1]) << 16; });
 }
 
 template <typename T, typename O, int ACT>
@@ -817,7 +896,7 @@ Choice choose(const Product &p, int sms) {
             if (s > 1 && (p.offsets || p.out_f32 || steps < 4 * s || np * nq * s * c.cg > sms)) break;
             const double rounds = std::ceil(np * nq * s * c.cg / sms);
             double t = rounds * (std::ceil(steps / s) * c.step + c.tile);
-            if (s > 1) t += 4000 + (double)p.P * (double)p.Q * s * 4 / 4000;
+            if (s > 1) t += 9000 + (double)p.P * (double)p.Q * s * 4 / 4000;    // a second launch, every part once more
             if (t < least) {
                 least = t;
                 best = Choice{c.cg, c.bq, s};

@@ -70,18 +70,21 @@ class _Groups:
         return self.offsets.data_ptr(), self.gather.data_ptr(), self.slots.data_ptr(), self.slots.shape[1]
 
 
-def _call(name, fixed, x, where):
-    """Runs a C entry on x's device and stream; returns the call's status word.  A call that needs scratch says
-    so before it does anything and is repeated with it."""
+def _call(name, fixed, x, where, scratch):
+    """Runs a C entry on x's device and stream; returns the call's status word.  Where `scratch` says that a
+    workspace is likely its size is asked for first; a call that needs one after all says so before it does
+    anything and is repeated with it."""
     L = _lib.lib()
     run = getattr(L, name)
     stream = stream_handle(x.device)
     word = x.new_empty(2)                       # 4 bytes
-    rc = run(_PACK(*fixed, 0, 0, word.data_ptr()), stream)
+    rc = _lib.SPMM_EWORKSPACE
+    if not scratch:
+        rc = run(_PACK(*fixed, 0, 0, word.data_ptr()), stream)
     if rc == _lib.SPMM_EWORKSPACE:
         n = getattr(L, name + '_workspace_size')(_PACK(*fixed, 0, 0, 0))
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        rc = run(_PACK(*fixed, ws.data_ptr(), n, word.data_ptr()), stream)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        rc = run(_PACK(*fixed, ws.data_ptr() if n else 0, n, word.data_ptr()), stream)
     if rc:
         _lib.check(rc, where)
     return word
@@ -109,7 +112,8 @@ def _forward(x, w, g, bias, residual, activation, want_slope):
             1, _TYPES[x.dtype], _ACT[activation], 0, 0, 0, rows, k, n, g.count, x.shape[0], *g.pointers(),
             x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(),
             0 if residual is None else residual.data_ptr(), y.data_ptr(), 0 if slope is None else slope.data_ptr(),
-            0, 0, 0, 0, x.stride(0), sk, sn, sg, bias_g, res_ld, n, 0, 0, 0, 0, 0, 0), x, 'matmul')
+            0, 0, 0, 0, x.stride(0), sk, sn, sg, bias_g, res_ld, n, 0, 0, 0, 0, 0, 0), x, 'matmul',
+            (k | (n if sn == 1 else 0)) % 8 != 0)
     return y, slope, status
 
 
@@ -137,7 +141,7 @@ def _backward(dy, x, w, g, slope, need_dx, need_dw, need_dbias):
             x.data_ptr(), w.data_ptr(), 0, 0, 0, 0 if slope is None else slope.data_ptr(), dy.data_ptr(),
             0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
             0 if dbias is None else dbias.data_ptr(), x.stride(0), sk, sn, sg, 0, 0, 0, dy.stride(0), k, dw_k, dw_n,
-            k * n, n), x, 'matmul_backward')
+            k * n, n), x, 'matmul_backward', slope is not None or g.gather is not None or (k | n) % 8 != 0)
     for t in (dx, dw, dbias):
         if t is not None:
             t._spmm_status = status
@@ -166,26 +170,26 @@ class _MatMul(torch.autograd.Function):
 
 def _check_xw(x, w, w_dim):
     for name, t in (('x', x), ('w', w)):
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+        if not isinstance(t, torch.Tensor) or t.layout is not torch.strided:
             raise ValueError(f'{name} must be a dense tensor')
     if w.dim() != w_dim:
         raise ValueError(f'Expected {w_dim}D w, got {w.dim()}D')
     if x.dtype not in _TYPES:
         raise TypeError(f'x must be bfloat16 or float16, got {x.dtype}')
-    if w.dtype != x.dtype:
+    if w.dtype is not x.dtype:
         raise TypeError(f'w dtype must match x ({x.dtype}), got {w.dtype}')
     if x.dim() < 1 or x.shape[-1] != w.shape[-2]:
         raise ValueError(f'x has {x.shape[-1] if x.dim() else 0} columns, expected {w.shape[-2]}')
-    if w.device != x.device:
+    if w.get_device() != x.get_device():
         raise ValueError('w must be on x\'s device')
 
 
 def _check_like(name, t, x, shape):
-    if t.shape != shape or t.layout != torch.strided:
-        raise ValueError(f'{name} must be {tuple(shape)}, got {tuple(t.shape)}')
-    if t.dtype != x.dtype:
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.layout is not torch.strided:
+        raise ValueError(f'{name} must be a dense tensor of shape {tuple(shape)}')
+    if t.dtype is not x.dtype:
         raise TypeError(f'{name} dtype must match x ({x.dtype}), got {t.dtype}')
-    if t.device != x.device:
+    if t.get_device() != x.get_device():
         raise ValueError(f'{name} must be on x\'s device')
 
 
@@ -200,7 +204,9 @@ def _run(x, w, g, bias, residual, activation, return_slope):
         y, slope, status = _forward(x, w, g, bias, residual, activation, True)
         y._spmm_status = status
         return y, slope
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad
+                                    or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         y, status = _MatMul.apply(x, w, bias, residual, activation, g)
     else:
         y, _, status = _forward(x, w, g, bias, residual, activation, False)
@@ -220,7 +226,7 @@ def dense_matmul(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] 
     involve no autograd graph: ``(y, slope)`` comes back, ``slope`` (int16
     fixed point, None without an activation) being the activation's derivative.
     """
-    if activation not in ACTIVATIONS:
+    if activation not in _ACT:
         raise ValueError(f'activation must be one of {ACTIVATIONS}')
     _check_xw(x, w, 2)
     shape = x.shape[:-1] + (w.shape[1],)
@@ -311,7 +317,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, groups: Union[Routing, torc
     checked here: a table that decreases or leaves [0, R] gives wrong values,
     but reads and writes nothing outside the operands.
     """
-    if activation not in ACTIVATIONS:
+    if activation not in _ACT:
         raise ValueError(f'activation must be one of {ACTIVATIONS}')
     _check_xw(x, w, 3)
     if x.dim() != 2:

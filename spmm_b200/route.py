@@ -56,18 +56,19 @@ class Routing:
 def check_routing(r, device=None) -> None:
     if not isinstance(r, Routing):
         raise TypeError(f'routing must be a Routing, got {type(r).__name__}')
+    index = None if device is None else -1 if device.index is None else device.index
     for name, dim in (('experts', 2), ('slots', 2), ('rows', 1), ('offsets', 1)):
         t = getattr(r, name)
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
             raise ValueError(f'routing.{name} must be a contiguous {dim}D int32 tensor')
-        if device is not None and t.device != device:
+        if index is not None and t.get_device() != index:
             raise ValueError('routing must be on the operands\' device')
     if r.experts.shape != r.slots.shape or r.rows.shape[0] != r.slots.numel() or r.offsets.shape[0] < 2:
         raise ValueError('routing arrays do not belong together')
 
 
 def need_cuda(t: torch.Tensor, what: str) -> None:
-    if t.device.type != 'cuda':
+    if not t.is_cuda:
         raise ValueError(f'{what} must be a dense CUDA tensor')
 
 
