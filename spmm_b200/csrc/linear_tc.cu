@@ -61,7 +61,7 @@ struct Shape {
     static constexpr int kStageBytes = kP * 128 + kBRows * 128;
     static constexpr int kStages = CG == 2 ? 6 : BQ == 256 ? 4 : BQ == 128 ? 6 : 8;
     // Rows of a K-major B box.  Few rows come in boxes of 16: one token then costs 2 KB a stage, not 8.
-    static constexpr int kBoxQ = BQ == 64 ? 16 : 64;
+    static constexpr int kBoxQ = BQ == 64 ? 16 : CG == 2 ? 128 : 64;
     static constexpr int kTmem = 2 * BQ;
     static constexpr int kTable = 2 * (SPMM_MAX_GROUPS + 2) * 4;
     static constexpr int kRing = kStages * kStageBytes, kOut = kEpiWarps * 2048;
@@ -113,6 +113,12 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive_local(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
                                          uint32_t bar) {
@@ -152,19 +158,20 @@ __device__ __forceinline__ void commit_local(uint64_t *bar) {
                          smem_u32(bar))
                      : "memory");
     else
-        mma_commit(bar);
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                     : "memory");
 }
 // Arrives on `bar` (of both CTAs of a pair) when the MMAs issued before are done.
 template <int CG>
-__device__ __forceinline__ void commit(uint64_t *bar, uint16_t mask) {
+__device__ __forceinline__ void commit(uint32_t bar, uint16_t mask) {
     if constexpr (CG == 2)
         asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                smem_u32(bar)),
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
             "h"(mask)
             : "memory");
     else
-        mma_commit(bar);
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                     : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void alloc_tmem(uint32_t *dst, uint32_t cols) {
@@ -196,38 +203,51 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&v)[32]) {
         : "r"(t));
 }
 
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // One poll during which the thread may sleep in the hardware until the phase completes (2 us at most): eight
 // epilogue warps wait for most of a tile's time, and polling costs power that the tensor cores could use.
-__device__ __forceinline__ bool poll_asleep(uint64_t *bar, uint32_t parity) {
+__device__ __forceinline__ bool poll_asleep(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.b32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "r"(bar), "r"(parity), "r"(2000u)
         : "memory");
     return ok != 0;
 }
-// Bounded wait for the phase of `bar` with the given parity; false on abort or expiry.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, Bars &s, const TcArgs &a) {
-    if (mbar_try_wait(bar, parity)) return true;
+// The rest of a wait that did not end at once; false on abort or expiry.
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int *abort, int32_t *status,
+                                     long long cycles) {
     const long long t0 = clock64();
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 16; ++i)
             if (poll_asleep(bar, parity)) return true;
-        if (s.abort) return false;
-        if (clock64() - t0 > a.p.wait_cycles) {
-            s.abort = 1;
-            if (a.p.status) atomicCAS(a.p.status, 0, (int)SPMM_ETIMEOUT);
+        if (*abort) return false;
+        if (clock64() - t0 > cycles) {
+            *abort = 1;
+            if (status) atomicCAS(status, 0, (int)SPMM_ETIMEOUT);
             return false;
         }
     }
 }
-// The same for a converged warp: one answer for all lanes, so that they stay converged.
-__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, Bars &s, const TcArgs &a) {
-    return __all_sync(kFullMask, wait_bar(bar, parity, s, a));
+// Bounded wait of a converged warp for the phase of `bar` (shared address) with the given parity: one answer for
+// all lanes, so that they stay converged; false on abort or expiry.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, Bars &s, const TcArgs &a) {
+    if (__all_sync(kFullMask, poll(bar, parity))) return true;
+    return __all_sync(kFullMask, wait_on(bar, parity, &s.abort, a.p.status, a.p.wait_cycles));
 }
 // The same without the abort flag: for copies and MMAs already in flight.
 __device__ __forceinline__ bool drain_bar(uint64_t *bar, uint32_t parity) {
@@ -286,64 +306,66 @@ __device__ __forceinline__ void fill_table(const Product &p, Table t) {
 }
 
 // (p tile, q tile) number i of np x nq: bands of kBand q tiles, within a band every p in turn, q fastest.
-__device__ __forceinline__ void raster(int64_t i, int64_t np, int64_t nq, int64_t &pt, int64_t &qt) {
-    const int64_t band = i / (np * kBand), rest = i - band * np * kBand;
-    const int64_t width = nq - band * kBand < kBand ? nq - band * kBand : kBand;
+__device__ __forceinline__ void raster(uint32_t i, uint32_t np, uint32_t nq, uint32_t &pt, uint32_t &qt) {
+    const uint32_t band = i / (np * kBand), rest = i - band * np * kBand;
+    const uint32_t left = nq - band * kBand, width = left < kBand ? left : kBand;
     pt = rest / width;
     qt = band * kBand + rest - pt * width;
 }
 
-// Tile number i; false behind the last one.
+// Tile number i; false behind the last one.  32-bit numbers (the host checks): every role asks for every tile,
+// and three 64-bit divisions each time showed between tiles.
 template <int CG, int BQ>
-__device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, int64_t i, Tile &o) {
+__device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, uint32_t i, Tile &o) {
     const Product &p = a.p;
-    const int64_t np = (p.P + kP * CG - 1) / (kP * CG);
-    int64_t pt, qt;
+    const uint32_t P = (uint32_t)p.P, Q = (uint32_t)p.Q;
+    const uint32_t np = (P + kP * CG - 1) / (kP * CG);
+    uint32_t pt, qt;
     o.zero = false;
     o.r0 = 0;
     o.last = 0;
-    int64_t len = p.R;
     o.part = 0;
+    int32_t len = (int32_t)p.R;
     if (p.red && p.offsets) {
-        const int64_t nq = (p.Q + BQ - 1) / BQ, per = np * nq;
-        o.group = i / per;
-        if (o.group >= p.groups) return false;
-        raster(i - o.group * per, np, nq, pt, qt);
+        const uint32_t nq = (Q + BQ - 1) / BQ, per = np * nq, g = i / per;
+        if (g >= (uint32_t)p.groups) return false;
+        o.group = g;
+        raster(i - g * per, np, nq, pt, qt);
         o.q0 = qt * BQ;
-        o.nq = (int)(p.Q - o.q0 < BQ ? p.Q - o.q0 : BQ);
-        o.r0 = t.first[o.group];
-        len = t.first[o.group + 1] - o.r0;
+        o.nq = (int)(Q - qt * BQ < BQ ? Q - qt * BQ : BQ);
+        o.r0 = t.first[g];
+        len = t.first[g + 1] - t.first[g];
         if (len < 0) len = 0;
-        o.last = (int)(len & (kR - 1));
+        o.last = len & (kR - 1);
     } else if (p.offsets) {
         const int G = (int)p.groups;
-        const int64_t nq = t.qtiles[G + 1];
+        const uint32_t nq = (uint32_t)t.qtiles[G + 1];
         if (i >= np * nq) return false;
         raster(i, np, nq, pt, qt);
         int lo = 0, hi = G;          // the last group with qtiles[g] <= qt
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (t.qtiles[mid] <= qt) lo = mid; else hi = mid - 1;
+            if ((uint32_t)t.qtiles[mid] <= qt) lo = mid; else hi = mid - 1;
         }
         o.group = lo;
-        o.q0 = t.first[lo] + (qt - t.qtiles[lo]) * BQ;
-        const int64_t left = t.first[lo + 1] - o.q0;
-        o.nq = (int)(left < BQ ? left : BQ);
+        const int32_t q0 = t.first[lo] + (int32_t)(qt - t.qtiles[lo]) * BQ, left = t.first[lo + 1] - q0;
+        o.q0 = q0;
+        o.nq = left < BQ ? left : BQ;
         if (lo == G) {
             o.zero = true;
             len = 0;
         }
     } else {
-        const int64_t nq = (p.Q + BQ - 1) / BQ, all = np * nq;
+        const uint32_t nq = (Q + BQ - 1) / BQ, all = np * nq;
         if (i >= all * a.splits) return false;
-        o.part = (int)(i / all);
+        o.part = a.splits > 1 ? (int)(i / all) : 0;
         raster(i - o.part * all, np, nq, pt, qt);
         o.group = 0;
         o.q0 = qt * BQ;
-        o.nq = (int)(p.Q - o.q0 < BQ ? p.Q - o.q0 : BQ);
+        o.nq = (int)(Q - qt * BQ < BQ ? Q - qt * BQ : BQ);
     }
-    o.p0 = pt * kP * CG;
-    o.steps = (int)((len + kR - 1) / kR);
+    o.p0 = (int64_t)pt * (kP * CG);
+    o.steps = (int)(((uint32_t)len + kR - 1) / kR);
     if (a.splits > 1) {
         const int lo = (int)((int64_t)o.steps * o.part / a.splits);
         o.steps = (int)((int64_t)o.steps * (o.part + 1) / a.splits) - lo;
@@ -583,35 +605,43 @@ __device__ __forceinline__ void zero_rows(uint8_t *stage, int bytes, int last) {
 }
 
 // The producer: a step's boxes into the next stage of the ring.  Called by the
-// whole warp, an elected lane issues.
+// whole warp, an elected lane issues.  What a tile fixes is worked out once a
+// tile: with everything inside the step, issuing three copies took 350 cycles
+// of the 512 that the MMAs of a pair's step take.
 template <int CG, int BQ>
 struct Loader {
+    using Sh = Shape<CG, BQ>;
     const Maps &maps;
     const TcArgs &a;
-    Bars &s;
-    uint8_t *ring;
-    uint32_t rank, lead;
+    uint32_t full, full_lead, tail, ring;    // shared addresses; the barriers of the pair's first CTA
+    uint32_t rank;
     uint32_t n, st, ph;      // steps issued; the next stage and its phase
     uint32_t tails, odd;     // pairs: bit st, whether stage st has held a ragged last step; an odd number of them
+    int32_t pa, qb, g, r;    // the tile's coordinates
+    uint32_t bytes;
+    int boxes;
 
-    __device__ __forceinline__ void step(const Tile &t, int k) {
-        using Sh = Shape<CG, BQ>;
+    __device__ __forceinline__ void open(const Tile &t) {
+        const int mine = mma_cols<CG>(t.nq) / CG, box_rows = a.b_kmajor ? Sh::kBoxQ : 64;   // B rows of this CTA
+        boxes = (mine + box_rows - 1) / box_rows;
+        bytes = kP * 128 + boxes * box_rows * 128;
+        pa = (int32_t)t.p0 + rank * kP;
+        qb = (int32_t)t.q0 + rank * mine;
+        g = a.a_grouped ? (int32_t)t.group : 0;
+        r = (int32_t)t.r0;
+    }
+    // `ragged`: the last step of a tile whose group ends within it.
+    __device__ __forceinline__ void step(bool ragged) {
         if (elect()) {
-            const int mine = mma_cols<CG>(t.nq) / CG, box_rows = a.b_kmajor ? Sh::kBoxQ : 64;   // B rows of this CTA
-            const int boxes = (mine + box_rows - 1) / box_rows;
-            const uint32_t bytes = kP * 128 + boxes * box_rows * 128;
-            const int32_t pa = (int32_t)(t.p0 + rank * kP), qb = (int32_t)(t.q0 + rank * mine);
-            const int32_t g = a.a_grouped ? (int32_t)t.group : 0, r = (int32_t)(t.r0 + (int64_t)k * kR);
-            uint32_t bar = smem_u32(&s.full[st]);
-            if (CG == 2 && t.last && k == t.steps - 1) {   // each CTA has rows to zero first
-                bar = smem_u32(&s.tail[st]);
-                mbar_arrive_expect_tx(&s.tail[st], bytes);
-                if (rank == 0) mbar_arrive(&s.full[st]);
-            } else {
-                if (rank == 0) mbar_arrive_expect_tx(&s.full[st], bytes * CG);
-                if constexpr (CG == 2) bar = map_cta(bar, lead);
+            uint32_t bar = full_lead + st * 8;
+            if (CG == 2 && ragged) {         // each CTA has rows to zero first
+                bar = tail + st * 8;
+                expect(bar, bytes);
+                if (rank == 0) arrive_local(full + st * 8);
+            } else if (rank == 0) {
+                expect(full + st * 8, bytes * CG);
             }
-            const uint32_t dst = smem_u32(ring + st * Sh::kStageBytes), db = dst + kP * 128;
+            const uint32_t dst = ring + st * Sh::kStageBytes, db = dst + kP * 128;
             if (a.a_kmajor) {
                 tma_load<CG>(dst, &maps.a, r, pa, g, bar);
             } else {
@@ -629,10 +659,11 @@ struct Loader {
             }
         }
         __syncwarp();
-        if (CG == 2 && t.last && k == t.steps - 1) {
+        if (CG == 2 && ragged) {
             tails |= 1u << st;
             odd ^= 1u << st;
         }
+        r += kR;
         ++n;
         if (++st == Sh::kStages) {
             st = 0;
@@ -656,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t crank = CG == 2 ? cluster_rank() : 0;
     const uint32_t rank = crank % CG, lead = crank - rank;     // within the pair; the pair's first CTA
-    const int64_t first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+    const uint32_t first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
         if (p.R > 0) {
@@ -680,12 +711,15 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         if (a.clear_status && blockIdx.x == 0 && p.status) *p.status = 0;
     }
     if (warp == 2) alloc_tmem<CG>(&s.tmem, Sh::kTmem);
-    Loader<CG, BQ> load{maps, a, s, ring, rank, lead, 0, 0, 0, 0, 0};
+    const uint32_t full = smem_u32(s.full), empty = smem_u32(s.empty), tail = smem_u32(s.tail), peer = smem_u32(s.peer);
+    const uint32_t acc_full = smem_u32(s.acc_full), acc_empty = smem_u32(s.acc_empty);
+    Loader<CG, BQ> load{maps, a, full, CG == 2 ? map_cta(full, lead) : full, tail, smem_u32(ring), rank};
     Tile t;
     if (CG == 1 && warp == 0 && !p.offsets && !a.expire_probe) {   // fill the ring before anything else is ready
         __syncwarp();
         if (get_tile<CG, BQ>(a, table, first_tile, t)) {
-            for (int k = 0; k < t.steps && k < Sh::kStages; ++k) load.step(t, k);
+            load.open(t);
+            for (int k = 0; k < t.steps && k < Sh::kStages; ++k) load.step(false);
         }
     }
     fill_table<BQ>(p, table);
@@ -697,20 +731,20 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 
     if (warp == 0) {
         bool ok = true;
-        if (a.expire_probe) ok = wait_warp(&s.never, 0u, s, a);
-        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
-            for (int k = i == first_tile ? (int)load.n : 0; k < t.steps; ++k) {
-                if (!wait_warp(&s.empty[load.st], load.ph ^ 1, s, a)) {
-                    ok = false;
-                    break;
-                }
-                load.step(t, k);
+        if (a.expire_probe) ok = wait_warp(smem_u32(&s.never), 0u, s, a);
+        int k = (int)load.n;
+        for (uint32_t i = first_tile; ok && get_tile<CG, BQ>(a, table, i, t); i += tile_step, k = 0) {
+            if (k == 0) load.open(t);
+            for (; k < t.steps; ++k) {
+                ok = wait_warp(empty + load.st * 8, load.ph ^ 1, s, a);
+                if (!ok) break;
+                load.step(t.last && k == t.steps - 1);
             }
         }
         const uint32_t n = load.n;
         if (ok) {               // every stage has been read: nothing arrives here after the CTA has left
             for (uint32_t m = n > Sh::kStages ? n - Sh::kStages : 0; m < n; ++m)
-                if (!wait_warp(&s.empty[m % Sh::kStages], (m / Sh::kStages) & 1, s, a)) {
+                if (!wait_warp(empty + m % Sh::kStages * 8, (m / Sh::kStages) & 1, s, a)) {
                     ok = false;
                     break;
                 }
@@ -724,57 +758,69 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     } else if (warp == 1 && rank == 0) {
         const uint16_t both = (uint16_t)(3u << lead);
         uint32_t acc = 0, st = 0, ph = 0, odd = 0;   // accumulators used; stage and its phase; see Loader
-        bool ok = true, issued = false;
+        bool ok = true;
         const uint32_t idesc0 = (1u << 4) | ((uint32_t)a.bf16 << 7) | ((uint32_t)a.bf16 << 10) |
                                 ((a.a_kmajor ? 0u : 1u) << 15) | ((a.b_kmajor ? 0u : 1u) << 16) |
                                 ((uint32_t)(kP * CG >> 4) << 24);
         const uint32_t a_adv = (a.a_kmajor ? 32 : 2048) >> 4, b_adv = (a.b_kmajor ? 32 : 2048) >> 4;
-        for (int64_t i = first_tile; ok && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
+        // descriptors of the first stage; only their low words depend on the stage and on r
+        const uint64_t da0 = smem_desc(smem_u32(ring), a.a_kmajor), db0 = smem_desc(smem_u32(ring) + kP * 128, a.b_kmajor);
+        const uint32_t da_hi = (uint32_t)(da0 >> 32), db_hi = (uint32_t)(db0 >> 32);
+        uint32_t da = (uint32_t)da0, db = (uint32_t)db0;
+        auto mma = [&](uint32_t d, uint32_t idesc, int c, uint32_t accumulate) {
+            mma_f16<CG>(d, (uint64_t)da_hi << 32 | (da + c * a_adv), (uint64_t)db_hi << 32 | (db + c * b_adv), idesc,
+                        accumulate);
+        };
+        for (uint32_t i = first_tile; ok && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             if (t.steps == 0) continue;
             const uint32_t as = acc & 1, ap = (acc >> 1) & 1;
             ++acc;
-            ok = wait_warp(&s.acc_empty[as], ap ^ 1, s, a);
+            ok = wait_warp(acc_empty + as * 8, ap ^ 1, s, a);
             if (!ok) break;
             tc_fence_after();
             const uint32_t idesc = idesc0 | ((uint32_t)(mma_cols<CG>(t.nq) >> 3) << 17), d = tmem + as * BQ;
             for (int k = 0; k < t.steps; ++k) {
-                ok = wait_warp(&s.full[st], ph, s, a);
+                ok = wait_warp(full + st * 8, ph, s, a);
                 if (!ok) break;
-                uint8_t *sa = ring + st * Sh::kStageBytes;
-                int chunks = kR / 16;
-                if (t.last && k == t.steps - 1) {   // rows behind the group: zeros up to the MMA's 16
-                    chunks = (t.last + 15) / 16;
-                    if constexpr (CG == 2) ok = wait_warp(&s.tail[st], odd >> st & 1, s, a);
+                const bool last = k == t.steps - 1;
+                if (t.last && last) {           // rows behind the group: zeros up to the MMA's 16
+                    if constexpr (CG == 2) ok = wait_warp(tail + st * 8, odd >> st & 1, s, a);
                     if (!ok) break;
-                    zero_rows(sa, Sh::kStageBytes, t.last);
+                    zero_rows(ring + st * Sh::kStageBytes, Sh::kStageBytes, t.last);
                     if constexpr (CG == 2) {
-                        ok = wait_warp(&s.peer[st], odd >> st & 1, s, a);
+                        ok = wait_warp(peer + st * 8, odd >> st & 1, s, a);
                         asm volatile("fence.acq_rel.cluster;" ::: "memory");
                     }
                     if (!ok) break;
                     odd ^= 1u << st;
-                }
-                tc_fence_after();
-                if (elect()) {
-                    const uint64_t da = smem_desc(smem_u32(sa), a.a_kmajor);
-                    const uint64_t db = smem_desc(smem_u32(sa + kP * 128), a.b_kmajor);
+                    tc_fence_after();
+                    if (elect())
+                        for (int c = 0; c < (t.last + 15) / 16; ++c) mma(d, idesc, c, k > 0 || c > 0);
+                } else {
+                    tc_fence_after();
+                    if (elect()) {
+                        mma(d, idesc, 0, k > 0);
 #pragma unroll
-                    for (int c = 0; c < kR / 16; ++c)
-                        if (c < chunks)
-                            mma_f16<CG>(d, da + (uint64_t)(c * a_adv), db + (uint64_t)(c * b_adv), idesc,
-                                        k > 0 || c > 0);
-                    commit<CG>(&s.empty[st], both);
-                    if (k == t.steps - 1) commit<CG>(&s.acc_full[as], both);
+                        for (int c = 1; c < kR / 16; ++c) mma(d, idesc, c, 1);
+                    }
                 }
-                issued = true;
                 __syncwarp();
+                if (elect()) {
+                    commit<CG>(empty + st * 8, both);
+                    if (last) commit<CG>(acc_full + as * 8, both);
+                }
+                __syncwarp();
+                da += Sh::kStageBytes >> 4;
+                db += Sh::kStageBytes >> 4;
                 if (++st == Sh::kStages) {
                     st = 0;
                     ph ^= 1;
+                    da = (uint32_t)da0;
+                    db = (uint32_t)db0;
                 }
             }
         }
-        if (!ok && issued) {   // MMAs in flight end before tensor memory is freed
+        if (!ok && acc) {      // MMAs in flight end before tensor memory is freed
             if (elect()) commit_local<CG>(&s.drain);
             __syncwarp();
             drain_bar(&s.drain, 0);
@@ -782,14 +828,14 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         __syncwarp();
     } else if (CG == 2 && warp == 1) {      // the pair's second CTA zeroes its rows of ragged last steps
         uint32_t n = 0, odd = 0;
-        for (int64_t i = first_tile; p.red && p.offsets && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
+        for (uint32_t i = first_tile; p.red && p.offsets && get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             n += t.steps;
             if (t.steps == 0 || t.last == 0) continue;
             const uint32_t st = (n - 1) % Sh::kStages;
-            if (!wait_warp(&s.tail[st], odd >> st & 1, s, a)) break;
+            if (!wait_warp(tail + st * 8, odd >> st & 1, s, a)) break;
             odd ^= 1u << st;
             zero_rows(ring + st * Sh::kStageBytes, Sh::kStageBytes, t.last);
-            if (lane == 0) arrive_cluster(map_cta(smem_u32(&s.peer[st]), lead));
+            if (lane == 0) arrive_cluster(map_cta(peer + st * 8, lead));
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -797,7 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         uint8_t *stage = stages + (warp - 4) * 2048;
         uint32_t acc = 0;
-        for (int64_t i = first_tile; get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
+        for (uint32_t i = first_tile; get_tile<CG, BQ>(a, table, i, t); i += tile_step) {
             const int64_t p0 = t.p0 + rank * kP + quad * 32;
             const bool have = t.steps > 0;
             const uint32_t as = acc & 1, at = lanes + as * BQ;
@@ -805,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             if (have) {
                 const uint32_t ap = (acc >> 1) & 1;
                 ++acc;
-                if (!wait_warp(&s.acc_full[as], ap, s, a)) break;
+                if (!wait_warp(acc_full + as * 8, ap, s, a)) break;
                 tc_fence_after();
             }
             float v[32];
@@ -1005,6 +1051,7 @@ int launch(const Product &p, const How &how, cudaStream_t s) {
     const int64_t np = ceil_div(p.P, kP * CG);
     int64_t tiles = np * (p.red ? p.groups * ceil_div(p.Q, BQ) : ceil_div(p.Q, BQ) + (p.offsets ? p.groups : 0));
     tiles *= how.splits;
+    if (tiles > INT32_MAX / 2) return SPMM_EUNSUPPORTED;
     if (tiles > how.sms / CG) tiles = how.sms / CG;
     auto kernel = tc_kernel<CG, BQ, T, O>;
     static std::atomic<uint64_t> ready{0};        // devices (below 64) on which the kernel may use its shared memory
