@@ -7,11 +7,12 @@
 // depends on float32(logit) + bias alone, so it is exact; weights come from
 // float32 exponentials relative to the row's maximum.
 //
-// Grouping.  A stable counting sort by expert: tokens are cut into chunks, a
-// CTA counts its chunk's choices per expert, one pass turns the counts into
-// first positions, and a CTA per chunk places its choices in order (ranks
-// within a warp by match, warps by a prefix over their counts).  Integer sums
-// only: the result does not depend on the order of the atomics.
+// Grouping.  A stable counting sort by expert: tokens are cut into one chunk per
+// SM, a CTA counts its chunk's choices per expert, and a second kernel's CTA per
+// chunk sums the counts of the chunks before its own and places its choices in
+// order (ranks within a warp by match, warps by a prefix over their counts).
+// Integer sums only: the result does not depend on the order of the atomics.  A
+// third kernel that scanned the counts of 512 chunks cost 5 us and a launch.
 #include <type_traits>
 
 #include "linear.cuh"
@@ -19,8 +20,7 @@
 namespace spmm {
 namespace {
 
-constexpr int kWarps = 8;                  // warps of a CTA that places or differentiates
-constexpr int kChooseWarps = 16;           // of one that chooses: two tokens a warp at 32 tokens a chunk
+constexpr int kWarps = 8;                  // warps of a CTA that differentiates
 constexpr int kMaxExperts = SPMM_MAX_GROUPS;
 constexpr uint32_t kNone = 0x007FFFFFu;    // key of -inf: not selectable, like every smaller key
 
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_r
 }
 
 template <typename T, int V, bool PACKED>
-__global__ void __launch_bounds__(kChooseWarps * 32) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
+__global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
     extern __shared__ int sm[];
     const int experts = (int)p.experts;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) sm[e] = 0;
@@ -300,36 +300,29 @@ __global__ void __launch_bounds__(kChooseWarps * 32) route_choose_kernel(spmm_ro
     for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[(int64_t)blockIdx.x * experts + e] = sm[e];
 }
 
-// counts[chunk][e] -> the chunk's choices of e before it; totals[e].  A CTA per 32 experts, a warp per run of chunks.
-__global__ void __launch_bounds__(1024) route_scan_kernel(int *counts, int chunks, int experts, int *totals) {
-    __shared__ int part[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int e = blockIdx.x * 32 + lane;
-    const int per = (chunks + 31) / 32, a = warp * per, b = a + per < chunks ? a + per : chunks;
-    int s = 0;
-    if (e < experts)
-        for (int c = a; c < b; ++c) s += counts[(int64_t)c * experts + e];
-    part[warp][lane] = s;
-    __syncthreads();
-    int run = 0;
-    for (int w = 0; w < warp; ++w) run += part[w][lane];
-    if (e < experts) {
-        for (int c = a; c < b; ++c) {
-            const int v = counts[(int64_t)c * experts + e];
-            counts[(int64_t)c * experts + e] = run;
-            run += v;
-        }
-        if (warp == 31) totals[e] = run;
-    }
-}
-
-__global__ void __launch_bounds__(kWarps * 32) route_place_kernel(spmm_route_args p, int64_t chunk, const int *counts,
-                                                                  const int *totals) {
+__global__ void __launch_bounds__(1024) route_place_kernel(spmm_route_args p, int64_t chunk, const int *counts,
+                                                           int chunks) {
     extern __shared__ int sm[];
     __shared__ int tmp[33];
     const int experts = (int)p.experts;
     int *base = sm, *wcount = sm + experts;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) base[e] = totals[e];
+    int *before = wcount;              // choices of an expert in earlier chunks, until place() needs the room
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) base[e] = before[e] = 0;
+    __syncthreads();
+    // several threads an expert, each every parts-th chunk: the loads' latency is what this costs
+    const int parts = (int)blockDim.x > experts ? blockDim.x / experts : 1;
+    for (int i = threadIdx.x; i < parts * experts; i += blockDim.x) {
+        const int e = i % experts;
+        int sum = 0, earlier = 0;
+#pragma unroll 8
+        for (int c = i / experts; c < chunks; c += parts) {
+            const int v = __ldg(counts + (int64_t)c * experts + e);
+            earlier += c < (int)blockIdx.x ? v : 0;
+            sum += v;
+        }
+        atomicAdd(base + e, sum);
+        atomicAdd(before + e, earlier);
+    }
     __syncthreads();
     const int total = cta_exclusive(base, experts, tmp);
     if (blockIdx.x == 0) {
@@ -341,8 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_place_kernel(spmm_route_arg
     const int64_t i0 = blockIdx.x * chunk * p.top, i1 = i0 + chunk * p.top < all ? i0 + chunk * p.top : all;
     for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x)
         if (i >= total) p.rows[i] = -1;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x)
-        base[e] += counts[(int64_t)blockIdx.x * experts + e];
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) base[e] += before[e];
     __syncthreads();
     place(p, i0, i1, base, wcount);
 }
@@ -610,7 +602,13 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const __grid_c
 
 // ---- host side --------------------------------------------------------------------
 
-constexpr int64_t kChunks = 512;   // chunks of the grouping, at most
+constexpr int64_t kChunks = 148;   // chunks of the grouping, at most
+
+// Warps of a CTA that keeps an int per expert and warp in shared memory (below 48 KB with the static part).
+int warps_for(int64_t experts, int most) {
+    const int64_t fit = 40 * 1024 / (experts * 4) - 1;
+    return (int)(fit < 1 ? 1 : fit < most ? fit : most);
+}
 
 int check_route(const spmm_route_args *p) {
     if (!p || p->version != 1) return SPMM_EINVAL;
@@ -632,22 +630,20 @@ int64_t chunk_tokens(const spmm_route_args *p) {
 
 template <typename T, int V, bool PACKED>
 int run_route(const spmm_route_args &p, cudaStream_t s) {
-    const int e4 = (int)p.experts * 4;
+    const int e4 = (int)p.experts * 4, most = V <= 8 ? 32 : 16;   // registers: V logits and keys a thread
     if (small_route(&p)) {
-        const int most = V <= 8 ? 32 : 16;   // registers: V logits and keys a thread
-        int warps = (int)(p.tokens < 1 ? 1 : p.tokens < most ? p.tokens : most);
-        while (warps > 1 && (warps + 1) * e4 > 40 * 1024) --warps;   // below 48 KB with the static part
+        const int fit = warps_for(p.experts, most);
+        const int warps = (int)(p.tokens < 1 ? 1 : p.tokens < fit ? p.tokens : fit);
         route_small_kernel<T, V, PACKED><<<1, warps * 32, (warps + 1) * e4, s>>>(p);
         SPMM_PRODUCT_LAUNCHED();
         return SPMM_OK;
     }
     const int64_t chunk = chunk_tokens(&p), chunks = ceil_div(p.tokens, chunk);
-    int *counts = (int *)p.workspace, *totals = counts + chunks * p.experts;
-    route_choose_kernel<T, V, PACKED><<<(unsigned)chunks, kChooseWarps * 32, e4, s>>>(p, chunk, counts);
+    int *counts = (int *)p.workspace;
+    const int choose = (int)(chunk < most ? chunk : most), place = warps_for(p.experts, 32);
+    route_choose_kernel<T, V, PACKED><<<(unsigned)chunks, choose * 32, e4, s>>>(p, chunk, counts);
     SPMM_PRODUCT_LAUNCHED();
-    route_scan_kernel<<<(unsigned)ceil_div(p.experts, 32), 1024, 0, s>>>(counts, (int)chunks, (int)p.experts, totals);
-    SPMM_PRODUCT_LAUNCHED();
-    route_place_kernel<<<(unsigned)chunks, kWarps * 32, (kWarps + 1) * e4, s>>>(p, chunk, counts, totals);
+    route_place_kernel<<<(unsigned)chunks, place * 32, (place + 1) * e4, s>>>(p, chunk, counts, (int)chunks);
     SPMM_PRODUCT_LAUNCHED();
     return SPMM_OK;
 }
@@ -732,7 +728,7 @@ using namespace spmm;
 
 extern "C" size_t spmm_route_workspace_size(const spmm_route_args *p) {
     if (check_route(p) != SPMM_OK || small_route(p)) return 0;
-    return (size_t)(ceil_div(p->tokens, chunk_tokens(p)) + 1) * p->experts * 4;
+    return (size_t)ceil_div(p->tokens, chunk_tokens(p)) * p->experts * 4;
 }
 
 extern "C" int spmm_route(const spmm_route_args *p, spmm_stream_t stream) {

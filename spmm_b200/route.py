@@ -24,7 +24,7 @@ SCORINGS = ('softmax', 'sigmoid')
 _TYPES = {torch.float32: _lib.DENSE_F32, torch.bfloat16: _lib.DENSE_BF16, torch.float16: _lib.DENSE_F16}
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Routing:
     """Rows grouped by expert, all int32 on one CUDA device.
 
@@ -109,11 +109,9 @@ def _topk(logits, top, scoring, renormalize, scale, bias):
         args = head + (weights.data_ptr(), chosen.data_ptr(), slots.data_ptr(), rows.data_ptr(), offsets.data_ptr(),
                        0, 0)
         stream = stream_handle(device)
-        rc = L.spmm_route(_ROUTE(*args, 0, 0), stream)
-        if rc == _lib.SPMM_EWORKSPACE:         # said before anything is launched
-            n = L.spmm_route_workspace_size(_ROUTE(*args, 0, 0))
-            ws = torch.empty(n, dtype=torch.uint8, device=device)
-            rc = L.spmm_route(_ROUTE(*args, ws.data_ptr(), n), stream)
+        n = L.spmm_route_workspace_size(_ROUTE(*args, 0, 0))
+        ws = chosen.new_empty(n // 4) if n else None
+        rc = L.spmm_route(_ROUTE(*args, ws.data_ptr() if n else 0, n), stream)
         _lib.check(rc, 'route_topk')
     return weights, chosen, slots, rows, offsets
 
