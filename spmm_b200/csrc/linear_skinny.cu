@@ -9,9 +9,10 @@
 //
 // r contiguous: KS of a CTA's 8 warps share 4 p and take 256 r each in turn, a
 // lane 8 of them (KS = 1 where there are warps enough without: sharing costs a
-// barrier and leaves a warp little to stream).  p contiguous: a CTA owns 32 p; 4 lanes cover them, so a warp reads 8
-// rows r of 64 bytes at once and 16 warps take 128 r in turn.  Sums over lanes
-// by shuffles, over warps in shared memory, in a fixed order.
+// barrier and leaves a warp little to stream).  p contiguous: a CTA owns WP = 64
+// p (32 where that leaves SMs without work); WP / 8 lanes cover them, so a warp
+// reads 4 (8) rows r of 128 (64) bytes at once and 16 warps take the next ones.
+// Sums over lanes by shuffles, over warps in shared memory, in a fixed order.
 #include "linear.cuh"
 
 namespace spmm {
@@ -82,7 +83,7 @@ __device__ __forceinline__ void rows_rmajor(const Product &p, int64_t g, int64_t
 #pragma unroll
     for (int i = 0; i < kNP; ++i) a[i] = A + (p0 + i < p.P ? p0 + i : p.P - 1) * p.a_p;
     float acc[kNP][R] = {};
-#pragma unroll 2
+#pragma unroll (KS == 1 && R <= 2 ? 4 : 2)
     for (int64_t r = part * 256 + lane * 8; r < p.R; r += KS * 256) {
         uint4 w[kNP], x[R];
 #pragma unroll
@@ -148,19 +149,19 @@ __global__ void __launch_bounds__(256) skinny_rmajor_kernel(const __grid_constan
     }
 }
 
-constexpr int kWP = 32;     // p of a CTA, p contiguous
-constexpr int kWarps = 16;
+constexpr int kWarps = 16;  // of a CTA, p contiguous
 
-template <typename T, typename O, int R>
+template <typename T, typename O, int R, int WP>
 __device__ __forceinline__ void rows_pmajor(const Product &p, int64_t g, int64_t q, int64_t p0, float *sm) {
+    constexpr int kLanes = WP / 8, kRows = 32 / kLanes;       // lanes a row of A, rows a warp
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t pl = p0 + (lane & 3) * 8;
+    const int64_t pl = p0 + (lane % kLanes) * 8;
     const T *A = (const T *)p.A + g * p.a_g + (pl + 8 <= p.P ? pl : 0), *b[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) b[j] = row_of<T>(p, q + j);
     float acc[R][8] = {};
-#pragma unroll 4
-    for (int64_t r = warp * 8 + (lane >> 2); r < p.R; r += kWarps * 8) {
+#pragma unroll 8
+    for (int64_t r = warp * kRows + lane / kLanes; r < p.R; r += kWarps * kRows) {
         const uint4 w = __ldg((const uint4 *)(A + r * p.a_r));
         float x[R], wf[8];
 #pragma unroll
@@ -177,33 +178,33 @@ __device__ __forceinline__ void rows_pmajor(const Product &p, int64_t g, int64_t
         for (int e = 0; e < 8; ++e) {
             float v = acc[j][e];
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(kFullMask, v, o);
-            if (lane < 4) sm[(warp * R + j) * kWP + lane * 8 + e] = v;
+            for (int o = kLanes; o < 32; o <<= 1) v += __shfl_xor_sync(kFullMask, v, o);
+            if (lane < kLanes) sm[(warp * R + j) * WP + lane * 8 + e] = v;
         }
     __syncthreads();
-    if (threadIdx.x < kWP * R) {
+    if (threadIdx.x < WP * R) {
         float z = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) z += sm[w * R * kWP + threadIdx.x];
-        const int64_t pp = p0 + threadIdx.x % kWP;
-        if (pp < p.P) put<T, O>(p, g, q + threadIdx.x / kWP, pp, z);
+        for (int w = 0; w < kWarps; ++w) z += sm[w * R * WP + threadIdx.x];
+        const int64_t pp = p0 + threadIdx.x % WP;
+        if (pp < p.P) put<T, O>(p, g, q + threadIdx.x / WP, pp, z);
     }
     __syncthreads();
 }
 
-template <typename T, typename O>
+template <typename T, typename O, int WP>
 __global__ void __launch_bounds__(kWarps * 32) skinny_pmajor_kernel(const __grid_constant__ Product p, int clear) {
-    __shared__ float sm[kWarps * 4 * kWP];
+    __shared__ float sm[kWarps * 4 * WP];
     if (clear && p.status && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = 0;
-    const int64_t g = blockIdx.y, p0 = (int64_t)blockIdx.x * kWP;
+    const int64_t g = blockIdx.y, p0 = (int64_t)blockIdx.x * WP;
     const Rows w = group_rows(p, g);
-    if (w.zero) return put_zeros<O>(p, w, p0, kWP);
+    if (w.zero) return put_zeros<O>(p, w, p0, WP);
     for (int64_t q = w.q0; q < w.q1;) {
         const int64_t n = w.q1 - q;
-        if (n >= 4) rows_pmajor<T, O, 4>(p, g, q, p0, sm), q += 4;
-        else if (n == 3) rows_pmajor<T, O, 3>(p, g, q, p0, sm), q += 3;
-        else if (n == 2) rows_pmajor<T, O, 2>(p, g, q, p0, sm), q += 2;
-        else rows_pmajor<T, O, 1>(p, g, q, p0, sm), q += 1;
+        if (n >= 4) rows_pmajor<T, O, 4, WP>(p, g, q, p0, sm), q += 4;
+        else if (n == 3) rows_pmajor<T, O, 3, WP>(p, g, q, p0, sm), q += 3;
+        else if (n == 2) rows_pmajor<T, O, 2, WP>(p, g, q, p0, sm), q += 2;
+        else rows_pmajor<T, O, 1, WP>(p, g, q, p0, sm), q += 1;
     }
 }
 
@@ -219,8 +220,11 @@ int run(const Product &p, bool clear, cudaStream_t s) {
             skinny_rmajor_kernel<T, O, 2><<<dim3((unsigned)ceil_div(quads, 4), gy), 256, 0, s>>>(p, clear);
         else
             skinny_rmajor_kernel<T, O, 8><<<dim3((unsigned)quads, gy), 256, 0, s>>>(p, clear);
-    } else
-        skinny_pmajor_kernel<T, O><<<dim3((unsigned)ceil_div(p.P, kWP), gy), kWarps * 32, 0, s>>>(p, clear);
+    } else if (ceil_div(p.P, 64) * (p.Q < p.groups ? p.Q : p.groups) >= 148 * 2) {
+        skinny_pmajor_kernel<T, O, 64><<<dim3((unsigned)ceil_div(p.P, 64), gy), kWarps * 32, 0, s>>>(p, clear);
+    } else {
+        skinny_pmajor_kernel<T, O, 32><<<dim3((unsigned)ceil_div(p.P, 32), gy), kWarps * 32, 0, s>>>(p, clear);
+    }
     SPMM_PRODUCT_LAUNCHED();
     return SPMM_OK;
 }

@@ -41,7 +41,10 @@ constexpr int kP = 128;             // p per CTA
 constexpr int kChunk = kR * 128;    // bytes of 64 rows of 128 bytes
 constexpr int kThreads = 384;     // 4 warps of roles, 8 of the epilogue
 constexpr int kEpiWarps = 8;
-constexpr int kBand = 8;            // q tiles that one sweep over p covers
+// q tiles that one sweep over p covers: sixteen of one group's rows (8192 x 16384 x 4096: 811 us, with 8 833 us, as
+// the weights pass through L2 half as often), eight of ragged groups, whose weights change every few q tiles anyway
+// (4096 x 4096 x 4096 in 8 groups: 303 us, with 16 308 us).
+constexpr int kBandOne = 16, kBandGroups = 8;
 
 struct Maps {
     CUtensorMap a, b;
@@ -305,12 +308,13 @@ __device__ __forceinline__ void fill_table(const Product &p, Table t) {
     if (lane == 0) t.qtiles[G + 1] = before;
 }
 
-// (p tile, q tile) number i of np x nq: bands of kBand q tiles, within a band every p in turn, q fastest.
-__device__ __forceinline__ void raster(uint32_t i, uint32_t np, uint32_t nq, uint32_t &pt, uint32_t &qt) {
-    const uint32_t band = i / (np * kBand), rest = i - band * np * kBand;
-    const uint32_t left = nq - band * kBand, width = left < kBand ? left : kBand;
+// (p tile, q tile) number i of np x nq: bands of `wide` q tiles, within a band every p in turn, q fastest.
+__device__ __forceinline__ void raster(uint32_t i, uint32_t np, uint32_t nq, uint32_t wide, uint32_t &pt,
+                                       uint32_t &qt) {
+    const uint32_t band = i / (np * wide), rest = i - band * np * wide;
+    const uint32_t left = nq - band * wide, width = left < wide ? left : wide;
     pt = rest / width;
-    qt = band * kBand + rest - pt * width;
+    qt = band * wide + rest - pt * width;
 }
 
 // Tile number i; false behind the last one.  32-bit numbers (the host checks): every role asks for every tile,
@@ -330,7 +334,7 @@ __device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, uint32_t i, T
         const uint32_t nq = (Q + BQ - 1) / BQ, per = np * nq, g = i / per;
         if (g >= (uint32_t)p.groups) return false;
         o.group = g;
-        raster(i - g * per, np, nq, pt, qt);
+        raster(i - g * per, np, nq, kBandGroups, pt, qt);
         o.q0 = qt * BQ;
         o.nq = (int)(Q - qt * BQ < BQ ? Q - qt * BQ : BQ);
         o.r0 = t.first[g];
@@ -341,7 +345,7 @@ __device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, uint32_t i, T
         const int G = (int)p.groups;
         const uint32_t nq = (uint32_t)t.qtiles[G + 1];
         if (i >= np * nq) return false;
-        raster(i, np, nq, pt, qt);
+        raster(i, np, nq, kBandGroups, pt, qt);
         int lo = 0, hi = G;          // the last group with qtiles[g] <= qt
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -359,7 +363,7 @@ __device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, uint32_t i, T
         const uint32_t nq = (Q + BQ - 1) / BQ, all = np * nq;
         if (i >= all * a.splits) return false;
         o.part = a.splits > 1 ? (int)(i / all) : 0;
-        raster(i - o.part * all, np, nq, pt, qt);
+        raster(i - o.part * all, np, nq, kBandOne, pt, qt);
         o.group = 0;
         o.q0 = qt * BQ;
         o.nq = (int)(Q - qt * BQ < BQ ? Q - qt * BQ : BQ);
