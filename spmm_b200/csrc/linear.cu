@@ -248,30 +248,28 @@ bool in_place(const void *p, int64_t ld, int64_t gs, int64_t cols) {
 }
 
 // `rows` x `cols` values (per group): in place, or a copy (gathered by `map`) that run_copies makes.
-int carve(const Operand src, int64_t src_rows, const int32_t *map, int64_t groups, int64_t rows, int64_t cols,
-          Arena &a, bool sizing, Operand &out, Copies &copies) {
-    out = src;
-    if (rows == 0 || cols == 0) return SPMM_OK;
+Operand carve(const Operand src, int64_t src_rows, const int32_t *map, int64_t groups, int64_t rows, int64_t cols,
+              Arena &a, Copies &copies) {
+    Operand out = src;
+    if (rows == 0 || cols == 0) return out;
     const int64_t ld = ceil_div(cols, 8) * 8;
     if (rows == 1) out.ld = ld;         // one row: its stride is never used
     if (groups == 1) out.gs = 0;
-    if (!map && in_place(src.ptr, out.ld, out.gs, cols)) return SPMM_OK;
+    if (!map && in_place(src.ptr, out.ld, out.gs, cols)) return out;
     const int64_t blocks = groups > 1 && src.gs == 0 ? 1 : groups;   // one block shared by all groups
     out.ld = ld;
     out.gs = blocks > 1 ? rows * ld : 0;
     uint16_t *buf = a.take<uint16_t>(blocks * rows * ld);
-    if (sizing) return SPMM_OK;
-    if (!buf) return SPMM_EWORKSPACE;
     out.ptr = buf;
     const int64_t all = (int64_t)((uintptr_t)src.ptr / 2) | src.ld | (blocks > 1 ? src.gs : 0) | cols;
     const int32_t width = all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
     copies.job[copies.count++] = CopyJob{(const uint16_t *)src.ptr, src.ld, src.gs, src_rows, map, buf,
                                          ld, out.gs, rows, cols, blocks, width};
-    return SPMM_OK;
+    return out;
 }
 
-int carve_x(const spmm_linear *p, Arena &a, bool sizing, Operand &x, Copies &copies) {
-    return carve({p->x, p->x_ld, 0}, p->x_rows, p->gather, 1, p->rows, p->k, a, sizing, x, copies);
+Operand carve_x(const spmm_linear *p, Arena &a, Copies &copies) {
+    return carve({p->x, p->x_ld, 0}, p->x_rows, p->gather, 1, p->rows, p->k, a, copies);
 }
 
 // w's strides along n, k and the groups, in place or of the copy.
@@ -280,13 +278,11 @@ struct Weight {
     int64_t n, k, g;
 };
 
-int carve_w(const spmm_linear *p, Arena &a, bool sizing, Weight &w, Copies &copies) {
+Weight carve_w(const spmm_linear *p, Arena &a, Copies &copies) {
     const bool n_unit = p->w_n == 1;
-    Operand o;
-    SPMM_TRY(carve({p->w, n_unit ? p->w_k : p->w_n, p->w_g}, n_unit ? p->k : p->n, nullptr, p->groups,
-                   n_unit ? p->k : p->n, n_unit ? p->n : p->k, a, sizing, o, copies));
-    w = n_unit ? Weight{o.ptr, 1, o.ld, o.gs} : Weight{o.ptr, o.ld, 1, o.gs};
-    return SPMM_OK;
+    const int64_t rows = n_unit ? p->k : p->n, cols = n_unit ? p->n : p->k;
+    const Operand o = carve({p->w, n_unit ? p->w_k : p->w_n, p->w_g}, rows, nullptr, p->groups, rows, cols, a, copies);
+    return n_unit ? Weight{o.ptr, 1, o.ld, o.gs} : Weight{o.ptr, o.ld, 1, o.gs};
 }
 
 int64_t wait_cycles(int32_t wait_us) { return wait_us > 0 ? (int64_t)wait_us * 2000 : 1ll << 32; }
@@ -301,11 +297,18 @@ Product base(const spmm_linear *p) {
     return g;
 }
 
-int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
-    Operand x;
-    Weight w;
+// A call lays out its scratch and decides on its kernels first; only then, and
+// if the workspace suffices, it launches anything.  need: the scratch in bytes
+// (all that a sizing call wants).
+int settle(const Arena &a, bool sizing, size_t &need) {
+    need = (a.used + 255) & ~(size_t)255;
+    return !sizing && a.used > a.cap ? SPMM_EWORKSPACE : SPMM_OK;
+}
+
+int forward(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStream_t s) {
+    const bool probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
     Copies copies{};
-    SPMM_TRY(carve_w(p, a, sizing, w, copies));
+    const Weight w = carve_w(p, a, copies);
     Product g = base(p);
     g.P = p->n;
     g.Q = p->rows;
@@ -316,14 +319,13 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     g.a_r = w.k;
     g.a_g = w.g;
     g.b_r = 1;
+    Operand x{p->x, p->x_ld, 0};
     if (p->gather && skinny_fits(g) && in_place(p->x, p->x_ld, 0, p->k)) {   // reads the gathered rows itself
         g.gather = p->gather;
         g.gather_rows = p->x_rows;
-        x = Operand{p->x, p->x_ld, 0};
     } else {
-        SPMM_TRY(carve_x(p, a, sizing, x, copies));
+        x = carve_x(p, a, copies);
     }
-    SPMM_TRY(run_copies(copies, s));
     g.B = x.ptr;
     g.b_q = x.ld;
     g.C = p->y;
@@ -333,22 +335,28 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
     g.residual = p->residual;
     g.residual_ld = p->residual_ld;
     g.slope = p->slope;
-    return launch_product(g, a, sizing, true, p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT, s);
+    ProductPlan plan;
+    SPMM_TRY(plan_product(g, probe, a, plan));
+    SPMM_TRY(settle(a, sizing, need));
+    if (sizing) return SPMM_OK;
+    if (p->status && !plan.launches) SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
+    SPMM_TRY(run_copies(copies, s));
+    return run_product(g, plan, true, probe, s);
 }
 
 template <typename T>
-int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
-    Operand x{}, dz{p->dy, p->dy_ld, 0};
-    Weight w{};
-    Copies copies{};
-    if (p->dw) SPMM_TRY(carve_x(p, a, sizing, x, copies));
-    if (p->dx) SPMM_TRY(carve_w(p, a, sizing, w, copies));
-    const int64_t tiles = ceil_div(p->rows, kDzRows) + (p->offsets ? p->groups + 1 : 0);
+int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStream_t s) {
     const bool any = p->rows > 0 && p->n > 0, probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
+    const int64_t tiles = ceil_div(p->rows, kDzRows) + (p->offsets ? p->groups + 1 : 0);
     const bool make_dz = p->slope && any && (p->dx || p->dw);
     const bool one_tile = p->dbias && any && tiles == 1 && !p->offsets;
     const bool parts = p->dbias && any && !one_tile, sums = p->dx && p->gather;
     if (ceil_div(p->n, kDzCols) > 65535) return SPMM_EUNSUPPORTED;
+    Copies copies{};
+    Operand x{}, dz{p->dy, p->dy_ld, 0};
+    Weight w{};
+    if (p->dw) x = carve_x(p, a, copies);
+    if (p->dx) w = carve_w(p, a, copies);
     T *dzp = nullptr;
     float *part = nullptr, *dxs = nullptr;
     if (make_dz) {
@@ -356,93 +364,83 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
         dzp = a.take<T>(p->rows * ld);
         dz = Operand{dzp, ld, 0};
     } else if (any && (p->dx || p->dw)) {
-        SPMM_TRY(carve(dz, p->rows, nullptr, 1, p->rows, p->n, a, sizing, dz, copies));
+        dz = carve(dz, p->rows, nullptr, 1, p->rows, p->n, a, copies);
     }
     if (parts) part = a.take<float>(tiles * p->n);
     if (sums) dxs = a.take<float>(p->rows * p->k);
-    if (!sizing) {
-        if ((make_dz && !dzp) || (parts && !part) || (sums && !dxs)) return SPMM_EWORKSPACE;
-        SPMM_TRY(run_copies(copies, s));
-        if (make_dz || parts || one_tile) {
-            const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
-            const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p->n, kDzCols));
-            T *direct = one_tile ? (T *)p->dbias : nullptr;
-            if (vec)
-                dz_kernel<T, true><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct,
-                                                        p->offsets, p->groups, p->rows, p->n);
-            else
-                dz_kernel<T, false><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part,
-                                                         direct, p->offsets, p->groups, p->rows, p->n);
-            SPMM_PRODUCT_LAUNCHED();
-        }
-        if (p->dbias && p->n && !one_tile) {
-            dbias_kernel<T><<<dim3((unsigned)ceil_div(p->n, 128), (unsigned)p->groups), 128, 0, s>>>(
-                part, p->offsets, any ? p->rows : 0, p->n, (T *)p->dbias, p->dbias_g);
-            SPMM_PRODUCT_LAUNCHED();
-        }
-    }
+    Product gx = base(p), gw = base(p);
+    ProductPlan px{}, pw{};
     if (p->dx) {
-        Product g = base(p);
-        g.P = p->k;
-        g.Q = p->rows;
-        g.R = p->n;
-        g.A = w.ptr;
-        g.a_p = w.k;
-        g.a_r = w.n;
-        g.a_g = w.g;
-        g.B = dz.ptr;
-        g.b_q = dz.ld;
-        g.b_r = 1;
-        g.C = p->gather ? (void *)dxs : p->dx;
-        g.c_q = p->gather ? p->k : p->dx_ld;
-        g.out_f32 = p->gather != nullptr;
-        SPMM_TRY(launch_product(g, a, sizing, true, probe, s));
-        if (p->gather && !sizing)
-            SPMM_TRY(launch_gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, p->dx, p->dx_ld, g.f16, s));
+        gx.P = p->k;
+        gx.Q = p->rows;
+        gx.R = p->n;
+        gx.A = w.ptr;
+        gx.a_p = w.k;
+        gx.a_r = w.n;
+        gx.a_g = w.g;
+        gx.B = dz.ptr;
+        gx.b_q = dz.ld;
+        gx.b_r = 1;
+        gx.C = sums ? (void *)dxs : p->dx;
+        gx.c_q = sums ? p->k : p->dx_ld;
+        gx.out_f32 = sums;
+        SPMM_TRY(plan_product(gx, probe, a, px));
     }
     if (p->dw) {
-        Product g = base(p);
         const bool n_unit = p->dw_n == 1;
-        g.red = 1;
-        g.R = p->rows;
-        g.P = n_unit ? p->n : p->k;
-        g.Q = n_unit ? p->k : p->n;
-        g.A = n_unit ? dz.ptr : x.ptr;
-        g.a_p = 1;
-        g.a_r = n_unit ? dz.ld : x.ld;
-        g.B = n_unit ? x.ptr : dz.ptr;
-        g.b_q = 1;
-        g.b_r = n_unit ? x.ld : dz.ld;
-        g.C = p->dw;
-        g.c_q = n_unit ? p->dw_k : p->dw_n;
-        g.c_g = p->dw_g;
-        SPMM_TRY(launch_product(g, a, sizing, !p->dx, probe, s));
+        gw.red = 1;
+        gw.R = p->rows;
+        gw.P = n_unit ? p->n : p->k;
+        gw.Q = n_unit ? p->k : p->n;
+        gw.A = n_unit ? dz.ptr : x.ptr;
+        gw.a_p = 1;
+        gw.a_r = n_unit ? dz.ld : x.ld;
+        gw.B = n_unit ? x.ptr : dz.ptr;
+        gw.b_q = 1;
+        gw.b_r = n_unit ? x.ld : dz.ld;
+        gw.C = p->dw;
+        gw.c_q = n_unit ? p->dw_k : p->dw_n;
+        gw.c_g = p->dw_g;
+        SPMM_TRY(plan_product(gw, probe, a, pw));
     }
-    return SPMM_OK;
+    SPMM_TRY(settle(a, sizing, need));
+    if (sizing) return SPMM_OK;
+    if (p->status && !px.launches && !pw.launches)
+        SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
+    SPMM_TRY(run_copies(copies, s));
+    if (make_dz || parts || one_tile) {
+        const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
+        const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p->n, kDzCols));
+        T *direct = one_tile ? (T *)p->dbias : nullptr;
+        if (vec)
+            dz_kernel<T, true><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct,
+                                                    p->offsets, p->groups, p->rows, p->n);
+        else
+            dz_kernel<T, false><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct,
+                                                     p->offsets, p->groups, p->rows, p->n);
+        SPMM_PRODUCT_LAUNCHED();
+    }
+    if (p->dbias && p->n && !one_tile) {
+        dbias_kernel<T><<<dim3((unsigned)ceil_div(p->n, 128), (unsigned)p->groups), 128, 0, s>>>(
+            part, p->offsets, any ? p->rows : 0, p->n, (T *)p->dbias, p->dbias_g);
+        SPMM_PRODUCT_LAUNCHED();
+    }
+    SPMM_TRY(run_product(gx, px, true, probe, s));
+    if (sums)
+        SPMM_TRY(launch_gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, p->dx, p->dx_ld, gx.f16, s));
+    return run_product(gw, pw, !px.launches, probe, s);
 }
 
-int backward(const spmm_linear *p, Arena &a, bool sizing, cudaStream_t s) {
-    return p->dtype == SPMM_DENSE_F16 ? gradients<__half>(p, a, sizing, s)
-                                      : gradients<__nv_bfloat16>(p, a, sizing, s);
+int backward(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStream_t s) {
+    return p->dtype == SPMM_DENSE_F16 ? gradients<__half>(p, a, sizing, need, s)
+                                      : gradients<__nv_bfloat16>(p, a, sizing, need, s);
 }
 
-size_t sized(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool, cudaStream_t)) {
+size_t sized(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool, size_t &, cudaStream_t)) {
     if (check_sizes(p) != SPMM_OK) return 0;
     Arena a(nullptr, 0);
-    (void)run(p, a, true, nullptr);
-    return (a.used + 255) & ~(size_t)255;
-}
-
-// Whether the workspace is too small: asked before anything is launched.
-bool short_of(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool, cudaStream_t)) {
-    const size_t need = sized(p, run);
-    return need && (!p->workspace || p->workspace_bytes < need);
-}
-
-// The products clear the status word themselves; a call without any does it here.
-int clear_status(const spmm_linear *p, bool product, cudaStream_t s) {
-    if (p->status && !product) SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
-    return SPMM_OK;
+    size_t need = 0;
+    return run(p, a, true, need, nullptr) == SPMM_OK ? need : 0;
 }
 
 }  // namespace
@@ -471,10 +469,9 @@ extern "C" int spmm_linear_forward(const spmm_linear *p, spmm_stream_t stream) {
     if (out && !p->y) return SPMM_EINVAL;
     if (out && p->k && (!p->x || !p->w)) return SPMM_EINVAL;
     if (p->rows > 1 && p->y_ld < p->n) return SPMM_EINVAL;
-    if (spmm::short_of(p, spmm::forward)) return SPMM_EWORKSPACE;
-    SPMM_TRY(spmm::clear_status(p, out > 0, (cudaStream_t)stream));
-    spmm::Arena a(p->workspace, p->workspace_bytes);
-    return spmm::forward(p, a, false, (cudaStream_t)stream);
+    spmm::Arena a(p->workspace, p->workspace ? p->workspace_bytes : 0);
+    size_t need;
+    return spmm::forward(p, a, false, need, (cudaStream_t)stream);
 }
 
 extern "C" int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream) {
@@ -483,9 +480,7 @@ extern "C" int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream) 
     if (p->dx && ((p->k * p->n && !p->w) || (p->gather && (!p->slots || p->top < 1)))) return SPMM_EINVAL;
     if (p->dw && ((p->rows * p->k && !p->x) || (p->dw_k != 1 && p->dw_n != 1))) return SPMM_EINVAL;
     if (p->dx && p->x_rows > 1 && p->dx_ld < p->k) return SPMM_EINVAL;
-    if (spmm::short_of(p, spmm::backward)) return SPMM_EWORKSPACE;
-    const bool product = (p->dx && p->rows * p->k) || (!p->dx && p->dw && p->k * p->n);
-    SPMM_TRY(spmm::clear_status(p, product, (cudaStream_t)stream));
-    spmm::Arena a(p->workspace, p->workspace_bytes);
-    return spmm::backward(p, a, false, (cudaStream_t)stream);
+    spmm::Arena a(p->workspace, p->workspace ? p->workspace_bytes : 0);
+    size_t need;
+    return spmm::backward(p, a, false, need, (cudaStream_t)stream);
 }

@@ -176,9 +176,16 @@ struct Product {
     int64_t wait_cycles;
 };
 
+// How a product runs, decided before anything is launched; scratch comes from `arena`.
+struct ProductPlan {
+    bool launches, skinny;
+    int cg, bq, splits;      // tensor-core kernel: CTAs of a tile, its q, parts of the sum over r
+    float *parts;
+    int dev, sms;
+};
+int plan_product(const Product &p, bool probe, Arena &arena, ProductPlan &plan);
 // `clear`: the kernel sets *status to 0 first (the first product of a call); `probe`: SPMM_CFG_EXPIRE_FIRST_WAIT.
-// Scratch comes from `arena`; `sizing` only counts it.
-int launch_product(const Product &p, Arena &arena, bool sizing, bool clear, bool probe, cudaStream_t s);
+int run_product(const Product &p, const ProductPlan &plan, bool clear, bool probe, cudaStream_t s);
 
 // The same for at most four rows per group on average (operands aligned, see skinny_fits).
 bool skinny_fits(const Product &p);

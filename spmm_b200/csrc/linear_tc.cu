@@ -925,28 +925,28 @@ struct Choice {
 Choice choose(const Product &p, int sms) {
     struct Cost {
         int cg, bq;
-        double step, tile;
+        int64_t step, tile;
     };
-    static const Cost costs[] = {{2, 256, 540, 6000}, {1, 128, 600, 3500}, {1, 64, 420, 2500}};
-    const double groups = (double)p.groups;
-    const double steps = (double)ceil_div(p.red && p.offsets ? ceil_div(p.R, p.groups) : p.R, kR);
+    // measured at 4096 x 4096 weights with 16 to 1024 rows: a step of a narrow tile costs nearly what a wide one
+    // does (its weights come through the same 64 bytes a cycle from L2), but there are more tiles to share out
+    static const Cost costs[] = {{2, 256, 540, 6000}, {1, 128, 500, 3500}, {1, 64, 460, 2500}};
+    const int64_t steps = ceil_div(p.red && p.offsets ? ceil_div(p.R, p.groups) : p.R, kR);
     Choice best{2, 256, 1};
-    double least = 1e300;
+    int64_t least = INT64_MAX;
     for (const Cost &c : costs) {
-        const double np = (double)ceil_div(p.P, kP * c.cg);
-        double nq;
-        if (p.red) nq = groups * (double)ceil_div(p.Q, c.bq);
-        else if (!p.offsets) nq = (double)ceil_div(p.Q, c.bq);
-        else {
-            const double per = (double)p.Q / groups;
-            nq = per < 1 ? (double)p.Q : groups * std::ceil(per / c.bq);
-            if (per > c.bq / 2) nq += groups * 0.5;
+        const int64_t np = ceil_div(p.P, kP * c.cg), slots = sms / c.cg;
+        int64_t nq = ceil_div(p.Q, c.bq);
+        if (p.red) {
+            nq *= p.groups;
+        } else if (p.offsets) {      // every group ends within a tile, half a tile early on average
+            const int64_t per = p.Q / p.groups;
+            nq = per < 1 ? p.Q : p.groups * ceil_div(per, c.bq) + (per > c.bq / 2 ? p.groups / 2 : 0);
         }
-        for (int s = 1; s <= 16; ++s) {
-            if (s > 1 && (p.offsets || p.out_f32 || steps < 4 * s || np * nq * s * c.cg > sms)) break;
-            const double rounds = std::ceil(np * nq * s * c.cg / sms);
-            double t = rounds * (std::ceil(steps / s) * c.step + c.tile);
-            if (s > 1) t += 9000 + (double)p.P * (double)p.Q * s * 4 / 4000;    // a second launch, every part once more
+        const int64_t tiles = np * nq;
+        for (int s = 1; s <= 16; s += s < 4 ? 1 : 4) {
+            if (s > 1 && (p.offsets || p.out_f32 || steps < 4 * s || tiles * s > slots)) break;
+            int64_t t = ceil_div(tiles * s, slots) * (ceil_div(steps, s) * c.step + c.tile);
+            if (s > 1) t += 9000 + p.P * p.Q * s / 1000;    // a second launch, every part once more
             if (t < least) {
                 least = t;
                 best = Choice{c.cg, c.bq, s};
@@ -1091,18 +1091,11 @@ int by_shape(const Product &p, const Choice &c, const How &how, cudaStream_t s) 
 }
 
 template <typename T>
-int run(const Product &p, Arena &arena, bool sizing, How how, cudaStream_t s) {
-    const Choice c = choose(p, how.sms);
-    how.splits = c.splits;
-    if (c.splits == 1) {
-        if (sizing) return SPMM_OK;
-        return p.out_f32 ? by_shape<T, float>(p, c, how, s) : by_shape<T, T>(p, c, how, s);
-    }
-    float *parts = arena.take<float>(p.P * p.Q * c.splits);
-    if (sizing) return SPMM_OK;
-    if (!parts) return SPMM_EWORKSPACE;
+int run(const Product &p, const ProductPlan &plan, How how, cudaStream_t s) {
+    const Choice c{plan.cg, plan.bq, plan.splits};
+    if (c.splits == 1) return p.out_f32 ? by_shape<T, float>(p, c, how, s) : by_shape<T, T>(p, c, how, s);
     Product raw = p;          // plain float32 sums of each part
-    raw.C = parts;
+    raw.C = plan.parts;
     raw.c_q = p.P;
     raw.c_g = 0;
     raw.out_f32 = 1;
@@ -1110,18 +1103,37 @@ int run(const Product &p, Arena &arena, bool sizing, How how, cudaStream_t s) {
     raw.bias = raw.residual = nullptr;
     raw.slope = nullptr;
     SPMM_TRY((by_shape<T, float>(raw, c, how, s)));
-    return join<T>(p, parts, c.splits, s);
+    return join<T>(p, plan.parts, c.splits, s);
 }
 
 }  // namespace
 
-int launch_product(const Product &p, Arena &arena, bool sizing, bool clear, bool probe, cudaStream_t s) {
-    if (p.P == 0 || p.Q == 0 || (p.red && p.groups == 0)) return SPMM_OK;
-    if (!probe && skinny_fits(p)) return sizing ? SPMM_OK : launch_skinny(p, clear, s);
-    How how{clear, probe, 1, 0, 148};
-    SPMM_CUDA_TRY(cudaGetDevice(&how.dev));
-    SPMM_CUDA_TRY(cudaDeviceGetAttribute(&how.sms, cudaDevAttrMultiProcessorCount, how.dev));
-    return p.f16 ? run<__half>(p, arena, sizing, how, s) : run<__nv_bfloat16>(p, arena, sizing, how, s);
+int plan_product(const Product &p, bool probe, Arena &arena, ProductPlan &plan) {
+    plan = ProductPlan{};
+    if (p.P == 0 || p.Q == 0) return SPMM_OK;
+    plan.launches = true;
+    plan.skinny = !probe && skinny_fits(p);
+    if (plan.skinny) return SPMM_OK;
+    static std::atomic<int> known[64];        // SMs of a device
+    SPMM_CUDA_TRY(cudaGetDevice(&plan.dev));
+    plan.sms = plan.dev < 64 ? known[plan.dev].load(std::memory_order_relaxed) : 0;
+    if (plan.sms == 0) {
+        SPMM_CUDA_TRY(cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, plan.dev));
+        if (plan.dev < 64) known[plan.dev].store(plan.sms, std::memory_order_relaxed);
+    }
+    const Choice c = choose(p, plan.sms);
+    plan.cg = c.cg;
+    plan.bq = c.bq;
+    plan.splits = c.splits;
+    if (c.splits > 1) plan.parts = arena.take<float>(p.P * p.Q * c.splits);
+    return SPMM_OK;
+}
+
+int run_product(const Product &p, const ProductPlan &plan, bool clear, bool probe, cudaStream_t s) {
+    if (!plan.launches) return SPMM_OK;
+    if (plan.skinny) return launch_skinny(p, clear, s);
+    const How how{clear, probe, plan.splits, plan.dev, plan.sms};
+    return p.f16 ? run<__half>(p, plan, how, s) : run<__nv_bfloat16>(p, plan, how, s);
 }
 
 }  // namespace spmm
