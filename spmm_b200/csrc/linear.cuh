@@ -187,7 +187,7 @@ int plan_product(const Product &p, bool probe, Arena &arena, ProductPlan &plan);
 // `clear`: the kernel sets *status to 0 first (the first product of a call); `probe`: SPMM_CFG_EXPIRE_FIRST_WAIT.
 int run_product(const Product &p, const ProductPlan &plan, bool clear, bool probe, cudaStream_t s);
 
-// The same for at most four rows per group on average (operands aligned, see skinny_fits).
+// The same for about one row per group (operands aligned, see skinny_fits).
 bool skinny_fits(const Product &p);
 int launch_skinny(const Product &p, bool clear, cudaStream_t s);
 

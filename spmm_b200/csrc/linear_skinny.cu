@@ -1,11 +1,12 @@
 // linear_skinny.cu -- products of a handful of rows: y[q][p] = sum_r A[p][r] B[q][r]
-// for one to four q per group, the single tokens of a decoding step.
+// for about one q per group, the single tokens of a decoding step.
 //
 // Every value of A (the weights) is used once per row, so the time is that of
 // reading A; what counts is many independent 16-byte loads from the first
 // microsecond on.  Plain loads and FMAs do that with less start-up than a ring
-// of bulk copies, barriers and tensor memory: 1 x 4096 x 4096 takes 7 us where
-// the tensor-core kernel needs 13.
+// of bulk copies, barriers and tensor memory: 1 x 4096 x 4096 takes 9.2 us with
+// the weights in HBM where the tensor-core kernel needs 12.5 (and 8 against 12
+// with them in L2); its floor is 5.1 us.
 //
 // r contiguous: KS of a CTA's 8 warps share 4 p and take 256 r each in turn, a
 // lane 8 of them (KS = 1 where there are warps enough without: sharing costs a
@@ -231,8 +232,15 @@ int run(const Product &p, bool clear, cudaStream_t s) {
 
 }  // namespace
 
+// Where this kernel is the faster one.  One group of 4096 x 4096, us here / on
+// the tensor cores: 1 row 9.2 / 12.5 (p contiguous) and 10.9 / 13.3 (r
+// contiguous), 2 rows 9.9 / 12.7 and 12.3 / 13.0, 3 rows 11.4 / 12.6 and 14.0 /
+// 13.4.  64 groups of 2048 x 1408: 64 rows 45 / 49 (and it gathers rows itself,
+// which saves a copy), 128 rows 65 / 60.  It takes four rows at a time, so many
+// rows in one group cost far more than on the tensor cores; hence at most 64.
 bool skinny_fits(const Product &p) {
-    if (p.red || p.Q > 4 * p.groups || p.b_r != 1) return false;
+    const int64_t most = !p.offsets ? (p.a_r == 1 ? 2 : 3) : p.groups < 64 ? p.groups : 64;
+    if (p.red || p.Q > most || p.b_r != 1) return false;
     return p.a_r == 1 ? p.R % 8 == 0 : p.P % 8 == 0;
 }
 

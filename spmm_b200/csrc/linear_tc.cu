@@ -11,7 +11,7 @@
 // 128 x 256 x 64 products.
 //
 // Persistent CTAs (or pairs); warp 0 loads 64-wide steps of r by TMA into a
-// ring of 128-byte-swizzled stages, warp 1 issues the MMAs, warps 4-7 bring
+// ring of 128-byte-swizzled stages, warp 1 issues the MMAs, warps 4-11 bring
 // the finished accumulator out of tensor memory while the next tile is summed
 // into the other one.  Either operand may be contiguous along r (K-major) or
 // along p / q (MN-major): only the TMA box and the descriptors differ, so
@@ -22,13 +22,17 @@
 // rows of the next group that a box brings along are zeroed in shared memory
 // before the MMA reads them (0 * NaN would not do).
 //
+// What bounds it: the MMAs (the tensor pipe is active 80 % of the time at 4096 x
+// 8192 x 2048 with silu), and over seconds the card's power limit: 8192 x 16384
+// x 4096 bf16 811 us alone and 814 us sustained (1,350 TFLOP/s, 96 % of the
+// library product measured beside it), 4096 x 8192 x 2048 111 us (1,236).
+//
 // Every wait is bounded; on expiry the CTA raises its abort flag and the
 // call's status word, drains its copies and MMAs, frees tensor memory and
 // returns.
 #include <cuda.h>
 
 #include <atomic>
-#include <cmath>
 
 #include "linear.cuh"
 #include "ptx.cuh"
@@ -39,7 +43,7 @@ namespace {
 constexpr int kR = 64;              // r per stage: 128 bytes
 constexpr int kP = 128;             // p per CTA
 constexpr int kChunk = kR * 128;    // bytes of 64 rows of 128 bytes
-constexpr int kThreads = 384;     // 4 warps of roles, 8 of the epilogue
+constexpr int kThreads = 384;       // 4 warps of roles, 8 of the epilogue
 constexpr int kEpiWarps = 8;
 // q tiles that one sweep over p covers: sixteen of one group's rows (8192 x 16384 x 4096: 811 us, with 8 833 us, as
 // the weights pass through L2 half as often), eight of ragged groups, whose weights change every few q tiles anyway
@@ -62,14 +66,14 @@ template <int CG, int BQ>
 struct Shape {
     static constexpr int kBRows = BQ / CG;                    // B rows of one CTA
     static constexpr int kStageBytes = kP * 128 + kBRows * 128;
-    static constexpr int kStages = CG == 2 ? 6 : BQ == 256 ? 4 : BQ == 128 ? 6 : 8;
+    static constexpr int kStages = CG == 2 || BQ == 128 ? 6 : 8;
     // Rows of a K-major B box.  Few rows come in boxes of 16: one token then costs 2 KB a stage, not 8.
     static constexpr int kBoxQ = BQ == 64 ? 16 : CG == 2 ? 128 : 64;
     static constexpr int kTmem = 2 * BQ;
     static constexpr int kTable = 2 * (SPMM_MAX_GROUPS + 2) * 4;
     static constexpr int kRing = kStages * kStageBytes, kOut = kEpiWarps * 2048;
     static constexpr int kSmem = 1024 + kRing + kOut + kTable + 512;
-    static_assert(BQ % 64 == 0 && kTmem >= 32 && kTmem <= 512, "accumulators");
+    static_assert(BQ % 64 == 0 && kTmem <= 512, "accumulators");
     static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -768,7 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                                 ((uint32_t)(kP * CG >> 4) << 24);
         const uint32_t a_adv = (a.a_kmajor ? 32 : 2048) >> 4, b_adv = (a.b_kmajor ? 32 : 2048) >> 4;
         // descriptors of the first stage; only their low words depend on the stage and on r
-        const uint64_t da0 = smem_desc(smem_u32(ring), a.a_kmajor), db0 = smem_desc(smem_u32(ring) + kP * 128, a.b_kmajor);
+        const uint64_t da0 = smem_desc(smem_u32(ring), a.a_kmajor);
+        const uint64_t db0 = smem_desc(smem_u32(ring) + kP * 128, a.b_kmajor);
         const uint32_t da_hi = (uint32_t)(da0 >> 32), db_hi = (uint32_t)(db0 >> 32);
         uint32_t da = (uint32_t)da0, db = (uint32_t)db0;
         auto mma = [&](uint32_t d, uint32_t idesc, int c, uint32_t accumulate) {

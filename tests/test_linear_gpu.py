@@ -279,6 +279,43 @@ def test_many_tiles(cuda, t, k, n):
     check_dense(normal(t, k), normal(k, n, scale=k ** -0.5), normal(n), normal(t, n), 'gelu_tanh')
 
 
+@pytest.mark.parametrize('t, k, n', [(70001, 64, 72), (3, 72, 70000), (5, 70000, 8)])
+def test_long_dimensions(cuda, t, k, n):
+    torch.manual_seed(t)
+    check_dense(normal(t, k), normal(k, n, scale=k ** -0.5), normal(n), None, 'silu')
+
+
+@pytest.mark.parametrize('t, k, n', [(70000, 32768, 16), (70000, 16, 32768)])
+def test_offsets_past_32_bits(cuda, t, k, n):
+    """x, or y and the slopes, of more than 2**31 values: the last rows against the same rows alone."""
+    torch.manual_seed(k)
+    x, w = torch.empty(t, k, device='cuda', dtype=BF).normal_(), normal(k, n, scale=k ** -0.5)
+    y, slope = S.dense_matmul(x, w, activation='silu', return_slope=True)
+    z = x[-70:].double() @ w.double()
+    want, d = act64(z, 'silu')
+    E = (k + 8) * STEP * (x[-70:].double().abs() @ w.double().abs())
+    close(y[-70:], want, 1.2 * E + 2.0 ** -20 * z.abs(), BF, 'y')
+    assert ((slope[-70:].double() / 16384 - d).abs() <= 2.0 ** -15 + 1.2 * E + 2.0 ** -20).all()
+    dx, dw, _ = S.dense_matmul_backward(y, x, w, None)
+    tail = S.dense_matmul_backward(y[-70:], x[-70:], w, None)[0]
+    bound = (n + 16) * STEP * (y[-70:].double().abs() @ w.double().abs().t())
+    close(dx[-70:], y[-70:].double() @ w.double().t(), bound, BF, 'dx')
+    close(tail, y[-70:].double() @ w.double().t(), bound, BF, 'dx of the tail')
+    assert torch.isfinite(dw).all()
+
+
+def test_one_group_takes_all_rows(cuda):
+    """The kernel for a handful of rows is chosen by their average; one group may still have them all."""
+    torch.manual_seed(8)
+    x, w = normal(31, 256), normal(32, 256, 136, scale=1 / 16)
+    for g in (0, 17, 31):
+        offsets = torch.zeros(33, dtype=torch.int32)
+        offsets[g + 1:] = 29
+        y = S.grouped_matmul(x, w, offsets.cuda(), activation='gelu')
+        ref = reference(x, w, group_of(offsets, 31), torch.arange(31, device='cuda'), None, 'gelu', None)
+        close(y, *ref['y'], BF, 'y')
+
+
 def test_many_ragged_groups(cuda):
     torch.manual_seed(11)
     G, k, n = 200, 192, 328
