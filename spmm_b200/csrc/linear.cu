@@ -165,6 +165,7 @@ __global__ void dbias_kernel(const float *part, const int32_t *offsets, int64_t 
     }
     if (c >= n) return;
     float v = 0.f;
+#pragma unroll 16
     for (int64_t t = first; t < last; ++t) v += part[t * n + c];
     out[g * out_g + c] = from_f32<T>(v);
 }

@@ -309,19 +309,35 @@ __global__ void __launch_bounds__(1024) route_place_kernel(spmm_route_args p, in
     int *before = wcount;              // choices of an expert in earlier chunks, until place() needs the room
     for (int e = threadIdx.x; e < experts; e += blockDim.x) base[e] = before[e] = 0;
     __syncthreads();
-    // several threads an expert, each every parts-th chunk: the loads' latency is what this costs
-    const int parts = (int)blockDim.x > experts ? blockDim.x / experts : 1;
-    for (int i = threadIdx.x; i < parts * experts; i += blockDim.x) {
-        const int e = i % experts;
-        int sum = 0, earlier = 0;
+    // Four experts a thread where their number allows, several threads an expert, each every parts-th chunk: what
+    // this costs is the loads' latency.
+    const int each = experts % 4 == 0 ? 4 : 1, columns = experts / each;
+    const int parts = (int)blockDim.x > columns ? blockDim.x / columns : 1;
+    for (int i = threadIdx.x; i < parts * columns; i += blockDim.x) {
+        const int e = i % columns * each;
+        int sum[4] = {}, earlier[4] = {};
 #pragma unroll 8
-        for (int c = i / experts; c < chunks; c += parts) {
-            const int v = __ldg(counts + (int64_t)c * experts + e);
-            earlier += c < (int)blockIdx.x ? v : 0;
-            sum += v;
+        for (int c = i / columns; c < chunks; c += parts) {
+            int v[4] = {};
+            const int *row = counts + (int64_t)c * experts + e;
+            if (each == 4) {
+                const int4 w = __ldg((const int4 *)row);
+                v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+            } else {
+                v[0] = __ldg(row);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                earlier[u] += c < (int)blockIdx.x ? v[u] : 0;
+                sum[u] += v[u];
+            }
         }
-        atomicAdd(base + e, sum);
-        atomicAdd(before + e, earlier);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < each) {
+                atomicAdd(base + e + u, sum[u]);
+                atomicAdd(before + e + u, earlier[u]);
+            }
     }
     __syncthreads();
     const int total = cta_exclusive(base, experts, tmp);

@@ -249,7 +249,8 @@ def test_grouped(cuda, lens, tail, k, n, dtype, act, w_t):
 
 @pytest.mark.parametrize('tokens, experts, top, k, n, masked', [
     (1, 4, 1, 64, 64, 0), (3, 8, 8, 40, 24, 1), (50, 16, 3, 136, 72, 5), (200, 64, 6, 256, 128, 0),
-    (600, 5, 2, 65, 130, 20), (2500, 9, 4, 328, 392, 77), (900, 64, 8, 192, 264, 0)])
+    (600, 5, 2, 65, 130, 20), (2500, 9, 4, 328, 392, 77), (900, 64, 8, 192, 264, 0),
+    (10, 64, 6, 136, 72, 2)])
 @pytest.mark.parametrize('w_t', [False, True])
 def test_grouped_gather(cuda, tokens, experts, top, k, n, masked, w_t):
     torch.manual_seed(tokens)
