@@ -47,6 +47,7 @@ __device__ __forceinline__ void copy_piece(const uint16_t *row, int64_t c, int64
 // I: 32-bit piece numbers where they suffice; two 64-bit divisions a piece took longer than moving it.
 template <typename I>
 __global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ Copies all) {
+    chained_start();
     const CopyJob &j = all.job[blockIdx.y];
     const I per = (I)(j.dst_ld / 8), block = (I)j.rows * per, items = block * (I)j.copies;
     for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < items; i += (I)gridDim.x * 256) {
@@ -77,10 +78,8 @@ int run_copies(const Copies &all, cudaStream_t s) {
         pieces = j.copies * j.rows * (j.dst_ld / 8) > pieces ? j.copies * j.rows * (j.dst_ld / 8) : pieces;
     }
     const dim3 grid((unsigned)(most < 148 * 32 ? most : 148 * 32), (unsigned)all.count);
-    if (pieces < INT32_MAX) copy_rows_kernel<uint32_t><<<grid, 256, 0, s>>>(all);
-    else copy_rows_kernel<int64_t><<<grid, 256, 0, s>>>(all);
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
+    return launch_chained(pieces < INT32_MAX ? copy_rows_kernel<uint32_t> : copy_rows_kernel<int64_t>, grid, 256, 0, s,
+                          1, all);
 }
 
 // ---- gradient of the activation and of the bias -------------------------------
@@ -95,6 +94,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, const int16_t *slope, T *dz,
                                                  int64_t dz_ld, float *part, T *dbias, const int32_t *offsets,
                                                  int64_t groups, int64_t rows, int64_t n) {
+    chained_start();
     __shared__ float sums[8][kDzCols];
     const RowTile t = find_row_tile(offsets, groups, rows, kDzRows, blockIdx.x);
     if (t.group > groups || (offsets && t.group == groups)) return;
@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, con
 template <typename T>
 __global__ void dbias_kernel(const float *part, const int32_t *offsets, int64_t rows, int64_t n, T *out,
                              int64_t out_g) {
+    chained_start();
     const int64_t g = blockIdx.y, c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     int64_t first = 0, last;
     if (offsets) {
@@ -176,6 +177,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(256) gather_sum_kernel(const float *src, int64_t rows, const int32_t *slots,
                                                          int64_t tokens, int64_t top, int64_t n, T *out,
                                                          int64_t out_ld) {
+    chained_start();
     const int64_t per = n / V, items = tokens * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
         const int64_t t = i / per, c = (i - t * per) * V;
@@ -215,10 +217,8 @@ int gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tok
     const bool vec = n % 4 == 0 && out_ld % 4 == 0 && (uintptr_t)out % 8 == 0;
     const int64_t blocks = ceil_div(tokens * (vec ? n / 4 : n), 256);
     const unsigned grid = (unsigned)(blocks < 148 * 64 ? blocks : 148 * 64);
-    if (vec) gather_sum_kernel<T, 4><<<grid, 256, 0, s>>>(src, rows, slots, tokens, top, n, out, out_ld);
-    else gather_sum_kernel<T, 1><<<grid, 256, 0, s>>>(src, rows, slots, tokens, top, n, out, out_ld);
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
+    return launch_chained(vec ? gather_sum_kernel<T, 4> : gather_sum_kernel<T, 1>, dim3(grid), 256, 0, s, 1, src, rows,
+                          slots, tokens, top, n, out, out_ld);
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -413,18 +413,13 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
         const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
         const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p->n, kDzCols));
         T *direct = one_tile ? (T *)p->dbias : nullptr;
-        if (vec)
-            dz_kernel<T, true><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct,
-                                                    p->offsets, p->groups, p->rows, p->n);
-        else
-            dz_kernel<T, false><<<grid, 256, 0, s>>>((const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct,
-                                                     p->offsets, p->groups, p->rows, p->n);
-        SPMM_PRODUCT_LAUNCHED();
+        SPMM_TRY(launch_chained(vec ? dz_kernel<T, true> : dz_kernel<T, false>, grid, 256, 0, s, 1, (const T *)p->dy,
+                                p->dy_ld, p->slope, dzp, dz.ld, part, direct, p->offsets, p->groups, p->rows, p->n));
     }
     if (p->dbias && p->n && !one_tile) {
-        dbias_kernel<T><<<dim3((unsigned)ceil_div(p->n, 128), (unsigned)p->groups), 128, 0, s>>>(
-            part, p->offsets, any ? p->rows : 0, p->n, (T *)p->dbias, p->dbias_g);
-        SPMM_PRODUCT_LAUNCHED();
+        const dim3 grid((unsigned)ceil_div(p->n, 128), (unsigned)p->groups);
+        SPMM_TRY(launch_chained(dbias_kernel<T>, grid, 128, 0, s, 1, part, p->offsets, any ? p->rows : 0, p->n,
+                                (T *)p->dbias, p->dbias_g));
     }
     SPMM_TRY(run_product(gx, px, true, probe, s));
     if (sums)

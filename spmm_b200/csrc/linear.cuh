@@ -43,6 +43,40 @@ __device__ __forceinline__ int64_t group_first(const int32_t *offsets, int64_t g
     return o < 0 ? 0 : o > total ? total : o;
 }
 
+// Chained launches.  Every kernel of these operators starts with chained_start():
+// its blocks may be launched as soon as the blocks of the kernel before it on
+// the stream have ended, set themselves up, and wait there until that kernel's
+// writes are visible; nothing in global memory is read or written before.  Every
+// thread waits, so that a kernel never ends before the one it follows.  Forward
+// and backward of 512 x 1536 x 2304, call after call: 66 -> 56 us.  (Letting the
+// next kernel in at the start of this one instead: 61 us; its blocks then sit on
+// the SMs that this one's last blocks want.)
+__device__ __forceinline__ void chained_start() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+int launch_chained(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t shared, cudaStream_t s, int cluster,
+                   Args &&...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, Params(args)...) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return SPMM_ECUDA;
+    }
+    note_product_launch();
+    return SPMM_OK;
+}
+
 // A tile of up to `size` consecutive rows of one group; group == groups is the
 // tail of rows behind the last group, group > groups no tile.
 struct RowTile {

@@ -131,6 +131,7 @@ __device__ __forceinline__ void rows_rmajor(const Product &p, int64_t g, int64_t
 
 template <typename T, typename O, int KS>
 __global__ void __launch_bounds__(256) skinny_rmajor_kernel(const __grid_constant__ Product p, int clear) {
+    chained_start();
     __shared__ float sm[8 * kNP * 4];
     if (clear && p.status && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = 0;
     const int64_t g = blockIdx.y;
@@ -195,6 +196,7 @@ __device__ __forceinline__ void rows_pmajor(const Product &p, int64_t g, int64_t
 
 template <typename T, typename O, int WP>
 __global__ void __launch_bounds__(kWarps * 32) skinny_pmajor_kernel(const __grid_constant__ Product p, int clear) {
+    chained_start();
     __shared__ float sm[kWarps * 4 * WP];
     if (clear && p.status && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = 0;
     const int64_t g = blockIdx.y, p0 = (int64_t)blockIdx.x * WP;
@@ -212,22 +214,23 @@ __global__ void __launch_bounds__(kWarps * 32) skinny_pmajor_kernel(const __grid
 template <typename T, typename O>
 int run(const Product &p, bool clear, cudaStream_t s) {
     const unsigned gy = (unsigned)(p.offsets ? p.groups + 1 : 1);
+    const int64_t busy = p.Q < p.groups ? p.Q : p.groups;      // groups with rows, at most
     if (p.a_r == 1) {
         // warps of the whole call without sharing: 148 SMs hold about 4,700 at once
-        const int64_t quads = ceil_div(p.P, kNP), warps = quads * (p.Q < p.groups ? p.Q : p.groups);
+        const int64_t quads = ceil_div(p.P, kNP), warps = quads * busy;
         if (warps >= 4096 || p.R <= 256)
-            skinny_rmajor_kernel<T, O, 1><<<dim3((unsigned)ceil_div(quads, 8), gy), 256, 0, s>>>(p, clear);
-        else if (warps >= 2048 || p.R <= 512)
-            skinny_rmajor_kernel<T, O, 2><<<dim3((unsigned)ceil_div(quads, 4), gy), 256, 0, s>>>(p, clear);
-        else
-            skinny_rmajor_kernel<T, O, 8><<<dim3((unsigned)quads, gy), 256, 0, s>>>(p, clear);
-    } else if (ceil_div(p.P, 64) * (p.Q < p.groups ? p.Q : p.groups) >= 148 * 2) {
-        skinny_pmajor_kernel<T, O, 64><<<dim3((unsigned)ceil_div(p.P, 64), gy), kWarps * 32, 0, s>>>(p, clear);
-    } else {
-        skinny_pmajor_kernel<T, O, 32><<<dim3((unsigned)ceil_div(p.P, 32), gy), kWarps * 32, 0, s>>>(p, clear);
+            return launch_chained(skinny_rmajor_kernel<T, O, 1>, dim3((unsigned)ceil_div(quads, 8), gy), 256, 0, s, 1, p,
+                                  clear);
+        if (warps >= 2048 || p.R <= 512)
+            return launch_chained(skinny_rmajor_kernel<T, O, 2>, dim3((unsigned)ceil_div(quads, 4), gy), 256, 0, s, 1, p,
+                                  clear);
+        return launch_chained(skinny_rmajor_kernel<T, O, 8>, dim3((unsigned)quads, gy), 256, 0, s, 1, p, clear);
     }
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
+    if (ceil_div(p.P, 64) * busy >= 148 * 2)
+        return launch_chained(skinny_pmajor_kernel<T, O, 64>, dim3((unsigned)ceil_div(p.P, 64), gy), kWarps * 32, 0, s, 1,
+                              p, clear);
+    return launch_chained(skinny_pmajor_kernel<T, O, 32>, dim3((unsigned)ceil_div(p.P, 32), gy), kWarps * 32, 0, s, 1, p,
+                          clear);
 }
 
 }  // namespace

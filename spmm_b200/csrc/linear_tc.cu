@@ -716,9 +716,11 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         mbar_init(&s.never, 1);
         s.abort = 0;
         fence_mbar_init();
-        if (a.clear_status && blockIdx.x == 0 && p.status) *p.status = 0;
     }
     if (warp == 2) alloc_tmem<CG>(&s.tmem, Sh::kTmem);
+    __syncwarp();
+    chained_start();
+    if (a.clear_status && threadIdx.x == 0 && blockIdx.x == 0 && p.status) *p.status = 0;
     const uint32_t full = smem_u32(s.full), empty = smem_u32(s.empty), tail = smem_u32(s.tail), peer = smem_u32(s.peer);
     const uint32_t acc_full = smem_u32(s.acc_full), acc_empty = smem_u32(s.acc_empty);
     Loader<CG, BQ> load{maps, a, full, CG == 2 ? map_cta(full, lead) : full, tail, smem_u32(ring), rank};
@@ -964,6 +966,7 @@ Choice choose(const Product &p, int sms) {
 // Partial results of a split sum: C = finish(sum over parts, in order).  Eight p a thread.
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Product p, const float *parts, int splits) {
+    chained_start();
     constexpr int V = VEC ? 8 : 1;
     const int64_t per = p.P / V, items = p.Q * per;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -1009,8 +1012,8 @@ int join(const Product &p, const float *parts, int splits, cudaStream_t s) {
     const unsigned grid = (unsigned)ceil_div(p.Q * (vec ? p.P / 8 : p.P), 256);
 #define SPMM_JOIN(ACT)                                                                       \
     do {                                                                                     \
-        if (vec) join_kernel<T, ACT, true><<<grid, 256, 0, s>>>(p, parts, splits);           \
-        else join_kernel<T, ACT, false><<<grid, 256, 0, s>>>(p, parts, splits);              \
+        SPMM_TRY(launch_chained(vec ? join_kernel<T, ACT, true> : join_kernel<T, ACT, false>, dim3(grid), 256, 0, s, \
+                                1, p, parts, splits));                                       \
     } while (0)
     switch (p.act) {
         case SPMM_ACT_NONE: SPMM_JOIN(SPMM_ACT_NONE); break;
@@ -1020,7 +1023,6 @@ int join(const Product &p, const float *parts, int splits, cudaStream_t s) {
         default: SPMM_JOIN(SPMM_ACT_SILU); break;
     }
 #undef SPMM_JOIN
-    SPMM_PRODUCT_LAUNCHED();
     return SPMM_OK;
 }
 
@@ -1069,23 +1071,7 @@ int launch(const Product &p, const How &how, cudaStream_t s) {
         SPMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem));
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * CG));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Sh::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = CG > 1 ? 1 : 0;
-    if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return SPMM_ECUDA;
-    }
-    note_product_launch();
-    return SPMM_OK;
+    return launch_chained(kernel, dim3((unsigned)(tiles * CG)), kThreads, Sh::kSmem, s, CG, maps, a);
 }
 
 template <typename T, typename O>

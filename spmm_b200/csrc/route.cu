@@ -272,6 +272,7 @@ __device__ __forceinline__ void place(const spmm_route_args &p, int64_t i0, int6
 // Everything in one CTA: for few tokens, where launches are what it costs.
 template <typename T, int V, bool PACKED>
 __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_route_args p) {
+    chained_start();
     extern __shared__ int sm[];
     __shared__ int tmp[33];
     const int experts = (int)p.experts;
@@ -290,6 +291,7 @@ __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_small_kernel(spmm_r
 
 template <typename T, int V, bool PACKED>
 __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_choose_kernel(spmm_route_args p, int64_t chunk, int *counts) {
+    chained_start();
     extern __shared__ int sm[];
     const int experts = (int)p.experts;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) sm[e] = 0;
@@ -302,6 +304,7 @@ __global__ void __launch_bounds__(V <= 8 ? 1024 : 512) route_choose_kernel(spmm_
 
 __global__ void __launch_bounds__(1024) route_place_kernel(spmm_route_args p, int64_t chunk, const int *counts,
                                                            int chunks) {
+    chained_start();
     extern __shared__ int sm[];
     __shared__ int tmp[33];
     const int experts = (int)p.experts;
@@ -361,6 +364,7 @@ __global__ void __launch_bounds__(1024) route_place_kernel(spmm_route_args p, in
 //   sigmoid:                      dl = ds s (1 - s)
 template <typename T, int V>
 __global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(spmm_route_args p) {
+    chained_start();
     const int lane = threadIdx.x & 31;
     const int experts = (int)p.experts, top = (int)p.top;
     const int64_t step = (int64_t)gridDim.x * kWarps;
@@ -472,6 +476,7 @@ __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC]) {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256, 3) combine_kernel(const __grid_constant__ spmm_combine_args p, int parts,
                                                          int part_cols) {
+    chained_start();
     const int lane = threadIdx.x & 31, top = (int)p.top;
     const int64_t items = p.tokens * parts, step = (int64_t)gridDim.x * 8;
     for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < items; i += step) {
@@ -545,6 +550,7 @@ __global__ void __launch_bounds__(256, 3) combine_kernel(const __grid_constant__
 // of y, with eight sums in registers.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const __grid_constant__ spmm_combine_args p) {
+    chained_start();
     const int lane = threadIdx.x & 31, top = (int)p.top;
     const int64_t step = (int64_t)gridDim.x * 8;
     const int64_t w0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -650,27 +656,22 @@ int run_route(const spmm_route_args &p, cudaStream_t s) {
     if (small_route(&p)) {
         const int fit = warps_for(p.experts, most);
         const int warps = (int)(p.tokens < 1 ? 1 : p.tokens < fit ? p.tokens : fit);
-        route_small_kernel<T, V, PACKED><<<1, warps * 32, (warps + 1) * e4, s>>>(p);
-        SPMM_PRODUCT_LAUNCHED();
-        return SPMM_OK;
+        return launch_chained(route_small_kernel<T, V, PACKED>, dim3(1), warps * 32, (warps + 1) * e4, s, 1, p);
     }
     const int64_t chunk = chunk_tokens(&p), chunks = ceil_div(p.tokens, chunk);
     int *counts = (int *)p.workspace;
     const int choose = (int)(chunk < most ? chunk : most), place = warps_for(p.experts, 32);
-    route_choose_kernel<T, V, PACKED><<<(unsigned)chunks, choose * 32, e4, s>>>(p, chunk, counts);
-    SPMM_PRODUCT_LAUNCHED();
-    route_place_kernel<<<(unsigned)chunks, place * 32, (place + 1) * e4, s>>>(p, chunk, counts, (int)chunks);
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
+    SPMM_TRY(launch_chained(route_choose_kernel<T, V, PACKED>, dim3((unsigned)chunks), choose * 32, e4, s, 1, p, chunk,
+                            counts));
+    return launch_chained(route_place_kernel, dim3((unsigned)chunks), place * 32, (place + 1) * e4, s, 1, p, chunk, counts,
+                          (int)chunks);
 }
 
 template <typename T, int V>
 int run_route_backward(const spmm_route_args &p, cudaStream_t s) {
     int64_t grid = ceil_div(p.tokens, kWarps);
     if (grid > 148 * 8) grid = 148 * 8;
-    route_backward_kernel<T, V><<<(unsigned)grid, kWarps * 32, 0, s>>>(p);
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
+    return launch_chained(route_backward_kernel<T, V>, dim3((unsigned)grid), kWarps * 32, 0, s, 1, p);
 }
 
 template <typename T>
@@ -719,9 +720,10 @@ int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
     if (backward) {
         int64_t grid = ceil_div(p.tokens > 0 ? p.tokens : 1, 8);
         if (grid > 148 * 8) grid = 148 * 8;
-        if (vec) combine_backward_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p);
-        else combine_backward_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
-    } else {
+        return launch_chained(vec ? combine_backward_kernel<T, W> : combine_backward_kernel<T, 1>, dim3((unsigned)grid),
+                              256, 0, s, 1, p);
+    }
+    {
         const int64_t wide = vec ? 32 * W : 32, chunks = ceil_div(p.n, wide);
         if (p.n > INT32_MAX - 1024) return SPMM_EUNSUPPORTED;
         int64_t parts = ceil_div(148 * 24, p.tokens);          // 24 warps an SM are resident
@@ -730,11 +732,9 @@ int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
         parts = ceil_div(p.n, cols);
         int64_t grid = ceil_div(p.tokens * parts, 8);
         if (grid > 148 * 12) grid = 148 * 12;
-        if (vec) combine_kernel<T, W><<<(unsigned)grid, 256, 0, s>>>(p, (int)parts, (int)cols);
-        else combine_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p, (int)parts, (int)cols);
+        return launch_chained(vec ? combine_kernel<T, W> : combine_kernel<T, 1>, dim3((unsigned)grid), 256, 0, s, 1, p,
+                              (int)parts, (int)cols);
     }
-    SPMM_PRODUCT_LAUNCHED();
-    return SPMM_OK;
 }
 
 }  // namespace
