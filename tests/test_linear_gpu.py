@@ -407,6 +407,66 @@ def test_autograd_matches_the_plain_calls(cuda):
         assert not S.dense_matmul(*leaves).requires_grad
 
 
+def test_single_gradients(cuda):
+    """One input at a time asks for a gradient, dense and grouped, with and without an activation."""
+    torch.manual_seed(6)
+    x, w, b, r, dy = normal(70, 40), normal(40, 24), normal(24), normal(70, 24), normal(70, 24)
+    offsets = torch.tensor([0, 30, 30, 70], dtype=torch.int32, device='cuda')
+    wg, bg = normal(3, 40, 24), normal(3, 24)
+    for act in ('none', 'silu'):
+        _, slope = S.dense_matmul(x, w, b, r, activation=act, return_slope=True)
+        want = S.dense_matmul_backward(dy, x, w, slope, bias=True) + (dy,)
+        for i in range(4):
+            args = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, b, r))]
+            g, = torch.autograd.grad(S.dense_matmul(*args, activation=act), args[i], dy)
+            assert torch.equal(g, want[i]), (act, i)
+        _, slope = S.grouped_matmul(x, wg, offsets, bg, activation=act, return_slope=True)
+        want = S.grouped_matmul_backward(dy, x, wg, offsets, slope, bias=True)
+        for i in range(3):
+            args = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, wg, bg))]
+            y = S.grouped_matmul(args[0], args[1], offsets, args[2], activation=act)
+            g, = torch.autograd.grad(y, args[i], dy)
+            assert torch.equal(g, want[i]), (act, i)
+
+
+@pytest.mark.parametrize('tokens, masked', [(0, 0), (9, 9)])
+def test_no_rows_at_all(cuda, tokens, masked):
+    """No tokens, or none that any expert takes: zeros everywhere, the experts' gradients among them."""
+    logits = torch.randn(tokens, 6, device='cuda')
+    logits[tokens - masked:] = float('-inf')
+    weights, r = S.route_topk(logits, 2)
+    x, w, b = normal(tokens, 32), normal(6, 32, 24), normal(6, 24)
+    y, slope = S.grouped_matmul(x, w, r, b, activation='gelu', gather=True, return_slope=True)
+    assert y.shape == (2 * tokens, 24) and not y.any() and S.product_status(y) == 0
+    dx, dw, db = S.grouped_matmul_backward(normal(2 * tokens, 24), x, w, r, slope, gather=True, bias=True)
+    assert dx.shape == x.shape and not dx.any() and not dw.any() and not db.any()
+    out = S.route_combine(y, r, weights)
+    assert out.shape == (tokens, 24) and not out.any()
+
+
+def test_calls_from_two_threads(cuda):
+    import threading
+    torch.manual_seed(12)
+    x, w = normal(300, 512), normal(512, 640)
+    want = S.dense_matmul(x, w, activation='silu')
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                y = S.dense_matmul(x, w, activation='silu')
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want):
+                    bad.append(1)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_streams_and_graphs(cuda):
     torch.manual_seed(4)
     lens = [70, 0, 3, 129]
@@ -450,6 +510,32 @@ def test_streams_and_graphs(cuda):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(want, outs[0]))
+
+
+def test_capture_while_an_eager_graph_lives(cuda):
+    """The plain calls build no autograd graph: captured with leaves that an eager graph still holds."""
+    torch.manual_seed(13)
+    leaves = [t.requires_grad_() for t in (normal(64, 48), normal(48, 80), normal(80))]
+    eager = S.dense_matmul(*leaves, activation='gelu')
+    dy = normal(64, 80)
+
+    def step():
+        y, slope = S.dense_matmul(*leaves, activation='gelu', return_slope=True)
+        assert not y.requires_grad
+        return (y,) + S.dense_matmul_backward(dy, leaves[0], leaves[1], slope, bias=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    eager.backward(dy)
+    assert torch.equal(got[0], eager.detach())
+    assert all(torch.equal(a, t.grad) for a, t in zip(got[1:], leaves))
 
 
 def test_expert_layer(cuda):

@@ -108,6 +108,8 @@ def test_weights_and_gradients(cuda, scoring, renormalize, T):
     check(torch.randn(T, 96, device='cuda') * 3, 5, scoring, renormalize, 2.5,
           torch.randn(96, device='cuda'))
     check((torch.randn(T, 70, device='cuda') * 3).to(BF), 7, scoring, renormalize)
+    check((torch.randn(T, 90, device='cuda') * 3).to(HF), 5, scoring, renormalize, 0.5,
+          torch.randn(90, device='cuda') * 2)
 
 
 @pytest.mark.parametrize('scoring', S.SCORINGS)
