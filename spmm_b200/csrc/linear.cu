@@ -148,27 +148,39 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, con
     }
 }
 
-// dbias[g] = sum of group g's tiles, in order.
+// dbias[g] = sum of group g's tiles: 32 columns a CTA, each of its 8 warps every
+// eighth tile, the warps' sums added in order.
 template <typename T>
-__global__ void dbias_kernel(const float *part, const int32_t *offsets, int64_t rows, int64_t n, T *out,
-                             int64_t out_g) {
+__global__ void __launch_bounds__(256) dbias_kernel(const float *part, const int32_t *offsets, int64_t rows, int64_t n,
+                                                    T *out, int64_t out_g) {
     chained_start();
-    const int64_t g = blockIdx.y, c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    int64_t first = 0, last;
+    __shared__ float sums[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t g = blockIdx.y, c = (int64_t)blockIdx.x * 32 + lane;
+    auto tiles_of = [&](int64_t e) {
+        const int64_t a = group_first(offsets, e, rows), b = group_first(offsets, e + 1, rows);
+        return b > a ? (b - a + kDzRows - 1) / kDzRows : 0;
+    };
+    int64_t first = 0, count = (rows + kDzRows - 1) / kDzRows;
     if (offsets) {
-        for (int64_t e = 0; e <= g; ++e) {
-            const int64_t a = group_first(offsets, e, rows), b = group_first(offsets, e + 1, rows);
-            const int64_t tiles = b > a ? (b - a + kDzRows - 1) / kDzRows : 0;
-            if (e < g) first += tiles; else last = first + tiles;
-        }
-    } else {
-        last = (rows + kDzRows - 1) / kDzRows;
+        for (int64_t e = lane; e < g; e += 32) first += tiles_of(e);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) first += __shfl_xor_sync(kFullMask, first, o);
+        count = tiles_of(g);
     }
-    if (c >= n) return;
     float v = 0.f;
-#pragma unroll 16
-    for (int64_t t = first; t < last; ++t) v += part[t * n + c];
-    out[g * out_g + c] = from_f32<T>(v);
+    if (c < n) {
+#pragma unroll 8
+        for (int64_t t = warp; t < count; t += 8) v += part[(first + t) * n + c];
+    }
+    sums[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && c < n) {
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += sums[w][lane];
+        out[g * out_g + c] = from_f32<T>(v);
+    }
 }
 
 // out[t] = sum_j src[slots[t][j]], in order of j: V values a thread, the rows of
@@ -417,8 +429,8 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
                                 p->dy_ld, p->slope, dzp, dz.ld, part, direct, p->offsets, p->groups, p->rows, p->n));
     }
     if (p->dbias && p->n && !one_tile) {
-        const dim3 grid((unsigned)ceil_div(p->n, 128), (unsigned)p->groups);
-        SPMM_TRY(launch_chained(dbias_kernel<T>, grid, 128, 0, s, 1, part, p->offsets, any ? p->rows : 0, p->n,
+        const dim3 grid((unsigned)ceil_div(p->n, 32), (unsigned)p->groups);
+        SPMM_TRY(launch_chained(dbias_kernel<T>, grid, 256, 0, s, 1, part, p->offsets, any ? p->rows : 0, p->n,
                                 (T *)p->dbias, p->dbias_g));
     }
     SPMM_TRY(run_product(gx, px, true, probe, s));
