@@ -89,7 +89,10 @@ constexpr int kDzCols = 256;   // columns of a CTA: 32 lanes of 8
 
 // dz = dy * act'(z) (rounded to the operands' type) and the tile's column sums
 // of the unrounded products.  A warp takes a row at a time, a lane 16 bytes of
-// it; bound by reading dy and the slopes and writing dz once.
+// it; bound by reading dy and the slopes and writing dz once.  Where dz is
+// written, dy and the slopes are not read again: they are loaded as a stream,
+// so that the cache keeps dz for the products (4096 x 8192: 47.5 -> 43.3 us;
+// tiles of 32 rows, before the streamed loads, took 50 us against 47.5).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, const int16_t *slope, T *dz,
                                                  int64_t dz_ld, float *part, T *dbias, const int32_t *offsets,
@@ -108,9 +111,10 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, con
             const int64_t r = t.first + i;
             float d[8];
             if constexpr (VEC) {
-                unpack8<T>(__ldg((const uint4 *)(dy + r * dy_ld + c0)), d);
+                const uint4 *from = (const uint4 *)(dy + r * dy_ld + c0);
+                unpack8<T>(slope ? __ldcs(from) : __ldg(from), d);
                 if (slope) {
-                    const uint4 v = __ldg((const uint4 *)(slope + r * n + c0));
+                    const uint4 v = __ldcs((const uint4 *)(slope + r * n + c0));
                     int16_t c[8];
                     memcpy(c, &v, 16);
 #pragma unroll
