@@ -451,7 +451,7 @@ int spmm_route_backward(const spmm_route_args *p, spmm_stream_t stream);
 /* Weighted sums back in token order: out[t] = sum_j weights[t][j] * y[slots[t][j]] + residual[t] (slots
  * outside [0, rows) are left out; sums in float32, one rounding).  backward: dy[slots[t][j]] =
  * weights[t][j] * dout[t] (rows behind offsets[experts] zero) and dweights[t][j] = <dout[t],
- * y[slots[t][j]]> (0 where there is no slot). */
+ * y[slots[t][j]]> (0 where there is no slot).  No two slots are alike. */
 typedef struct {
     int32_t version;            /* 1 */
     int32_t dtype;              /* enum spmm_dense_type: BF16, F16 or F32 */

@@ -33,6 +33,9 @@ class Routing:
     ``rows`` [T*k]: the token of each row of the grouped order, ascending within
     an expert; -1 behind the last expert's rows.
     ``offsets`` [E+1]: the first row of each expert, and the end of the last one.
+
+    ``route_topk`` makes one; in one of your own no row may have two choices
+    (two slots alike): the gradients give each row one choice's values.
     """
 
     experts: torch.Tensor
