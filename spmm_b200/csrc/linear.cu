@@ -87,6 +87,12 @@ int run_copies(const Copies &all, cudaStream_t s) {
 constexpr int kDzRows = 64;    // rows of a tile
 constexpr int kDzCols = 256;   // columns of a CTA: 32 lanes of 8
 
+// Where the sums of the tile that starts at row `first` of group g stand.  Group
+// [a, b) takes places from a / 64 + g on, the last at most b / 64 + g, which lies
+// before the next group's first; every place is below ceil(rows / 64) + groups
+// whatever the table holds, where a count of the tiles before would not be.
+__device__ __forceinline__ int64_t part_place(int64_t first, int64_t g) { return first / kDzRows + g; }
+
 // dz = dy * act'(z) (rounded to the operands' type) and the tile's column sums
 // of the unrounded products.  A warp takes a row at a time, a lane 16 bytes of
 // it; bound by reading dy and the slopes and writing dz once.  Where dz is
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, con
 #pragma unroll
         for (int w = 0; w < 8; ++w) v += sums[w][threadIdx.x];
         if (dbias) dbias[c] = from_f32<T>(v);       // the only tile of the only group
-        else part[(int64_t)blockIdx.x * n + c] = v;
+        else part[part_place(t.first, t.group) * n + c] = v;
     }
 }
 
@@ -161,16 +167,11 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float *part, const int
     __shared__ float sums[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t g = blockIdx.y, c = (int64_t)blockIdx.x * 32 + lane;
-    auto tiles_of = [&](int64_t e) {
-        const int64_t a = group_first(offsets, e, rows), b = group_first(offsets, e + 1, rows);
-        return b > a ? (b - a + kDzRows - 1) / kDzRows : 0;
-    };
     int64_t first = 0, count = (rows + kDzRows - 1) / kDzRows;
     if (offsets) {
-        for (int64_t e = lane; e < g; e += 32) first += tiles_of(e);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) first += __shfl_xor_sync(kFullMask, first, o);
-        count = tiles_of(g);
+        const int64_t a = group_first(offsets, g, rows), b = group_first(offsets, g + 1, rows);
+        first = part_place(a, g);
+        count = b > a ? (b - a + kDzRows - 1) / kDzRows : 0;
     }
     float v = 0.f;
     if (c < n) {

@@ -1,0 +1,80 @@
+"""Dense and grouped products at the edges of what their entries accept: wrong tables, scratch that ends where its
+size says, combinations that only the C entries take, far sizes, and what autograd keeps.
+
+Tolerances are those of test_linear_gpu.py: u = eps / 2 of the type for the one rounding of a result, and
+(K + 8) 2^-23 |x||w| for a float32 sum of K products.
+"""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import spmm_b200 as S
+from spmm_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+STEP = 2.0 ** -23
+
+
+def normal(*shape, dtype=BF, scale=1.0):
+    return (torch.randn(*shape, device='cuda') * scale).to(dtype)
+
+
+def int32(*values):
+    return torch.tensor(values, dtype=torch.int32, device='cuda')
+
+
+def linear(rows, k, n, groups=1, dtype=_lib.DENSE_BF16, **kw):
+    """A filled spmm_linear; tensors are given as tensors."""
+    a = _lib.Linear()
+    a.version, a.dtype, a.rows, a.x_rows, a.k, a.n, a.groups = 1, dtype, rows, rows, k, n, groups
+    a.x_ld = a.dx_ld = k
+    a.w_k = a.y_ld = a.dy_ld = a.residual_ld = a.bias_g = a.dbias_g = a.dw_k = n
+    a.w_n = a.dw_n = 1
+    a.w_g = a.dw_g = k * n
+    for name, v in kw.items():
+        setattr(a, name, v.data_ptr() if isinstance(v, torch.Tensor) else v)
+    return a
+
+
+def run(name, a, before=0, after=256):
+    """Runs a C entry with exactly its workspace, in the middle of a buffer of NaNs; returns the buffer and where in
+    it the workspace lay."""
+    L = _lib.lib()
+    need = getattr(L, name + '_workspace_size')(C.byref(a))
+    buf = torch.full((before + need + after,), 0xFF, dtype=torch.uint8, device='cuda')
+    buf[before:before + need] = 0
+    a.workspace, a.workspace_bytes = buf.data_ptr() + before, need
+    assert getattr(L, name)(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    return buf, before, before + need
+
+
+def test_decreasing_offsets_read_nothing_behind_the_workspace(cuda):
+    """offsets 0, R, 0, R, ...: every second group has all rows, far more tiles in all than rows alone would have."""
+    G, R, n = 300, 6400, 8
+    offsets = int32(*([0, R] * (G // 2 + 1))[:G + 1])
+    dy, dbias = normal(R, n), torch.empty(G, n, device='cuda', dtype=BF)
+    a = linear(R, 8, n, G, offsets=offsets, dy=dy, dbias=dbias)
+    # 15,000 tiles of 8 float32 before the last group: the guards reach further than that either way
+    buf, lo, hi = run('spmm_linear_backward', a, 1 << 20, 1 << 20)
+    assert torch.isfinite(dbias).all() and not dbias[1::2].any()
+    assert (buf[:lo] == 0xFF).all() and (buf[hi:] == 0xFF).all()
+
+
+def test_bias_gradients_of_groups_that_end_within_a_tile(cuda):
+    """Lengths around the tile of 64 rows, empty groups between them: each group's sum is its own."""
+    torch.manual_seed(1)
+    lens = [64, 0, 1, 63, 65, 0, 0, 128, 127, 129, 1, 1, 62, 64]
+    offsets = int32(0, *torch.tensor(lens).cumsum(0).tolist())
+    R, n = sum(lens) + 70, 136
+    x, w, dy = normal(R, 8), normal(len(lens), 8, n), normal(R, n)
+    db = S.grouped_matmul_backward(dy, x, w, offsets, bias=True)[2].double()
+    at = 0
+    for g, m in enumerate(lens):
+        rows = dy[at:at + m].double()
+        want, size = rows.sum(0), rows.abs().sum(0)
+        assert ((db[g] - want).abs() <= 2.0 ** -8 * want.abs() + (m + 8) * STEP * size * 1.01 + 2.0 ** -25).all(), g
+        at += m
