@@ -37,8 +37,10 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     return v;
 }
 
-// First row of group g (offsets clamped into [0, total], so a wrong table reads and writes nothing outside).
+// First row of group g (offsets clamped into [0, total], so a wrong table reads and writes nothing outside; the
+// first group starts at 0 whatever the table says, so that no row before it stays unwritten).
 __device__ __forceinline__ int64_t group_first(const int32_t *offsets, int64_t g, int64_t total) {
+    if (g == 0) return 0;
     const int64_t o = __ldg(offsets + g);
     return o < 0 ? 0 : o > total ? total : o;
 }

@@ -279,14 +279,25 @@ struct Table {
     int32_t *first, *qtiles;
 };
 
+// Where the offsets decrease, their running maximum stands in for them: groups that overlapped could have more
+// tiles together than 32 bits hold, and two of them would write the same rows.
 template <int BQ>
 __device__ __forceinline__ void fill_table(const Product &p, Table t) {
     if (!p.offsets) return;
     const int64_t total = p.red ? p.R : p.Q;
     const int G = (int)p.groups;
-    for (int g = threadIdx.x; g <= G; g += blockDim.x) t.first[g] = (int32_t)group_first(p.offsets, g, total);
+    bool falls = false;
+    for (int g = threadIdx.x; g <= G; g += blockDim.x) {
+        const int64_t a = group_first(p.offsets, g, total);
+        falls |= g < G && group_first(p.offsets, g + 1, total) < a;
+        t.first[g] = (int32_t)a;
+    }
     if (threadIdx.x == 0) t.first[G + 1] = (int32_t)total;
-    __syncthreads();
+    if (__syncthreads_or(falls)) {
+        if (threadIdx.x == 0)
+            for (int g = 1; g <= G; ++g) t.first[g] = t.first[g] > t.first[g - 1] ? t.first[g] : t.first[g - 1];
+        __syncthreads();
+    }
     if (p.red || threadIdx.x >= 32) return;
     const int lane = threadIdx.x;
     int before = 0;
@@ -295,7 +306,7 @@ __device__ __forceinline__ void fill_table(const Product &p, Table t) {
         int tiles = 0;
         if (g <= G) {
             const int64_t n = (int64_t)t.first[g + 1] - t.first[g];
-            tiles = n > 0 ? (int)((n + BQ - 1) / BQ) : 0;
+            tiles = (int)((n + BQ - 1) / BQ);
         }
         const int incl = [&] {
             int v = tiles;
@@ -343,7 +354,6 @@ __device__ __forceinline__ bool get_tile(const TcArgs &a, Table t, uint32_t i, T
         o.nq = (int)(Q - qt * BQ < BQ ? Q - qt * BQ : BQ);
         o.r0 = t.first[g];
         len = t.first[g + 1] - t.first[g];
-        if (len < 0) len = 0;
         o.last = len & (kR - 1);
     } else if (p.offsets) {
         const int G = (int)p.groups;

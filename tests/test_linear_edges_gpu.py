@@ -78,3 +78,19 @@ def test_bias_gradients_of_groups_that_end_within_a_tile(cuda):
         want, size = rows.sum(0), rows.abs().sum(0)
         assert ((db[g] - want).abs() <= 2.0 ** -8 * want.abs() + (m + 8) * STEP * size * 1.01 + 2.0 ** -25).all(), g
         at += m
+
+
+@pytest.mark.parametrize('table', [[0, 300, 100, 400, 250, 500], [0, 520, 0, 520, 0, 520], [400, 300, 200, 100, 0, 50],
+                                   [-7, 200, 900, 100, 1000, 300]])
+@pytest.mark.parametrize('n', [72, 640])
+def test_decreasing_offsets_count_as_their_running_maximum(cuda, table, n):
+    """On the tensor cores no two groups own the same row, whatever the table says; the first one starts at 0."""
+    torch.manual_seed(2)
+    R, k = 520, 136
+    x, w, dy = normal(R, k), normal(5, k, n, scale=k ** -0.5), normal(R, n)
+    wrong = int32(*table)
+    right = int32(0, *table[1:]).clamp(0, R).cummax(0).values.int()
+    assert torch.equal(S.grouped_matmul(x, w, wrong), S.grouped_matmul(x, w, right))
+    got, want = S.grouped_matmul_backward(dy, x, w, wrong), S.grouped_matmul_backward(dy, x, w, right)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert S.product_status(got[0]) == 0
