@@ -581,7 +581,7 @@ __device__ __forceinline__ void finish_columns(const TcArgs &a, const Tile &t, u
         store_columns<T, O, SPMM_ACT_NONE, false>(a, t, stage, p0, bias, v, c0, n);
     } else {
         switch (p.act) {
-            case SPMM_ACT_NONE: store_columns<T, O, SPMM_ACT_NONE, false>(a, t, stage, p0, bias, v, c0, n); break;
+            case SPMM_ACT_NONE: store_act<T, O, SPMM_ACT_NONE>(a, t, stage, p0, bias, v, c0, n); break;
             case SPMM_ACT_RELU: store_act<T, O, SPMM_ACT_RELU>(a, t, stage, p0, bias, v, c0, n); break;
             case SPMM_ACT_GELU: store_act<T, O, SPMM_ACT_GELU>(a, t, stage, p0, bias, v, c0, n); break;
             case SPMM_ACT_GELU_TANH: store_act<T, O, SPMM_ACT_GELU_TANH>(a, t, stage, p0, bias, v, c0, n); break;

@@ -36,6 +36,7 @@ def linear(rows, k, n, groups=1, dtype=_lib.DENSE_BF16, **kw):
     a.w_g = a.dw_g = k * n
     for name, v in kw.items():
         setattr(a, name, v.data_ptr() if isinstance(v, torch.Tensor) else v)
+    a.keep = kw            # the tensors live as long as the struct
     return a
 
 
@@ -94,3 +95,27 @@ def test_decreasing_offsets_count_as_their_running_maximum(cuda, table, n):
     got, want = S.grouped_matmul_backward(dy, x, w, wrong), S.grouped_matmul_backward(dy, x, w, right)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert S.product_status(got[0]) == 0
+
+
+@pytest.mark.parametrize('rows, k, n', [(1, 256, 136), (64, 8192, 136), (700, 64, 264), (3, 17, 9), (5, 0, 24)])
+@pytest.mark.parametrize('act', [0, 1])
+def test_slope_of_every_kernel(cuda, rows, k, n, act):
+    """A slope that is asked for is written whichever kernel the sizes choose, also where there is no activation."""
+    torch.manual_seed(3)
+    x, w = normal(rows, k), normal(k, n, scale=max(k, 1) ** -0.5)
+    y = torch.empty(rows, n, device='cuda', dtype=BF)
+    slope = torch.full((rows, n), 77, device='cuda', dtype=torch.int16)
+    run('spmm_linear_forward', linear(rows, k, n, x=x, w=w, y=y, slope=slope, activation=act))
+    z = x.double() @ w.double()
+    sure = z.abs() > (k + 8) * STEP * (x.double().abs() @ w.double().abs())
+    want = torch.full_like(slope, 16384) if act == 0 else torch.where(z > 0, 16384, 0).short()
+    assert torch.equal(slope[sure], want[sure]) if act else torch.equal(slope, want)
+
+
+def test_slope_of_rows_behind_the_last_group(cuda):
+    for R, end in ((300, 190), (40, 9)):
+        x, w = normal(R, 64), normal(2, 64, 72)
+        y = torch.empty(R, 72, device='cuda', dtype=BF)
+        slope = torch.full((R, 72), 77, device='cuda', dtype=torch.int16)
+        run('spmm_linear_forward', linear(R, 64, 72, 2, x=x, w=w, y=y, slope=slope, offsets=int32(0, 5, end)))
+        assert (slope[:end] == 16384).all() and not slope[end:].any() and not y[end:].any()
