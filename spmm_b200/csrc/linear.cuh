@@ -167,7 +167,7 @@ __device__ __forceinline__ float activate(float z, float &d) {
         const float y = z < -12.f ? 0.f : z * s;
         if constexpr (SLOPE)
             d = fabsf(z) > 12.f ? (z > 0.f ? 1.f : 0.f)
-                                : fmaf(y * (1.f - s), fmaf(0.21406859f, z2, 1.5957691216057308f), s);
+                                : fmaf(y * (1.f - s), fmaf(0.21406445f, z2, 1.5957691216057308f), s);
         return y;
     } else {
         d = 1.f;

@@ -119,3 +119,25 @@ def test_slope_of_rows_behind_the_last_group(cuda):
         slope = torch.full((R, 72), 77, device='cuda', dtype=torch.int16)
         run('spmm_linear_forward', linear(R, 64, 72, 2, x=x, w=w, y=y, slope=slope, offsets=int32(0, 5, end)))
         assert (slope[:end] == 16384).all() and not slope[end:].any() and not y[end:].any()
+
+
+def points(lo, hi):
+    """z = x + bias exactly: x in steps of 2^-10 (float16 has them up to 2, then 2^-9), bias in steps of 2^-16."""
+    x = torch.arange(int(lo * 1024), int(hi * 1024) + 1, device='cuda').double() / 1024
+    x = x.to(HF)[:, None]
+    bias = (torch.arange(64, device='cuda').double() / 65536).to(HF)
+    return x, bias, x.double() + bias.double()
+
+
+def test_derivative_of_tanh_gelu(cuda):
+    """The derivative's fixed point is half a unit off, 2^-15, and its float32 evaluation, with s the sigmoid of u =
+    1.6 z (1 + 0.045 z^2), q = 1.6 + 0.21 z^2 and d = s + z s (1 - s) q: u |u| 5 2^-24 off, the hardware's exponential
+    and reciprocal 2^-22 and 2^-23 of theirs, so s at most 1.3e-6 s; d changes by 1 + z q (1 - 2 s) times that and
+    four roundings of its second term: below 3e-7 for all z in [-2.2, -1]."""
+    x, bias, z = points(-2.2, -1.0)
+    w = torch.ones(1, 64, device='cuda', dtype=HF)
+    _, slope = S.dense_matmul(x, w, bias, activation='gelu_tanh', return_slope=True)
+    c = (2 / torch.pi) ** 0.5
+    t = torch.tanh(c * (z + 0.044715 * z ** 3))
+    want = 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+    assert ((slope.double() / 16384 - want).abs() <= 2.0 ** -15 + 3e-7).all()
