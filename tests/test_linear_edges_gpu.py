@@ -141,3 +141,15 @@ def test_derivative_of_tanh_gelu(cuda):
     t = torch.tanh(c * (z + 0.044715 * z ** 3))
     want = 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
     assert ((slope.double() / 16384 - want).abs() <= 2.0 ** -15 + 3e-7).all()
+
+
+def test_gelu_keeps_its_bits_far_from_zero(cuda):
+    """z erfc(-z / sqrt 2) / 2 for z in [-10, -1]: the exponent z^2 / 2 is two roundings and a constant off, 2.5 2^-24
+    of it, so 7.5e-6 at z = -10; the exponential 2^-22, the polynomial 4e-7, its argument 2^-23, three products 2^-24:
+    below 1.1e-5 before the rounding to bfloat16."""
+    x = torch.arange(-10 * 32, -31, device='cuda').double().div(32).to(BF)[:, None]
+    bias = (torch.arange(64, device='cuda').double() / 65536).to(BF)
+    z = x.double() + bias.double()
+    y = S.dense_matmul(x, torch.ones(1, 64, device='cuda', dtype=BF), bias, activation='gelu')
+    want = 0.5 * z * torch.special.erfc(-z / 2 ** 0.5)
+    assert ((y.double() - want).abs() <= (2.0 ** -8 + 1.1e-5 * (1 + 2.0 ** -8)) * want.abs()).all()
