@@ -419,7 +419,8 @@ int spmm_linear_backward(const spmm_linear *p, spmm_stream_t stream);
 /* Expert choice.  Of each token's `experts` logits the `top` largest by float32(logit) + bias are chosen,
  * best first, ties to the lowest index; a -inf or NaN sum is never chosen (+inf counts as the largest
  * float).  Weights: softmax over all logits (-inf and NaN count as zero) or sigmoid, times `scale`, of the
- * chosen ones, divided by their sum with `renormalize`; 0 where nothing was left to choose (expert -1).
+ * chosen ones, divided by their sum with `renormalize`; 0 where nothing was left to choose (expert -1), and
+ * where a renormalised sigmoid's logit is below -709 (a mask by the type's lowest value).
  * The choices are then grouped by expert, tokens ascending: offsets[e] is the first position of expert e,
  * rows[p] the token at position p (-1 behind the last group), slots[t][j] the position of a choice (-1:
  * none).  experts <= 1024, top <= min(experts, SPMM_MAX_TOP), tokens * top < 2^31. */

@@ -80,7 +80,30 @@ __device__ __forceinline__ void load_row(const T *row, int experts, int lane, fl
     }
 }
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+// sigmoid(v); 1 - sigmoid(v) is sigmoid(-v).  The exponential is of -|v|, so that neither end loses its bits: 1 - s
+// is 0 in float32 from a logit of 17 on, and 1 / (1 + exp(-v)) is 0 below -88.
+__device__ __forceinline__ float sigmoid(float v) {
+    const float e = expf(-fabsf(v));
+    return (v > 0.f ? 1.f : e) / (1.f + e);
+}
+
+// A renormalised sigmoid counts as 0 below this logit, where 64 bits cannot hold 1 + exp(-v) either: what masks by
+// the type's lowest value leave.
+constexpr float kSigmoidZero = -709.78f;
+
+// sigmoid(mine) over the sum of the chosen lanes' sigmoids, in a whole warp.  Sigmoids are taken relative to
+// exp(min(largest logit, 0)), so that the sum is at least 1 / 2 and small ones keep their ratios.
+__device__ __forceinline__ float sigmoid_share(float mine, bool chosen) {
+    const bool live = chosen && mine > kSigmoidZero;
+    const uint32_t m = __reduce_max_sync(kFullMask, live ? order_key(mine) : 0u);
+    const float largest = __uint_as_float(m & 0x80000000u ? m & 0x7FFFFFFFu : ~m);
+    const float e = expf(-fabsf(mine));
+    const float s = !live ? 0.f : (mine > 0.f ? 1.f : expf(mine - fminf(largest, 0.f))) / (1.f + e);
+    float sum = s;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+    return sum > 0.f ? s / sum : 0.f;
+}
 
 // Descending, by Batcher's odd-even merge network.
 template <int V>
@@ -165,14 +188,10 @@ __device__ __forceinline__ void choose(const spmm_route_args &p, int64_t t, int 
             r = softmax_row<V>(l);
         }
         weight = expert >= 0 && r.total > 0.f ? expf(mine - r.peak) / r.total : 0.f;
+    } else if (p.renormalize) {
+        weight = sigmoid_share(mine, expert >= 0);
     } else {
         weight = expert >= 0 ? sigmoid(mine) : 0.f;
-        if (p.renormalize) {
-            float s = weight;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-            weight = s > 0.f ? weight / s : 0.f;
-        }
     }
     weight *= p.scale;
 }
@@ -361,7 +380,7 @@ __global__ void __launch_bounds__(1024) route_place_kernel(spmm_route_args p, in
 // dlogits, a warp per token.  With g = scale * dweights at the chosen experts and 0 elsewhere:
 //   renormalised, w = s / sum s:  ds = (g - <g, w>) / sum s at the chosen ones
 //   softmax over all:             dl = p (ds - <ds, p>);  renormalised, s = exp(l) of the chosen ones: w (g - <g, w>)
-//   sigmoid:                      dl = ds s (1 - s)
+//   sigmoid:                      dl = ds s (1 - s);  renormalised w (g - <g, w>) (1 - s)
 template <typename T, int V>
 __global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(spmm_route_args p) {
     chained_start();
@@ -397,24 +416,17 @@ __global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(spmm_route_
                 r = softmax_row<V>(x);
             }
             s = e >= 0 && r.total > 0.f ? expf(l - r.peak) / r.total : 0.f;
-        } else {
-            s = e >= 0 ? sigmoid(l) : 0.f;
+        } else {               // the weight
+            s = p.renormalize ? sigmoid_share(l, e >= 0) : e >= 0 ? sigmoid(l) : 0.f;
         }
-        float w = s;
-        if (p.renormalize && p.scoring == SPMM_SCORE_SIGMOID) {
-            float sum = s;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-            w = sum > 0.f ? s / sum : 0.f;
-        }
-        float dot = g * w;
+        float dot = g * s;
 #pragma unroll
         for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
         if (p.scoring == SPMM_SCORE_SOFTMAX) {
             d = s * (g - dot);
             all = p.renormalize ? 0.f : dot;
         } else {
-            d = p.renormalize ? w * (g - dot) * (1.f - s) : g * s * (1.f - s);
+            d = s * (p.renormalize ? g - dot : g) * sigmoid(-l);
         }
         if (all != 0.f) {      // softmax over all: experts that were not chosen have -p <g, p>
             float x[V];

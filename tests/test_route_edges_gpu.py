@@ -1,0 +1,56 @@
+"""Expert choice and combination at the edges: logits far from 0, routings of a caller's own, what autograd keeps.
+
+Tolerances as in test_route_gpu.py: a weight (k + 16 + |l|) 2^-23 relative, as exponents are differences off by 2^-24
+of the larger logit, a gradient (k + 32 + |l|) 2^-23 of its terms' size.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import spmm_b200 as S
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+INF = float('inf')
+STEP = 2.0 ** -23
+
+
+@pytest.mark.parametrize('renormalize', [True, False])
+@pytest.mark.parametrize('centers', [(20.0,), (17.0, -3.0), (-100.0,), (-100.0, -40.0), (-300.0,), (60.0, -95.0)])
+@pytest.mark.parametrize('T', [64, 300])
+def test_sigmoids_far_from_zero(cuda, renormalize, centers, T):
+    """The gradient is held relative to w sigmoid(-l), not to w: 1 - s keeps its bits; weights keep their ratios."""
+    torch.manual_seed(21)
+    E, k = 24, 5
+    l = torch.randn(T, E, device='cuda') * 2 + torch.tensor(centers, device='cuda')[torch.arange(E) % len(centers)]
+    bias = torch.randn(E, device='cuda') * 3
+    w, r = S.route_topk(l, k, scoring='sigmoid', renormalize=renormalize, bias=bias)
+    g = torch.randn(T, k, device='cuda')
+    dl = S.route_topk_backward(g, l, r, scoring='sigmoid', renormalize=renormalize)
+    at = r.experts.long()
+    lj = l.double().gather(1, at)
+    share = -torch.logaddexp(torch.zeros_like(lj), -lj)          # log sigmoid
+    rest = torch.exp(-torch.logaddexp(torch.zeros_like(lj), lj))  # 1 - sigmoid
+    want = torch.softmax(share, 1) if renormalize else torch.exp(share)
+    tol = (k + 16 + float(lj.abs().max())) * STEP
+    assert ((w.double() - want).abs() <= tol * want + 1e-37).all()
+    gd = g.double()
+    if renormalize:
+        grad = want * (gd - (gd * want).sum(1, keepdim=True)) * rest
+        size = 2 * want * gd.abs().amax(1, keepdim=True) * rest
+    else:
+        grad = want * gd * rest
+        size = grad.abs()
+    got = dl.double().gather(1, at)
+    assert ((got - grad).abs() <= (tol + 16 * STEP) * size + 1e-37).all()
+    assert int((dl != 0).sum()) <= T * k
+
+
+@pytest.mark.parametrize('dtype', [F32, BF, HF])
+def test_a_mask_by_the_lowest_value_has_no_share(cuda, dtype):
+    l = torch.randn(200, 16, device='cuda').to(dtype)
+    l[:, 2:] = torch.finfo(dtype).min
+    l[100:] = torch.finfo(dtype).min
+    w, r = S.route_topk(l, 4, scoring='sigmoid')
+    assert (w[:100, 2:] == 0).all() and ((w[:100].sum(1) - 1).abs() <= 4 * STEP).all() and not w[100:].any()
