@@ -155,6 +155,7 @@ class _MatMul(torch.autograd.Function):
         ctx.save_for_backward(x, w, slope)
         ctx.g = g
         ctx.mark_non_differentiable(status)
+        ctx.set_materialize_grads(False)      # or the status would come back as a tensor of zeros
         return y, status
 
     @staticmethod
@@ -163,7 +164,7 @@ class _MatMul(torch.autograd.Function):
         x, w, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
-        if need[0] or need[1] or need[2]:
+        if dy is not None and (need[0] or need[1] or need[2]):
             dx, dw, db = _backward(dy, x, w, ctx.g, slope, need[0], need[1], need[2])
         return dx, dw, db, dy if need[3] else None, None, None
 

@@ -138,12 +138,15 @@ class _TopK(torch.autograd.Function):
         ctx.save_for_backward(logits, out[1])
         ctx.how = (scoring, renormalize, scale)
         ctx.mark_non_differentiable(*out[1:])
+        ctx.set_materialize_grads(False)      # or the routing would come back as four tensors of zeros
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dweights, *_):
         logits, experts = ctx.saved_tensors
+        if dweights is None:
+            return (None,) * 6
         return _topk_backward(dweights, logits, experts, *ctx.how), None, None, None, None, None
 
 
@@ -229,6 +232,7 @@ class _Combine(torch.autograd.Function):
         ctx.save_for_backward(y, weights)
         ctx.routing = routing
         ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)
         return _combine(y, routing, weights, residual)
 
     @staticmethod
@@ -237,7 +241,7 @@ class _Combine(torch.autograd.Function):
         y, weights = ctx.saved_tensors
         need = ctx.needs_input_grad
         dy = dw = None
-        if need[0] or need[1]:
+        if dout is not None and (need[0] or need[1]):
             dy, dw = _combine_backward(dout, y, ctx.routing, weights, need[0], need[1])
         return dy, dw, dout if ctx.has_residual and need[2] else None, None
 

@@ -153,3 +153,18 @@ def test_gelu_keeps_its_bits_far_from_zero(cuda):
     y = S.dense_matmul(x, torch.ones(1, 64, device='cuda', dtype=BF), bias, activation='gelu')
     want = 0.5 * z * torch.special.erfc(-z / 2 ** 0.5)
     assert ((y.double() - want).abs() <= (2.0 ** -8 + 1.1e-5 * (1 + 2.0 ** -8)) * want.abs()).all()
+
+
+def allocations(call):
+    before = torch.cuda.memory_stats()['allocation.all.allocated']
+    call()
+    return torch.cuda.memory_stats()['allocation.all.allocated'] - before
+
+
+def test_autograd_allocates_what_the_plain_call_does(cuda):
+    x, w, b, dy = normal(64, 48), normal(48, 80), normal(80), normal(64, 80)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    _, slope = S.dense_matmul(x, w, b, activation='silu', return_slope=True)
+    plain = allocations(lambda: S.dense_matmul_backward(dy, x, w, slope, bias=True))
+    y = S.dense_matmul(*leaves, activation='silu')
+    assert allocations(lambda: torch.autograd.grad(y, leaves, dy)) == plain

@@ -54,3 +54,35 @@ def test_a_mask_by_the_lowest_value_has_no_share(cuda, dtype):
     l[100:] = torch.finfo(dtype).min
     w, r = S.route_topk(l, 4, scoring='sigmoid')
     assert (w[:100, 2:] == 0).all() and ((w[:100].sum(1) - 1).abs() <= 4 * STEP).all() and not w[100:].any()
+
+
+def test_autograd_allocates_what_the_plain_call_does(cuda):
+    l, g = torch.randn(300, 32, device='cuda', requires_grad=True), torch.randn(300, 4, device='cuda')
+    w, r = S.route_topk(l, 4)
+
+    def count(call):
+        before = torch.cuda.memory_stats()['allocation.all.allocated']
+        call()
+        return torch.cuda.memory_stats()['allocation.all.allocated'] - before
+    plain = count(lambda: S.route_topk_backward(g, l.detach(), r))
+    assert count(lambda: torch.autograd.grad(w, l, g)) == plain
+
+
+def test_gradients_that_never_come(cuda):
+    """A later function that gives no gradient at all: none goes on, and nothing is computed."""
+    class Stop(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return t.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+    l = torch.randn(40, 8, device='cuda', requires_grad=True)
+    x = torch.randn(40, 16, device='cuda').to(BF).requires_grad_()
+    w = torch.randn(16, 8, device='cuda').to(BF).requires_grad_()
+    y = torch.randn(80, 24, device='cuda').to(BF).requires_grad_()
+    weights, r = S.route_topk(l, 2)
+    (Stop.apply(weights).sum() + Stop.apply(S.dense_matmul(x, w)).sum()
+     + Stop.apply(S.route_combine(y, r, weights.detach())).sum()).backward()
+    assert all(t.grad is None for t in (l, x, w, y))
