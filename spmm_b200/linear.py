@@ -152,8 +152,9 @@ class _MatMul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, activation, g):
         y, slope, status = _forward(x, w, g, bias, residual, activation, True)
-        ctx.save_for_backward(x, w, slope)
-        ctx.g = g
+        # the grouping too, so that writing it again before the backward pass is an error
+        ctx.save_for_backward(x, w, slope, g.offsets, g.gather, g.slots)
+        ctx.counts = g.rows, g.count
         ctx.mark_non_differentiable(status)
         ctx.set_materialize_grads(False)      # or the status would come back as a tensor of zeros
         return y, status
@@ -161,11 +162,11 @@ class _MatMul(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _):
-        x, w, slope = ctx.saved_tensors
+        x, w, slope, *groups = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if dy is not None and (need[0] or need[1] or need[2]):
-            dx, dw, db = _backward(dy, x, w, ctx.g, slope, need[0], need[1], need[2])
+            dx, dw, db = _backward(dy, x, w, _Groups(*groups, *ctx.counts), slope, need[0], need[1], need[2])
         return dx, dw, db, dy if need[3] else None, None, None
 
 

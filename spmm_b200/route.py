@@ -212,14 +212,14 @@ def _combine(y, routing, weights, residual):
     return out
 
 
-def _combine_backward(dout, y, routing, weights, need_dy=True, need_dweights=True):
+def _combine_backward(dout, y, slots, offsets, weights, need_dy=True, need_dweights=True):
     y, dout, weights = _unit_rows(y), _unit_rows(dout), weights.contiguous()
-    slots, n = routing.slots, y.shape[1]
+    n = y.shape[1]
     with on_device(y.device):
         dy = y.new_empty(y.shape) if need_dy else None
         dw = weights.new_empty(weights.shape) if need_dweights else None
-        args = _COMBINE(1, _TYPES[y.dtype], *slots.shape, y.shape[0], n, routing.num_experts, slots.data_ptr(),
-                        routing.offsets.data_ptr(), weights.data_ptr(), y.data_ptr(), 0, 0, dout.data_ptr(),
+        args = _COMBINE(1, _TYPES[y.dtype], *slots.shape, y.shape[0], n, offsets.shape[0] - 1, slots.data_ptr(),
+                        offsets.data_ptr(), weights.data_ptr(), y.data_ptr(), 0, 0, dout.data_ptr(),
                         dy.data_ptr() if need_dy else 0, dw.data_ptr() if need_dweights else 0, y.stride(0), 0, 0,
                         dout.stride(0), n)
         _lib.check(_lib.lib().spmm_combine_backward(args, stream_handle(y.device)), 'route_combine_backward')
@@ -229,8 +229,8 @@ def _combine_backward(dout, y, routing, weights, need_dy=True, need_dweights=Tru
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, residual, routing):
-        ctx.save_for_backward(y, weights)
-        ctx.routing = routing
+        # the routing too, so that writing it again before the backward pass is an error
+        ctx.save_for_backward(y, weights, routing.slots, routing.offsets)
         ctx.has_residual = residual is not None
         ctx.set_materialize_grads(False)
         return _combine(y, routing, weights, residual)
@@ -238,11 +238,11 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        y, weights = ctx.saved_tensors
+        y, weights, slots, offsets = ctx.saved_tensors
         need = ctx.needs_input_grad
         dy = dw = None
         if dout is not None and (need[0] or need[1]):
-            dy, dw = _combine_backward(dout, y, ctx.routing, weights, need[0], need[1])
+            dy, dw = _combine_backward(dout, y, slots, offsets, weights, need[0], need[1])
         return dy, dw, dout if ctx.has_residual and need[2] else None, None
 
 
@@ -284,4 +284,4 @@ def route_combine_backward(dout: torch.Tensor, y: torch.Tensor, routing: Routing
     if dout.shape != (routing.tokens, y.shape[1]) or dout.dtype != y.dtype or dout.device != y.device:
         raise ValueError('dout must have the result\'s shape, type and device')
     need_cuda(y, 'y')
-    return _combine_backward(dout, y, routing, weights)
+    return _combine_backward(dout, y, routing.slots, routing.offsets, weights)

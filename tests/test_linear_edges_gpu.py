@@ -168,3 +168,18 @@ def test_autograd_allocates_what_the_plain_call_does(cuda):
     plain = allocations(lambda: S.dense_matmul_backward(dy, x, w, slope, bias=True))
     y = S.dense_matmul(*leaves, activation='silu')
     assert allocations(lambda: torch.autograd.grad(y, leaves, dy)) == plain
+
+
+@pytest.mark.parametrize('which', ['offsets', 'rows', 'slots'])
+def test_a_grouping_written_again_before_the_backward_pass(cuda, which):
+    _, r = S.route_topk(torch.randn(50, 8, device='cuda'), 2)
+    x, w = normal(50, 40).requires_grad_(), normal(8, 40, 24).requires_grad_()
+    y = S.grouped_matmul(x, w, r, gather=True)
+    getattr(r, which).zero_()
+    with pytest.raises(RuntimeError, match='inplace'):
+        y.sum().backward()
+    offsets = int32(0, 20, 50)
+    y = S.grouped_matmul(x, w[:2], offsets)
+    offsets += 1
+    with pytest.raises(RuntimeError, match='inplace'):
+        y.sum().backward()

@@ -86,3 +86,13 @@ def test_gradients_that_never_come(cuda):
     (Stop.apply(weights).sum() + Stop.apply(S.dense_matmul(x, w)).sum()
      + Stop.apply(S.route_combine(y, r, weights.detach())).sum()).backward()
     assert all(t.grad is None for t in (l, x, w, y))
+
+
+@pytest.mark.parametrize('which', ['slots', 'offsets'])
+def test_a_routing_written_again_before_the_backward_pass(cuda, which):
+    w, r = S.route_topk(torch.randn(50, 8, device='cuda'), 2)
+    y = torch.randn(100, 24, device='cuda').to(BF).requires_grad_()
+    out = S.route_combine(y, r, w)
+    getattr(r, which).zero_()
+    with pytest.raises(RuntimeError, match='inplace'):
+        out.sum().backward()
