@@ -18,10 +18,11 @@ import struct
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._device import on_device, stream_handle
-from .route import Routing, check_routing, need_cuda
+from .route import Routing, check_routing, need_cuda, refuse_tangents
 
 __all__ = ['dense_matmul', 'dense_matmul_backward', 'grouped_matmul', 'grouped_matmul_backward', 'ACTIVATIONS']
 
@@ -236,6 +237,8 @@ def dense_matmul(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] 
         _check_like('bias', bias, x, (w.shape[1],))
     if residual is not None:
         _check_like('residual', residual, x, shape)
+    if forward_ad._current_level >= 0:
+        refuse_tangents(x=x, w=w, bias=bias, residual=residual)
     need_cuda(x, 'x')
     if x.dim() == 2:
         return _run(x, w, _Groups(None, None, None, x.shape[0], 1), bias, residual, activation, return_slope)
@@ -268,6 +271,8 @@ def dense_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sl
     _check_like('dy', dy, x, shape)
     rows = _rows(x)
     _check_slope(slope, (rows, w.shape[1]), x)
+    if forward_ad._current_level >= 0:
+        refuse_tangents(dy=dy, x=x, w=w)
     need_cuda(x, 'x')
     g = _Groups(None, None, None, rows, 1)
     if x.dim() == 2:
@@ -327,6 +332,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, groups: Union[Routing, torc
     g = _groups(x, w, groups, gather)
     if bias is not None:
         _check_like('bias', bias, x, (w.shape[0], w.shape[2]))
+    if forward_ad._current_level >= 0:
+        refuse_tangents(x=x, w=w, bias=bias)
     need_cuda(x, 'x')
     return _run(x, w, g, bias, None, activation, return_slope)
 
@@ -345,5 +352,7 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     g = _groups(x, w, groups, gather)
     _check_like('dy', dy, x, (g.rows, w.shape[2]))
     _check_slope(slope, (g.rows, w.shape[2]), x)
+    if forward_ad._current_level >= 0:
+        refuse_tangents(dy=dy, x=x, w=w)
     need_cuda(x, 'x')
     return _backward(dy, x, w, g, slope, True, True, bias)

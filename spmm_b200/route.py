@@ -14,6 +14,7 @@ from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._device import on_device, stream_handle
@@ -73,6 +74,14 @@ def check_routing(r, device=None) -> None:
 def need_cuda(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise ValueError(f'{what} must be a dense CUDA tensor')
+
+
+def refuse_tangents(**tensors: Optional[torch.Tensor]) -> None:
+    """The operators are differentiable backwards only; without this a tangent would be lost silently.  Called where
+    forward_ad._current_level says that there can be one."""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f'{name} has a tangent: there are no forward-mode derivatives')
 
 
 def _check_score(logits, scoring):
@@ -173,6 +182,8 @@ def route_topk(logits: torch.Tensor, top: int, *, scoring: str = 'softmax', reno
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (experts,)
                              or bias.device != logits.device):
         raise ValueError(f'bias must be a float32 tensor of {experts} values on the logits\' device')
+    if forward_ad._current_level >= 0:
+        refuse_tangents(logits=logits)
     need_cuda(logits, 'logits')
     bias = None if bias is None else bias.detach().contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
@@ -191,6 +202,8 @@ def route_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, routing: R
         raise ValueError('routing does not belong to these logits')
     if dweights.shape != routing.slots.shape or dweights.dtype != torch.float32 or dweights.device != logits.device:
         raise ValueError('dweights must be float32, of the weights\' shape and on their device')
+    if forward_ad._current_level >= 0:
+        refuse_tangents(dweights=dweights, logits=logits)
     need_cuda(logits, 'logits')
     return _topk_backward(dweights, logits, routing.experts, scoring, renormalize, float(scale))
 
@@ -271,6 +284,8 @@ def route_combine(y: torch.Tensor, routing: Routing, weights: torch.Tensor,
     if residual is not None and (residual.shape != shape or residual.dtype != y.dtype
                                  or residual.device != y.device):
         raise ValueError(f'residual must be {shape} of y\'s type on its device')
+    if forward_ad._current_level >= 0:
+        refuse_tangents(y=y, weights=weights, residual=residual)
     need_cuda(y, 'y')
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, residual)):
         return _Combine.apply(y, weights, residual, routing)
@@ -283,5 +298,7 @@ def route_combine_backward(dout: torch.Tensor, y: torch.Tensor, routing: Routing
     _check_combine(y, routing, weights)
     if dout.shape != (routing.tokens, y.shape[1]) or dout.dtype != y.dtype or dout.device != y.device:
         raise ValueError('dout must have the result\'s shape, type and device')
+    if forward_ad._current_level >= 0:
+        refuse_tangents(dout=dout, y=y, weights=weights)
     need_cuda(y, 'y')
     return _combine_backward(dout, y, routing.slots, routing.offsets, weights)
