@@ -470,6 +470,10 @@ typedef struct {
 } spmm_combine_args;
 int spmm_combine(const spmm_combine_args *p, spmm_stream_t stream);
 int spmm_combine_backward(const spmm_combine_args *p, spmm_stream_t stream);
+/* The same where rows before offsets[experts] may have no slot (choices that were dropped): tokens_of [rows]
+ * is each row's token, as spmm_route writes `rows`; a row that no slot of its token names gets a zero dy.
+ * Without it (NULL, or spmm_combine_backward) every such row has a slot, or its dy is left as it was. */
+int spmm_combine_backward_rows(const spmm_combine_args *p, const int32_t *tokens_of, spmm_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -41,7 +41,8 @@ EXPORTS = ('spmm_status_string', 'spmm_abi_version', 'spmm_boo_build_workspace_s
            'spmm_boo_matmul_groups', 'spmm_boo_plan_size', 'spmm_boo_plan_workspace_size',
            'spmm_boo_plan_build', 'spmm_linear_forward_workspace_size', 'spmm_linear_forward',
            'spmm_linear_backward_workspace_size', 'spmm_linear_backward', 'spmm_route_workspace_size',
-           'spmm_route', 'spmm_route_backward', 'spmm_combine', 'spmm_combine_backward')
+           'spmm_route', 'spmm_route_backward', 'spmm_combine', 'spmm_combine_backward',
+           'spmm_combine_backward_rows')
 
 
 class CsrDev(C.Structure):
@@ -212,6 +213,8 @@ def lib() -> C.CDLL:
         for n in ('spmm_route', 'spmm_route_backward', 'spmm_combine', 'spmm_combine_backward'):
             getattr(L, n).argtypes = [C.c_void_p, C.c_void_p]       # a RouteArgs or CombineArgs, or its bytes
             getattr(L, n).restype = C.c_int
+        L.spmm_combine_backward_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.spmm_combine_backward_rows.restype = C.c_int
         for n in ('spmm_boo_build_analyze', 'spmm_boo_build_emit', 'spmm_pbr_build_analyze',
                   'spmm_pbr_build_emit', 'spmm_boo_matmul', 'spmm_pbr_matmul'):
             getattr(L, n).restype = C.c_int

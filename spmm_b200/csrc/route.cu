@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(256, 3) combine_kernel(const __grid_constant__
 // A warp per token: dout's row, read once per eight choices, against their rows
 // of y, with eight sums in registers.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const __grid_constant__ spmm_combine_args p) {
+__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const __grid_constant__ spmm_combine_args p,
+                                                                  const int32_t *tokens_of) {
     chained_start();
     const int lane = threadIdx.x & 31, top = (int)p.top;
     const int64_t step = (int64_t)gridDim.x * 8;
@@ -628,9 +629,19 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const __grid_c
             }
         }
     }
-    if (p.dy) {   // rows behind the last group
-        for (int64_t r = group_first(p.offsets, p.experts, p.rows) + w0; r < p.rows; r += step)
-            for (int64_t c = lane; c < p.n; c += 32) ((T *)p.dy)[r * p.dy_ld + c] = from_f32<T>(0.f);
+    if (p.dy == nullptr) return;
+    auto clear = [&](int64_t r) {
+        for (int64_t c = lane; c < p.n; c += 32) ((T *)p.dy)[r * p.dy_ld + c] = from_f32<T>(0.f);
+    };
+    const int64_t end = group_first(p.offsets, p.experts, p.rows);
+    for (int64_t r = end + w0; r < p.rows; r += step) clear(r);      // behind the last group
+    if (tokens_of == nullptr) return;
+    for (int64_t r0 = w0 * 32; r0 < end; r0 += step * 32) {          // rows that no choice has, a lane each
+        const int64_t r = r0 + lane, t = r < end ? __ldg(tokens_of + r) : -1;
+        bool named = r >= end;
+        if (t >= 0 && t < p.tokens)
+            for (int j = 0; j < top; ++j) named |= __ldg(p.slots + t * top + j) == r;
+        for (unsigned left = __ballot_sync(kFullMask, !named); left; left &= left - 1) clear(r0 + __ffs(left) - 1);
     }
 }
 
@@ -722,7 +733,7 @@ int check_combine(const spmm_combine_args *p) {
 bool aligned16(const void *p, int64_t ld, int64_t per) { return (uintptr_t)p % 16 == 0 && ld % per == 0; }
 
 template <typename T>
-int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
+int run_combine(const spmm_combine_args &p, bool backward, const int32_t *tokens_of, cudaStream_t s) {
     constexpr int W = 16 / sizeof(T);
     bool vec = p.n % W == 0 && aligned16(p.y, p.y_ld, W);
     if (backward)
@@ -733,7 +744,7 @@ int run_combine(const spmm_combine_args &p, bool backward, cudaStream_t s) {
         int64_t grid = ceil_div(p.tokens > 0 ? p.tokens : 1, 8);
         if (grid > 148 * 8) grid = 148 * 8;
         return launch_chained(vec ? combine_backward_kernel<T, W> : combine_backward_kernel<T, 1>, dim3((unsigned)grid),
-                              256, 0, s, 1, p);
+                              256, 0, s, 1, p, tokens_of);
     }
     {
         const int64_t wide = vec ? 32 * W : 32, chunks = ceil_div(p.n, wide);
@@ -775,21 +786,27 @@ extern "C" int spmm_route_backward(const spmm_route_args *p, spmm_stream_t strea
     return by_type(*p, true, (cudaStream_t)stream);
 }
 
+static int combine_by_type(const spmm_combine_args *p, bool backward, const int32_t *tokens_of, cudaStream_t s) {
+    if (p->dtype == SPMM_DENSE_F32) return run_combine<float>(*p, backward, tokens_of, s);
+    if (p->dtype == SPMM_DENSE_F16) return run_combine<__half>(*p, backward, tokens_of, s);
+    return run_combine<__nv_bfloat16>(*p, backward, tokens_of, s);
+}
+
 extern "C" int spmm_combine(const spmm_combine_args *p, spmm_stream_t stream) {
     SPMM_TRY(check_combine(p));
     if (p->tokens == 0 || p->n == 0) return SPMM_OK;
     if (!p->slots || !p->weights || !p->out || (p->rows && !p->y)) return SPMM_EINVAL;
-    if (p->dtype == SPMM_DENSE_F32) return run_combine<float>(*p, false, (cudaStream_t)stream);
-    if (p->dtype == SPMM_DENSE_F16) return run_combine<__half>(*p, false, (cudaStream_t)stream);
-    return run_combine<__nv_bfloat16>(*p, false, (cudaStream_t)stream);
+    return combine_by_type(p, false, nullptr, (cudaStream_t)stream);
 }
 
-extern "C" int spmm_combine_backward(const spmm_combine_args *p, spmm_stream_t stream) {
+extern "C" int spmm_combine_backward_rows(const spmm_combine_args *p, const int32_t *tokens_of, spmm_stream_t stream) {
     SPMM_TRY(check_combine(p));
     if (!p->dy && !p->dweights) return SPMM_OK;
     if (p->tokens && (!p->slots || !p->weights || (p->n && (!p->dout || (p->rows && !p->y))))) return SPMM_EINVAL;
     if (p->dy && (!p->offsets || p->experts < 0)) return SPMM_EINVAL;
-    if (p->dtype == SPMM_DENSE_F32) return run_combine<float>(*p, true, (cudaStream_t)stream);
-    if (p->dtype == SPMM_DENSE_F16) return run_combine<__half>(*p, true, (cudaStream_t)stream);
-    return run_combine<__nv_bfloat16>(*p, true, (cudaStream_t)stream);
+    return combine_by_type(p, true, tokens_of, (cudaStream_t)stream);
+}
+
+extern "C" int spmm_combine_backward(const spmm_combine_args *p, spmm_stream_t stream) {
+    return spmm_combine_backward_rows(p, nullptr, stream);
 }

@@ -36,7 +36,9 @@ class Routing:
     ``offsets`` [E+1]: the first row of each expert, and the end of the last one.
 
     ``route_topk`` makes one; in one of your own no row may have two choices
-    (two slots alike): the gradients give each row one choice's values.
+    (two slots alike): the gradients give each row one choice's values.  A
+    choice is dropped by a slot of -1: its row then adds nothing and gets no
+    gradient from ``route_combine``.
     """
 
     experts: torch.Tensor
@@ -225,7 +227,7 @@ def _combine(y, routing, weights, residual):
     return out
 
 
-def _combine_backward(dout, y, slots, offsets, weights, need_dy=True, need_dweights=True):
+def _combine_backward(dout, y, slots, offsets, rows, weights, need_dy=True, need_dweights=True):
     y, dout, weights = _unit_rows(y), _unit_rows(dout), weights.contiguous()
     n = y.shape[1]
     with on_device(y.device):
@@ -235,7 +237,7 @@ def _combine_backward(dout, y, slots, offsets, weights, need_dy=True, need_dweig
                         offsets.data_ptr(), weights.data_ptr(), y.data_ptr(), 0, 0, dout.data_ptr(),
                         dy.data_ptr() if need_dy else 0, dw.data_ptr() if need_dweights else 0, y.stride(0), 0, 0,
                         dout.stride(0), n)
-        _lib.check(_lib.lib().spmm_combine_backward(args, stream_handle(y.device)), 'route_combine_backward')
+        _lib.check(_lib.lib().spmm_combine_backward_rows(args, rows.data_ptr(), stream_handle(y.device)), 'route_combine_backward')
     return dy, dw
 
 
@@ -243,7 +245,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, residual, routing):
         # the routing too, so that writing it again before the backward pass is an error
-        ctx.save_for_backward(y, weights, routing.slots, routing.offsets)
+        ctx.save_for_backward(y, weights, routing.slots, routing.offsets, routing.rows)
         ctx.has_residual = residual is not None
         ctx.set_materialize_grads(False)
         return _combine(y, routing, weights, residual)
@@ -251,11 +253,11 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        y, weights, slots, offsets = ctx.saved_tensors
+        y, weights, *routing = ctx.saved_tensors
         need = ctx.needs_input_grad
         dy = dw = None
         if dout is not None and (need[0] or need[1]):
-            dy, dw = _combine_backward(dout, y, slots, offsets, weights, need[0], need[1])
+            dy, dw = _combine_backward(dout, y, *routing, weights, need[0], need[1])
         return dy, dw, dout if ctx.has_residual and need[2] else None, None
 
 
@@ -301,4 +303,4 @@ def route_combine_backward(dout: torch.Tensor, y: torch.Tensor, routing: Routing
     if forward_ad._current_level >= 0:
         refuse_tangents(dout=dout, y=y, weights=weights)
     need_cuda(y, 'y')
-    return _combine_backward(dout, y, routing.slots, routing.offsets, weights)
+    return _combine_backward(dout, y, routing.slots, routing.offsets, routing.rows, weights)

@@ -96,3 +96,27 @@ def test_a_routing_written_again_before_the_backward_pass(cuda, which):
     getattr(r, which).zero_()
     with pytest.raises(RuntimeError, match='inplace'):
         out.sum().backward()
+
+
+@pytest.mark.parametrize('T, E, k, n, dtype', [(1, 8, 2, 64, BF), (50, 8, 2, 77, HF), (700, 16, 4, 520, BF),
+                                               (40, 64, 9, 136, F32), (5000, 8, 3, 24, BF)])
+def test_dropped_choices_have_no_gradient(cuda, T, E, k, n, dtype):
+    """Slots set to -1 leave rows without a choice: their dy is zero, not what the memory held."""
+    torch.manual_seed(T)
+    w, r = S.route_topk(torch.randn(T, E, device='cuda'), k)
+    slots = torch.where(torch.rand(T, k, device='cuda') < 0.3, -1, r.slots)
+    slots[0, 0] = -1
+    own = S.Routing(r.experts, slots, r.rows, r.offsets)
+    y, d = (torch.randn(s, n, device='cuda').to(dtype) for s in (T * k, T))
+    hold = torch.full((T * k, n), float('nan'), device='cuda', dtype=dtype)     # what new_empty may find
+    del hold
+    dy, dw = S.route_combine_backward(d, y, own, w)
+    kept = slots >= 0
+    want = torch.zeros(T * k, n, device='cuda', dtype=torch.float64)
+    want[slots[kept].long()] = (w.double()[:, :, None] * d.double()[:, None, :])[kept]
+    assert ((dy.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + STEP) * want.abs() + 2.0 ** -25).all()
+    assert not dw[~kept].any()
+    out = S.route_combine(y, own, w)
+    part = torch.where(kept[:, :, None], y.double()[slots.clamp(min=0).long()] * w.double()[:, :, None], 0.0)
+    lim = (k + 2) * STEP * part.abs().sum(1) + torch.finfo(dtype).eps / 2 * part.sum(1).abs() + 2.0 ** -25
+    assert ((out.double() - part.sum(1)).abs() <= lim).all()
