@@ -102,13 +102,14 @@ __device__ __forceinline__ int64_t part_place(int64_t first, int64_t g) { return
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, const int16_t *slope, T *dz,
                                                  int64_t dz_ld, float *part, T *dbias, const int32_t *offsets,
-                                                 int64_t groups, int64_t rows, int64_t n) {
+                                                 int64_t groups, int64_t rows, int64_t n, uint32_t tiles) {
     chained_start();
     __shared__ float sums[8][kDzCols];
-    const RowTile t = find_row_tile(offsets, groups, rows, kDzRows, blockIdx.x);
+    const int64_t strip = (int64_t)(blockIdx.x / tiles) * kDzCols;     // its first column
+    const RowTile t = find_row_tile(offsets, groups, rows, kDzRows, blockIdx.x % tiles);
     if (t.group > groups || (offsets && t.group == groups)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c0 = (int64_t)blockIdx.y * kDzCols + lane * 8;
+    const int64_t c0 = strip + lane * 8;
     const int cols = c0 >= n ? 0 : n - c0 < 8 ? (int)(n - c0) : 8;
     float acc[8] = {};
     if (cols) {
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T *dy, int64_t dy_ld, con
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = acc[e];
     __syncthreads();
-    const int64_t c = (int64_t)blockIdx.y * kDzCols + threadIdx.x;
+    const int64_t c = strip + threadIdx.x;
     if (c < n) {
         float v = 0.f;
 #pragma unroll
@@ -369,7 +370,8 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
     const bool make_dz = p->slope && any && (p->dx || p->dw);
     const bool one_tile = p->dbias && any && tiles == 1 && !p->offsets;
     const bool parts = p->dbias && any && !one_tile, sums = p->dx && p->gather;
-    if (ceil_div(p->n, kDzCols) > 65535) return SPMM_EUNSUPPORTED;
+    const int64_t dz_blocks = tiles * ceil_div(p->n, kDzCols);
+    if ((make_dz || parts || one_tile) && dz_blocks > INT32_MAX) return SPMM_EUNSUPPORTED;
     Copies copies{};
     Operand x{}, dz{p->dy, p->dy_ld, 0};
     Weight w{};
@@ -428,10 +430,10 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
     SPMM_TRY(run_copies(copies, s));
     if (make_dz || parts || one_tile) {
         const bool vec = p->n % 8 == 0 && in_place(p->dy, p->dy_ld, 0, p->n) && (uintptr_t)p->slope % 16 == 0;
-        const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p->n, kDzCols));
         T *direct = one_tile ? (T *)p->dbias : nullptr;
-        SPMM_TRY(launch_chained(vec ? dz_kernel<T, true> : dz_kernel<T, false>, grid, 256, 0, s, 1, (const T *)p->dy,
-                                p->dy_ld, p->slope, dzp, dz.ld, part, direct, p->offsets, p->groups, p->rows, p->n));
+        SPMM_TRY(launch_chained(vec ? dz_kernel<T, true> : dz_kernel<T, false>, dim3((unsigned)dz_blocks), 256, 0, s, 1,
+                                (const T *)p->dy, p->dy_ld, p->slope, dzp, dz.ld, part, direct, p->offsets, p->groups,
+                                p->rows, p->n, (uint32_t)tiles));
     }
     if (p->dbias && p->n && !one_tile) {
         const dim3 grid((unsigned)ceil_div(p->n, 32), (unsigned)p->groups);

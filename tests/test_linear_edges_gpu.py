@@ -183,3 +183,35 @@ def test_a_grouping_written_again_before_the_backward_pass(cuda, which):
     offsets += 1
     with pytest.raises(RuntimeError, match='inplace'):
         y.sum().backward()
+
+
+@pytest.mark.parametrize('rows, grouped', [(2, False), (70, False), (70, True)])
+def test_gradients_of_very_wide_results(cuda, rows, grouped):
+    """More columns than 65,535 blocks of 256.  dy is 0 but in a first and a last strip, so that the sums over n have
+    600 terms; N in the bound counts those."""
+    torch.manual_seed(9)
+    k, n = 8, 65535 * 256 + 320
+    at = torch.cat((torch.arange(300), torch.arange(n - 300, n))).cuda()
+    x, w = normal(rows, k), normal(k, n, scale=k ** -0.5)
+    dy = torch.zeros(rows, n, device='cuda', dtype=BF)
+    dy[:, at] = normal(rows, 600)
+    y, slope = (S.grouped_matmul(x, w[None], int32(0, rows), activation='silu', return_slope=True) if grouped else
+                S.dense_matmul(x, w, activation='silu', return_slope=True))
+    dx, dw, db = (S.grouped_matmul_backward(dy, x, w[None], int32(0, rows), slope, bias=True) if grouped else
+                  S.dense_matmul_backward(dy, x, w, slope, bias=True))
+    dw, db = dw.reshape(k, n), db.reshape(n)
+    z = x.double() @ w[:, at].double()
+    s = torch.sigmoid(z)
+    d = s * (1 + z * (1 - s))
+    E = (k + 8) * STEP * (x.double().abs() @ w[:, at].double().abs())
+    dz = dy[:, at].double() * d
+    eb = dy[:, at].double().abs() * (2.0 ** -15 + 1.2 * E + 2.0 ** -20)
+    ez = eb + 2.0 ** -8 * (dz.abs() + eb)
+
+    def close(got, want, err):
+        assert ((got.double() - want).abs() <= err + 2.0 ** -8 * (want.abs() + err) + 2.0 ** -25).all()
+    wd = w[:, at].double().t()
+    close(dx, dz @ wd, (ez + (600 + 16) * STEP * dz.abs()) @ wd.abs())
+    close(dw[:, at], x.double().t() @ dz, x.double().abs().t() @ (ez + (rows + 8) * STEP * dz.abs()))
+    close(db[at], dz.sum(0), (eb + (rows + 8) * STEP * dz.abs()).sum(0))
+    assert not dw[:, 300:n - 300].any() and not db[300:n - 300].any()
