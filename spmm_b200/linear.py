@@ -185,6 +185,9 @@ def _check_xw(x, w, w_dim):
         raise ValueError(f'x has {x.shape[-1] if x.dim() else 0} columns, expected {w.shape[-2]}')
     if w.get_device() != x.get_device():
         raise ValueError('w must be on x\'s device')
+    if x.numel() >= 2**31 or w.numel() >= 2**31:
+        if max(w.shape) >= 2**31 or _rows(x) >= 2**31:
+            raise ValueError('rows, columns and features must be below 2**31')
 
 
 def _check_like(name, t, x, shape):

@@ -267,6 +267,8 @@ def _check_combine(y, routing, weights):
     if y.dtype not in _TYPES:
         raise TypeError(f'y must be float32, bfloat16 or float16, got {y.dtype}')
     check_routing(routing, y.device)
+    if y.numel() >= 2**31 - 1024 and max(y.shape) >= 2**31 - 1024:
+        raise ValueError('y must have less than 2**31 - 1024 rows and columns')
     if y.shape[0] != routing.rows.shape[0]:
         raise ValueError(f'y has {y.shape[0]} rows, the routing {routing.rows.shape[0]}')
     if weights.shape != routing.slots.shape or weights.dtype != torch.float32 or weights.device != y.device:

@@ -40,3 +40,23 @@ def dual(*shape, dtype=BF):
 def test_tangents_are_refused(call):
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match='tangent'):
         call()
+
+
+def many(*shape):
+    """A tensor of any size in one element."""
+    return torch.zeros(1, dtype=BF).expand(*shape)
+
+
+@pytest.mark.parametrize('call', [
+    lambda: S.dense_matmul(many(2**31, 8), rand(8, 6)),
+    lambda: S.dense_matmul(many(2**16, 2**15, 8), rand(8, 6)),
+    lambda: S.dense_matmul(rand(4, 8), many(8, 2**31)),
+    lambda: S.dense_matmul(many(4, 2**31), many(2**31, 8)),
+    lambda: S.dense_matmul_backward(many(4, 2**31), rand(4, 8), many(8, 2**31)),
+    lambda: S.grouped_matmul(rand(8, 8), many(3, 8, 2**31), torch.zeros(4, dtype=torch.int32)),
+    lambda: S.route_combine(many(8, 2**31), routing(), torch.zeros(4, 2)),
+    lambda: S.route_combine_backward(many(4, 2**31 - 1024), many(8, 2**31 - 1024), routing(), torch.zeros(4, 2)),
+])
+def test_sizes_past_the_limit_are_refused(call):
+    with pytest.raises(ValueError, match=r'below 2\*\*31|less than 2\*\*31'):
+        call()
