@@ -372,7 +372,9 @@ int spmm_hem_hierarchy(int64_t rows, int64_t cols, const int64_t *indptr, const 
  * zero included; groups <= SPMM_MAX_GROUPS.  Strides are in elements; x, y,
  * residual, dy, dx have unit stride along their columns, w and dw along k or
  * along n.  16-byte aligned operands whose strides are multiples of 8 are read
- * in place; others are copied into the workspace first. */
+ * in place; others are copied into the workspace first.  These entries return
+ * SPMM_EALIGN for a pointer that is not aligned to its elements, or a workspace
+ * that is not aligned as said. */
 enum spmm_dense_type { SPMM_DENSE_F32 = 0, SPMM_DENSE_BF16 = 2, SPMM_DENSE_F16 = 3 };
 enum spmm_activation { SPMM_ACT_NONE = 0, SPMM_ACT_RELU = 1, SPMM_ACT_GELU = 2 /* erf */,
                        SPMM_ACT_GELU_TANH = 3, SPMM_ACT_SILU = 4 };
@@ -442,7 +444,7 @@ typedef struct {
     int32_t *offsets;           /* [experts + 1] */
     const float *dweights;      /* backward: [tokens][top]; reads logits and experts_out */
     void *dlogits;              /* backward: [tokens][experts] contiguous */
-    void *workspace;
+    void *workspace;            /* device scratch, 16-byte aligned, spmm_route_workspace_size() bytes */
     uint64_t workspace_bytes;
 } spmm_route_args;
 size_t spmm_route_workspace_size(const spmm_route_args *p);

@@ -252,6 +252,9 @@ int check_sizes(const spmm_linear *p) {
     if (!p->gather && p->x_rows != p->rows) return SPMM_EINVAL;
     if ((p->wait_us != 0 && p->wait_us < 1000) || (p->flags & ~SPMM_CFG_EXPIRE_FIRST_WAIT)) return SPMM_EINVAL;
     if (p->w_k != 1 && p->w_n != 1) return SPMM_EUNSUPPORTED;
+    if (!on_boundary(2, {p->x, p->w, p->bias, p->residual, p->y, p->slope, p->dy, p->dx, p->dw, p->dbias}) ||
+        !on_boundary(4, {p->offsets, p->gather, p->slots, p->status}) || !on_boundary(256, {p->workspace}))
+        return SPMM_EALIGN;
     return SPMM_OK;
 }
 

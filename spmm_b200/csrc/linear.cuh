@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace spmm {
@@ -35,6 +37,13 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     uint4 v;
     memcpy(&v, t, 16);
     return v;
+}
+
+// Whether every pointer (null too) lies on a boundary of `bytes`, a power of two.
+inline bool on_boundary(size_t bytes, std::initializer_list<const void *> pointers) {
+    uintptr_t all = 0;
+    for (const void *p : pointers) all |= (uintptr_t)p;
+    return (all & (bytes - 1)) == 0;
 }
 
 // First row of group g (offsets clamped into [0, total], so a wrong table reads and writes nothing outside; the

@@ -663,6 +663,10 @@ int check_route(const spmm_route_args *p) {
     if (p->experts > kMaxExperts || p->top > SPMM_MAX_TOP || p->tokens > INT32_MAX / p->top)
         return SPMM_EUNSUPPORTED;
     if (p->scoring != SPMM_SCORE_SOFTMAX && p->scoring != SPMM_SCORE_SIGMOID) return SPMM_EINVAL;
+    if (!on_boundary(p->dtype == SPMM_DENSE_F32 ? 4 : 2, {p->logits, p->dlogits}) ||
+        !on_boundary(4, {p->bias, p->weights, p->experts_out, p->slots, p->rows, p->offsets, p->dweights}) ||
+        !on_boundary(16, {p->workspace}))
+        return SPMM_EALIGN;
     return SPMM_OK;
 }
 
@@ -727,6 +731,9 @@ int check_combine(const spmm_combine_args *p) {
         return SPMM_EUNSUPPORTED;
     if (p->tokens < 0 || p->top < 1 || p->rows < 0 || p->n < 0) return SPMM_EINVAL;
     if (p->rows > INT32_MAX || p->top > INT32_MAX) return SPMM_EUNSUPPORTED;
+    if (!on_boundary(p->dtype == SPMM_DENSE_F32 ? 4 : 2, {p->y, p->residual, p->out, p->dout, p->dy}) ||
+        !on_boundary(4, {p->slots, p->offsets, p->weights, p->dweights}))
+        return SPMM_EALIGN;
     return SPMM_OK;
 }
 
@@ -801,6 +808,7 @@ extern "C" int spmm_combine(const spmm_combine_args *p, spmm_stream_t stream) {
 
 extern "C" int spmm_combine_backward_rows(const spmm_combine_args *p, const int32_t *tokens_of, spmm_stream_t stream) {
     SPMM_TRY(check_combine(p));
+    if (!on_boundary(4, {tokens_of})) return SPMM_EALIGN;
     if (!p->dy && !p->dweights) return SPMM_OK;
     if (p->tokens && (!p->slots || !p->weights || (p->n && (!p->dout || (p->rows && !p->y))))) return SPMM_EINVAL;
     if (p->dy && (!p->offsets || p->experts < 0)) return SPMM_EINVAL;
