@@ -215,3 +215,22 @@ def test_gradients_of_very_wide_results(cuda, rows, grouped):
     close(dw[:, at], x.double().t() @ dz, x.double().abs().t() @ (ez + (rows + 8) * STEP * dz.abs()))
     close(db[at], dz.sum(0), (eb + (rows + 8) * STEP * dz.abs()).sum(0))
     assert not dw[:, 300:n - 300].any() and not db[300:n - 300].any()
+
+
+@pytest.mark.parametrize('t, k, n', [(70000, 32768, 16), (70000, 16, 32768)])
+@pytest.mark.parametrize('w_t', [False, True])
+def test_weight_gradients_of_operands_past_32_bits(cuda, t, k, n, w_t):
+    """x or dy of more than 2**31 values, summed over all rows; dy is 0 but in three strips, so that the sum has 210
+    terms, the bound that of 210, and a strip that is lost or read elsewhere shows."""
+    torch.manual_seed(k)
+    at = torch.cat([torch.arange(a, a + 70) for a in (0, 65500, t - 70)]).cuda()
+    x = torch.empty(t, k, device='cuda', dtype=BF).normal_()
+    w = normal(n, k, scale=k ** -0.5).t() if w_t else normal(k, n, scale=k ** -0.5)
+    dy = torch.zeros(t, n, device='cuda', dtype=BF)
+    dy[at] = normal(210, n)
+    dw, db = S.dense_matmul_backward(dy, x, w, None, bias=True)[1:]
+    xs, ds = x[at].double(), dy[at].double()
+    want, size = xs.t() @ ds, xs.abs().t() @ ds.abs()
+    assert ((dw.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * (210 + 8) * STEP * size + 2.0 ** -25).all()
+    want, size = ds.sum(0), ds.abs().sum(0)
+    assert ((db.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * (210 + 8) * STEP * size + 2.0 ** -25).all()
