@@ -118,31 +118,36 @@ def _forward(x, w, g, bias, residual, activation, want_slope):
     return y, slope, status
 
 
-def _backward(dy, x, w, g, slope, need_dx, need_dw, need_dbias):
-    x, dy = _unit_rows(x), _unit_rows(dy)
+def _backward(dy, x, x_rows, w, g, slope, need_dx, need_dw, need_dbias):
+    """x is needed for dw alone, None without it."""
+    dy = _unit_rows(dy)
     w, (sk, sn, sg) = _w_strides(w)
     k, n = w.shape[-2:]
-    with on_device(x.device):
+    x_ptr, x_ld = 0, k
+    if x is not None:
+        x = _unit_rows(x)
+        x_ptr, x_ld = x.data_ptr(), x.stride(0)
+    with on_device(dy.device):
         dx = dw = dbias = None
         dw_k = dw_n = 0
         if need_dx:
-            dx = x.new_empty(x.shape)
+            dx = dy.new_empty((x_rows, k))
         if need_dw:
             lead = w.shape[:-2]
             if sn == 1:
-                dw = x.new_empty(lead + (k, n))
+                dw = dy.new_empty(lead + (k, n))
                 dw_k, dw_n = max(n, 1), 1
             else:
-                dw = x.new_empty(lead + (n, k)).transpose(-2, -1)
+                dw = dy.new_empty(lead + (n, k)).transpose(-2, -1)
                 dw_k, dw_n = 1, max(k, 1)
         if need_dbias:
-            dbias = x.new_empty(w.shape[:-2] + (n,))
+            dbias = dy.new_empty(w.shape[:-2] + (n,))
         status = _call('spmm_linear_backward', (
-            1, _TYPES[x.dtype], 0, 0, 0, 0, g.rows, k, n, g.count, x.shape[0], *g.pointers(),
-            x.data_ptr(), w.data_ptr(), 0, 0, 0, 0 if slope is None else slope.data_ptr(), dy.data_ptr(),
+            1, _TYPES[dy.dtype], 0, 0, 0, 0, g.rows, k, n, g.count, x_rows, *g.pointers(),
+            x_ptr, w.data_ptr(), 0, 0, 0, 0 if slope is None else slope.data_ptr(), dy.data_ptr(),
             0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
-            0 if dbias is None else dbias.data_ptr(), x.stride(0), sk, sn, sg, 0, 0, 0, dy.stride(0), k, dw_k, dw_n,
-            k * n, n), x, 'matmul_backward', slope is not None or g.gather is not None or (k | n) % 8 != 0)
+            0 if dbias is None else dbias.data_ptr(), x_ld, sk, sn, sg, 0, 0, 0, dy.stride(0), k, dw_k, dw_n,
+            k * n, n), dy, 'matmul_backward', slope is not None or g.gather is not None or (k | n) % 8 != 0)
     for t in (dx, dw, dbias):
         if t is not None:
             t._spmm_status = status
@@ -152,10 +157,12 @@ def _backward(dy, x, w, g, slope, need_dx, need_dw, need_dbias):
 class _MatMul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, activation, g):
-        y, slope, status = _forward(x, w, g, bias, residual, activation, True)
+        need = ctx.needs_input_grad
+        y, slope, status = _forward(x, w, g, bias, residual, activation, need[0] or need[1] or need[2])
         # the grouping too, so that writing it again before the backward pass is an error
-        ctx.save_for_backward(x, w, slope, g.offsets, g.gather, g.slots)
+        ctx.save_for_backward(x if need[1] else None, w, slope, g.offsets, g.gather, g.slots)
         ctx.counts = g.rows, g.count
+        ctx.x_rows = x.shape[0]
         ctx.mark_non_differentiable(status)
         ctx.set_materialize_grads(False)      # or the status would come back as a tensor of zeros
         return y, status
@@ -167,7 +174,7 @@ class _MatMul(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if dy is not None and (need[0] or need[1] or need[2]):
-            dx, dw, db = _backward(dy, x, w, _Groups(*groups, *ctx.counts), slope, need[0], need[1], need[2])
+            dx, dw, db = _backward(dy, x, ctx.x_rows, w, _Groups(*groups, *ctx.counts), slope, *need[:3])
         return dx, dw, db, dy if need[3] else None, None, None
 
 
@@ -279,8 +286,9 @@ def dense_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, sl
     need_cuda(x, 'x')
     g = _Groups(None, None, None, rows, 1)
     if x.dim() == 2:
-        return _backward(dy, x, w, g, slope, True, True, bias)
-    dx, dw, db = _backward(dy.reshape(rows, w.shape[1]), x.reshape(rows, x.shape[-1]), w, g, slope, True, True, bias)
+        return _backward(dy, x, x.shape[0], w, g, slope, True, True, bias)
+    dx, dw, db = _backward(dy.reshape(rows, w.shape[1]), x.reshape(rows, x.shape[-1]), rows, w, g, slope, True, True,
+                           bias)
     status = dx._spmm_status
     dx = dx.reshape(x.shape)
     dx._spmm_status = status
@@ -358,4 +366,4 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     if forward_ad._current_level >= 0:
         refuse_tangents(dy=dy, x=x, w=w)
     need_cuda(x, 'x')
-    return _backward(dy, x, w, g, slope, True, True, bias)
+    return _backward(dy, x, x.shape[0], w, g, slope, True, True, bias)

@@ -237,7 +237,8 @@ def _combine_backward(dout, y, slots, offsets, rows, weights, need_dy=True, need
                         offsets.data_ptr(), weights.data_ptr(), y.data_ptr(), 0, 0, dout.data_ptr(),
                         dy.data_ptr() if need_dy else 0, dw.data_ptr() if need_dweights else 0, y.stride(0), 0, 0,
                         dout.stride(0), n)
-        _lib.check(_lib.lib().spmm_combine_backward_rows(args, rows.data_ptr(), stream_handle(y.device)), 'route_combine_backward')
+        _lib.check(_lib.lib().spmm_combine_backward_rows(args, rows.data_ptr(), stream_handle(y.device)),
+                   'route_combine_backward')
     return dy, dw
 
 

@@ -234,3 +234,31 @@ def test_weight_gradients_of_operands_past_32_bits(cuda, t, k, n, w_t):
     assert ((dw.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * (210 + 8) * STEP * size + 2.0 ** -25).all()
     want, size = ds.sum(0), ds.abs().sum(0)
     assert ((db.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * (210 + 8) * STEP * size + 2.0 ** -25).all()
+
+
+def test_autograd_keeps_what_its_gradients_read(cuda):
+    """Frozen weights: x is not kept and may be written again; a residual alone needs no slope."""
+    x, w, b, r, dy = normal(64, 48), normal(48, 80), normal(80), normal(64, 80), normal(64, 80)
+    kept = []
+
+    def apply(*args):
+        kept.clear()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.data_ptr()) or t, lambda t: t):
+            return S.dense_matmul(*args, activation='silu')
+    xl = x.clone().requires_grad_()
+    y = apply(xl, w, b)
+    assert xl.data_ptr() not in kept and len(kept) == 2
+    _, slope = S.dense_matmul(x, w, b, activation='silu', return_slope=True)
+    want = S.dense_matmul_backward(dy, x, w, slope)
+    with torch.no_grad():
+        xl.zero_()
+    assert torch.equal(torch.autograd.grad(y, xl, dy)[0], want[0])
+    wl = w.clone().requires_grad_()
+    y = apply(x, wl, b)
+    assert x.data_ptr() in kept and torch.equal(torch.autograd.grad(y, wl, dy)[0], want[1])
+    bl = b.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(apply(x, w, bl), bl, dy)[0],
+                       S.dense_matmul_backward(dy, x, w, slope, bias=True)[2])
+    rl = r.clone().requires_grad_()
+    y = apply(x, w, b, rl)
+    assert len(kept) == 1 and torch.equal(torch.autograd.grad(y, rl, dy)[0], dy)
