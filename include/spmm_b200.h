@@ -379,13 +379,15 @@ enum spmm_dense_type { SPMM_DENSE_F32 = 0, SPMM_DENSE_BF16 = 2, SPMM_DENSE_F16 =
 enum spmm_activation { SPMM_ACT_NONE = 0, SPMM_ACT_RELU = 1, SPMM_ACT_GELU = 2 /* erf */,
                        SPMM_ACT_GELU_TANH = 3, SPMM_ACT_SILU = 4 };
 enum { SPMM_MAX_GROUPS = 1024, SPMM_MAX_TOP = 32 };
+/* spmm_linear::flags: *status is not set to 0 first, so that one word speaks for several calls. */
+enum { SPMM_LINEAR_KEEP_STATUS = 2 };
 
 typedef struct {
     int32_t version;            /* 1 */
     int32_t dtype;              /* enum spmm_dense_type: BF16 or F16 */
     int32_t activation;         /* enum spmm_activation (forward) */
     int32_t wait_us;            /* bounded device waits: 0 = about 2 s, else at least 1000 */
-    int32_t flags;              /* 0, or SPMM_CFG_EXPIRE_FIRST_WAIT (tests of the timeout path) */
+    int32_t flags;              /* SPMM_CFG_EXPIRE_FIRST_WAIT (tests of the timeout path), SPMM_LINEAR_KEEP_STATUS */
     int32_t reserved;           /* 0 */
     int64_t rows, k, n, groups; /* rows of y */
     int64_t x_rows;             /* rows of x (== rows without gather) */

@@ -99,6 +99,7 @@ def launch_cfg(engine: str = 'auto', workspace: int = 0, workspace_bytes: int = 
 
 DENSE_F32, DENSE_BF16, DENSE_F16 = 0, 2, 3
 MAX_GROUPS, MAX_TOP = 1024, 32
+LINEAR_KEEP_STATUS = 2
 
 
 class Linear(C.Structure):

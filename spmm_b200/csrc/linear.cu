@@ -250,7 +250,8 @@ int check_sizes(const spmm_linear *p) {
         return SPMM_EUNSUPPORTED;
     if (!p->offsets && p->groups != 1) return SPMM_EINVAL;
     if (!p->gather && p->x_rows != p->rows) return SPMM_EINVAL;
-    if ((p->wait_us != 0 && p->wait_us < 1000) || (p->flags & ~SPMM_CFG_EXPIRE_FIRST_WAIT)) return SPMM_EINVAL;
+    if ((p->wait_us != 0 && p->wait_us < 1000) || (p->flags & ~(SPMM_CFG_EXPIRE_FIRST_WAIT | SPMM_LINEAR_KEEP_STATUS)))
+        return SPMM_EINVAL;
     if (p->w_k != 1 && p->w_n != 1) return SPMM_EUNSUPPORTED;
     if (!on_boundary(2, {p->x, p->w, p->bias, p->residual, p->y, p->slope, p->dy, p->dx, p->dw, p->dbias}) ||
         !on_boundary(4, {p->offsets, p->gather, p->slots, p->status}) || !on_boundary(256, {p->workspace}))
@@ -328,7 +329,7 @@ int settle(const Arena &a, bool sizing, size_t &need) {
 }
 
 int forward(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStream_t s) {
-    const bool probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
+    const bool probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT, clear = !(p->flags & SPMM_LINEAR_KEEP_STATUS);
     Copies copies{};
     const Weight w = carve_w(p, a, copies);
     Product g = base(p);
@@ -361,14 +362,15 @@ int forward(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStrea
     SPMM_TRY(plan_product(g, probe, a, plan));
     SPMM_TRY(settle(a, sizing, need));
     if (sizing) return SPMM_OK;
-    if (p->status && !plan.launches) SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
+    if (p->status && clear && !plan.launches) SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
     SPMM_TRY(run_copies(copies, s));
-    return run_product(g, plan, true, probe, s);
+    return run_product(g, plan, clear, probe, s);
 }
 
 template <typename T>
 int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStream_t s) {
     const bool any = p->rows > 0 && p->n > 0, probe = p->flags & SPMM_CFG_EXPIRE_FIRST_WAIT;
+    const bool clear = !(p->flags & SPMM_LINEAR_KEEP_STATUS);
     const int64_t tiles = ceil_div(p->rows, kDzRows) + (p->offsets ? p->groups + 1 : 0);
     const bool make_dz = p->slope && any && (p->dx || p->dw);
     const bool one_tile = p->dbias && any && tiles == 1 && !p->offsets;
@@ -428,7 +430,7 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
     }
     SPMM_TRY(settle(a, sizing, need));
     if (sizing) return SPMM_OK;
-    if (p->status && !px.launches && !pw.launches)
+    if (p->status && clear && !px.launches && !pw.launches)
         SPMM_CUDA_TRY(cudaMemsetAsync(p->status, 0, sizeof(int32_t), s));
     SPMM_TRY(run_copies(copies, s));
     if (make_dz || parts || one_tile) {
@@ -443,10 +445,10 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
         SPMM_TRY(launch_chained(dbias_kernel<T>, grid, 256, 0, s, 1, part, p->offsets, any ? p->rows : 0, p->n,
                                 (T *)p->dbias, p->dbias_g));
     }
-    SPMM_TRY(run_product(gx, px, true, probe, s));
+    SPMM_TRY(run_product(gx, px, clear, probe, s));
     if (sums)
         SPMM_TRY(launch_gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, p->dx, p->dx_ld, gx.f16, s));
-    return run_product(gw, pw, !px.launches, probe, s);
+    return run_product(gw, pw, clear && !px.launches, probe, s);
 }
 
 int backward(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStream_t s) {

@@ -8,7 +8,8 @@ are the gradients as plain calls.  Not in the reference.
 
 Operands are bfloat16 or float16, sums float32, every output is rounded once.
 No call waits for the GPU; like ``boo_matmul``'s, a result carries the status
-of its bounded device waits (``product_status(y)``, ``check_product(y)``).
+of its bounded device waits (``product_status(y)``, ``check_product(y)``), and
+after a backward pass through autograd that of its gradients' waits as well.
 """
 
 from __future__ import annotations
@@ -71,14 +72,15 @@ class _Groups:
         return self.offsets.data_ptr(), self.gather.data_ptr(), self.slots.data_ptr(), self.slots.shape[1]
 
 
-def _call(name, fixed, x, where, scratch):
-    """Runs a C entry on x's device and stream; returns the call's status word.  Where `scratch` says that a
+def _call(name, fixed, x, where, scratch, word=None):
+    """Runs a C entry on x's device and stream; returns the call's status word (`word`, or a new one).  Where `scratch` says that a
     workspace is likely its size is asked for first; a call that needs one after all says so before it does
     anything and is repeated with it."""
     L = _lib.lib()
     run = getattr(L, name)
     stream = stream_handle(x.device)
-    word = x.new_empty(2)                       # 4 bytes
+    if word is None:
+        word = x.new_empty(2)                   # 4 bytes
     rc = _lib.SPMM_EWORKSPACE
     if not scratch:
         rc = run(_PACK(*fixed, 0, 0, word.data_ptr()), stream)
@@ -118,8 +120,8 @@ def _forward(x, w, g, bias, residual, activation, want_slope):
     return y, slope, status
 
 
-def _backward(dy, x, x_rows, w, g, slope, need_dx, need_dw, need_dbias):
-    """x is needed for dw alone, None without it."""
+def _backward(dy, x, x_rows, w, g, slope, need_dx, need_dw, need_dbias, word=None):
+    """x is needed for dw alone, None without it.  `word`: a status word that keeps what it says already."""
     dy = _unit_rows(dy)
     w, (sk, sn, sg) = _w_strides(w)
     k, n = w.shape[-2:]
@@ -143,11 +145,12 @@ def _backward(dy, x, x_rows, w, g, slope, need_dx, need_dw, need_dbias):
         if need_dbias:
             dbias = dy.new_empty(w.shape[:-2] + (n,))
         status = _call('spmm_linear_backward', (
-            1, _TYPES[dy.dtype], 0, 0, 0, 0, g.rows, k, n, g.count, x_rows, *g.pointers(),
+            1, _TYPES[dy.dtype], 0, 0, 0 if word is None else _lib.LINEAR_KEEP_STATUS, 0, g.rows, k, n, g.count, x_rows, *g.pointers(),
             x_ptr, w.data_ptr(), 0, 0, 0, 0 if slope is None else slope.data_ptr(), dy.data_ptr(),
             0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
             0 if dbias is None else dbias.data_ptr(), x_ld, sk, sn, sg, 0, 0, 0, dy.stride(0), k, dw_k, dw_n,
-            k * n, n), dy, 'matmul_backward', slope is not None or g.gather is not None or (k | n) % 8 != 0)
+            k * n, n), dy, 'matmul_backward', slope is not None or g.gather is not None or (k | n) % 8 != 0,
+            word)
     for t in (dx, dw, dbias):
         if t is not None:
             t._spmm_status = status
@@ -160,7 +163,7 @@ class _MatMul(torch.autograd.Function):
         need = ctx.needs_input_grad
         y, slope, status = _forward(x, w, g, bias, residual, activation, need[0] or need[1] or need[2])
         # the grouping too, so that writing it again before the backward pass is an error
-        ctx.save_for_backward(x if need[1] else None, w, slope, g.offsets, g.gather, g.slots)
+        ctx.save_for_backward(x if need[1] else None, w, slope, status, g.offsets, g.gather, g.slots)
         ctx.counts = g.rows, g.count
         ctx.x_rows = x.shape[0]
         ctx.mark_non_differentiable(status)
@@ -170,11 +173,12 @@ class _MatMul(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _):
-        x, w, slope, *groups = ctx.saved_tensors
+        x, w, slope, status, *groups = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if dy is not None and (need[0] or need[1] or need[2]):
-            dx, dw, db = _backward(dy, x, ctx.x_rows, w, _Groups(*groups, *ctx.counts), slope, *need[:3])
+            dx, dw, db = _backward(dy, x, ctx.x_rows, w, _Groups(*groups, *ctx.counts), slope, *need[:3],
+                                   word=status)   # y speaks for its gradients too
         return dx, dw, db, dy if need[3] else None, None, None
 
 

@@ -167,7 +167,8 @@ def test_autograd_allocates_what_the_plain_call_does(cuda):
     _, slope = S.dense_matmul(x, w, b, activation='silu', return_slope=True)
     plain = allocations(lambda: S.dense_matmul_backward(dy, x, w, slope, bias=True))
     y = S.dense_matmul(*leaves, activation='silu')
-    assert allocations(lambda: torch.autograd.grad(y, leaves, dy)) == plain
+    # one less: the forward pass's status word speaks for the backward pass too
+    assert allocations(lambda: torch.autograd.grad(y, leaves, dy)) == plain - 1
 
 
 @pytest.mark.parametrize('which', ['offsets', 'rows', 'slots'])
@@ -247,7 +248,7 @@ def test_autograd_keeps_what_its_gradients_read(cuda):
             return S.dense_matmul(*args, activation='silu')
     xl = x.clone().requires_grad_()
     y = apply(xl, w, b)
-    assert xl.data_ptr() not in kept and len(kept) == 2
+    assert xl.data_ptr() not in kept and len(kept) == 3     # w, the slopes, the status
     _, slope = S.dense_matmul(x, w, b, activation='silu', return_slope=True)
     want = S.dense_matmul_backward(dy, x, w, slope)
     with torch.no_grad():
@@ -261,4 +262,38 @@ def test_autograd_keeps_what_its_gradients_read(cuda):
                        S.dense_matmul_backward(dy, x, w, slope, bias=True)[2])
     rl = r.clone().requires_grad_()
     y = apply(x, w, b, rl)
-    assert len(kept) == 1 and torch.equal(torch.autograd.grad(y, rl, dy)[0], dy)
+    assert len(kept) == 2 and torch.equal(torch.autograd.grad(y, rl, dy)[0], dy)
+
+
+def test_an_expired_wait_of_the_backward_pass_is_reported(cuda, monkeypatch):
+    """A wait that nothing ends runs out in a backward pass through autograd: the product's result says so."""
+    from spmm_b200 import linear as L
+    x, w = normal(300, 256).requires_grad_(), normal(256, 512).requires_grad_()
+    y = S.dense_matmul(x, w)
+    assert S.product_status(y) == 0
+    pack = L._PACK
+
+    def short(version, dtype, act, wait_us, flags, *rest):
+        return pack(version, dtype, act, 2000, flags | _lib.SPMM_CFG_EXPIRE_FIRST_WAIT, *rest)
+    monkeypatch.setattr(L, '_PACK', short)
+    y.backward(torch.ones_like(y), retain_graph=True)
+    monkeypatch.setattr(L, '_PACK', pack)
+    assert S.product_status(y) == _lib.SPMM_ETIMEOUT
+    x.grad = w.grad = None
+    y.backward(torch.ones_like(y))            # the word keeps what it said; the gradients are right again
+    assert S.product_status(y) == _lib.SPMM_ETIMEOUT
+    want = S.dense_matmul_backward(torch.ones_like(y), x.detach(), w.detach())
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1]) and S.product_status(want[0]) == 0
+
+
+@pytest.mark.parametrize('rows', [1, 300, 0])
+def test_a_status_that_is_kept(cuda, rows):
+    x, w = normal(rows, 256), normal(256, 512)
+    y = torch.empty(rows, 512, device='cuda', dtype=BF)
+    for flags, want in ((_lib.LINEAR_KEEP_STATUS, 7), (0, 0)):
+        status = int32(7)
+        run('spmm_linear_forward', linear(rows, 256, 512, x=x, w=w, y=y, status=status, flags=flags))
+        assert int(status) == want
+        status, dx, dw = int32(7), torch.empty_like(x), torch.empty_like(w)
+        run('spmm_linear_backward', linear(rows, 256, 512, x=x, w=w, dy=y, dx=dx, dw=dw, status=status, flags=flags))
+        assert int(status) == want
