@@ -446,8 +446,8 @@ int gradients(const spmm_linear *p, Arena &a, bool sizing, size_t &need, cudaStr
                                 (T *)p->dbias, p->dbias_g));
     }
     SPMM_TRY(run_product(gx, px, clear, probe, s));
-    if (sums)
-        SPMM_TRY(launch_gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, p->dx, p->dx_ld, gx.f16, s));
+    if (sums && p->x_rows && p->k)
+        SPMM_TRY(gather_sum(dxs, p->rows, p->slots, p->x_rows, p->top, p->k, (T *)p->dx, p->dx_ld, s));
     return run_product(gw, pw, clear && !px.launches, probe, s);
 }
 
@@ -464,13 +464,6 @@ size_t sized(const spmm_linear *p, int (*run)(const spmm_linear *, Arena &, bool
 }
 
 }  // namespace
-
-int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,
-                      void *out, int64_t out_ld, int f16, cudaStream_t s) {
-    if (tokens == 0 || n == 0) return SPMM_OK;
-    return f16 ? gather_sum(src, rows, slots, tokens, top, n, (__half *)out, out_ld, s)
-               : gather_sum(src, rows, slots, tokens, top, n, (__nv_bfloat16 *)out, out_ld, s);
-}
 
 }  // namespace spmm
 

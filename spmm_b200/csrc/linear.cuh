@@ -261,8 +261,4 @@ int run_product(const Product &p, const ProductPlan &plan, bool clear, bool prob
 bool skinny_fits(const Product &p);
 int launch_skinny(const Product &p, bool clear, cudaStream_t s);
 
-// out[t] = sum_j weight * src[slots[t][j]] over float32 rows (the gradient of gathered rows).
-int launch_gather_sum(const float *src, int64_t rows, const int32_t *slots, int64_t tokens, int64_t top, int64_t n,
-                      void *out, int64_t out_ld, int f16, cudaStream_t s);
-
 }  // namespace spmm

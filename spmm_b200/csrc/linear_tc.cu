@@ -507,13 +507,7 @@ __device__ __forceinline__ void load_piece(uint8_t *stage, const T *base, int64_
     }
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    T e[2] = {from_f32<T>(a), from_f32<T>(b)};
-    uint32_t w;
-    memcpy(&w, e, 4);
-    return w;
-}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
