@@ -211,7 +211,9 @@ __device__ __forceinline__ float activate(float z, float &d) {
 
 // act'(z) in 16 bits.  It lies within (-2, 2), so fixed point in units of 2^-14
 // (off by at most 2^-15) keeps 4 to 30 times more of it than a 16-bit float
-// would; -32768 stands for NaN.  Adding 1.5 * 2^23 rounds to an integer in the
+// would near 1; a derivative below 2^-15 counts as 0, which moves dz by at most
+// 2^-15 of dy, less than its own rounding where the derivative is 2^-7 (bf16) or
+// 2^-4 (float16) or more.  -32768 stands for NaN.  Adding 1.5 * 2^23 rounds to an integer in the
 // low bits.
 __device__ __forceinline__ uint16_t slope_code(float s) {
     const uint32_t c = __float_as_uint(fmaf(s, 16384.f, 12582912.f));

@@ -6,7 +6,9 @@ block-diagonal matrix with ragged blocks, the products of a mixture of experts.
 Both are differentiable; ``dense_matmul_backward`` / ``grouped_matmul_backward``
 are the gradients as plain calls.  Not in the reference.
 
-Operands are bfloat16 or float16, sums float32, every output is rounded once.
+Operands are bfloat16 or float16, sums float32.  Every output is rounded once;
+dx and dw come from ``dz = dy * act'(z)``, which is rounded to the operands'
+type before (not without an activation).
 No call waits for the GPU; like ``boo_matmul``'s, a result carries the status
 of its bounded device waits (``product_status(y)``, ``check_product(y)``), and
 after a backward pass through autograd that of its gradients' waits as well.
@@ -336,8 +338,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, groups: Union[Routing, torc
     tokens [T, K] and row r reads token ``rows[r]``; without it x is [R, K] in
     grouped order.  Types, strides of w, differentiation and ``return_slope``
     as in ``dense_matmul``.  Offsets are read on the device and cannot be
-    checked here: a table that decreases or leaves [0, R] gives wrong values,
-    but reads and writes nothing outside the operands.
+    checked here: the first one counts as 0, and a table that decreases or
+    leaves [0, R] gives wrong values, but reads and writes nothing outside the
+    operands.
     """
     if activation not in _ACT:
         raise ValueError(f'activation must be one of {ACTIVATIONS}')
@@ -359,7 +362,8 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     """(dx, dw, dbias) of ``grouped_matmul``; dbias is None unless ``bias``.
 
     Empty groups get zeros, rows behind the last group a zero dx.  With
-    ``gather`` dx [T, K] sums over the rows that read the token, in float32.
+    ``gather`` dx [T, K] sums over the rows that the token's ``slots`` name, in
+    float32.
     """
     _check_xw(x, w, 3)
     if x.dim() != 2:

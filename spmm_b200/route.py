@@ -169,11 +169,15 @@ def route_topk(logits: torch.Tensor, top: int, *, scoring: str = 'softmax', reno
     experts with the largest ``float32(logit) + bias`` are chosen, best first,
     ties to the lowest index; an expert whose logit is -inf or NaN is never
     chosen, and a token without any left gets expert -1 with weight 0, so a
-    masked row takes no part.  ``bias`` [E] float32 moves the choice only.
+    masked row takes no part.  ``bias`` [E] float32 moves the choice only; it is
+    added to the logit with either scoring.  A router whose bias is added to the
+    sigmoid chooses other experts and is not this one.
 
     The weights [T, top] float32 are the chosen experts' softmax over all E
     logits (or their sigmoid), divided by their sum over the chosen ones with
-    ``renormalize``, times ``scale``.  Differentiable in ``logits``.
+    ``renormalize``, times ``scale``; a renormalised sigmoid whose logit is below
+    -709 (the type's lowest value as a mask) counts as 0.  Differentiable in
+    ``logits``.
     """
     _check_score(logits, scoring)
     tokens, experts = logits.shape
