@@ -406,12 +406,13 @@ def load_peaks():
 
 def csrc_sha16() -> str:
     """Hash of the CUDA sources of the sparse products and builders (spmm_b200/csrc without the dense, grouped
-    and routed products, which none of the workloads here runs)."""
+    and routed products, which none of the workloads here runs and no other source includes)."""
     import hashlib
     h = hashlib.sha256()
+    apart = ('linear.cu', 'linear.cuh', 'linear_skinny.cu', 'linear_tc.cu', 'route.cu')
     d = os.path.join(ROOT, 'spmm_b200', 'csrc')
     for f in sorted(os.listdir(d)):
-        if f.endswith(('.cu', '.cuh')) and not f.startswith(('linear', 'route')):
+        if f.endswith(('.cu', '.cuh')) and f not in apart:
             h.update(f.encode())
             h.update(open(os.path.join(d, f), 'rb').read())
     return h.hexdigest()[:16]
